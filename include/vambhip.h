@@ -483,8 +483,71 @@ int vh_vae_train_epoch_dp(vh_vae* h, const int64_t* perm, int64_t n_batches, int
                           const float* global_wsum, double loss_means[5]);
 
 
+/* =============================================================================================
+ * Low-rank adapters of many groups of rows beside a shared projection, and 8-bit activation checkpoints
+ * (no counterpart in the reference: a trained VAE corrected per sample of origin, vamb_amd/adapters.py).
+ *
+ *     u = x A_g^T    y = f(x W^T + b + scale u B_g^T)         f: identity or LeakyReLU, g: the row's group
+ *     p = dy f'(y)   v = scale p B_g   dx = p W + v A_g   dA_g = sum v^T x   dB_g = scale sum p^T u
+ *
+ * Unlike the handles above, these entry points take DEVICE pointers (of the calling thread's current device), enqueue on `stream`
+ * (a hipStream_t; NULL: the null stream) and return without synchronising; they allocate nothing, so that they may be captured
+ * into a graph.  Scratch memory is the caller's, of the size that the *_size entry gives; calls that may run at the same
+ * time need scratch of their own.  Tensors are float32 or bf16 (`dtype`), unit stride along a row, `ld*` elements between rows, any
+ * alignment of the element type.  Widths up to 2^20, rows up to 2^30, ranks up to 64, groups up to 16384.
+ * ============================================================================================= */
+enum { VH_F32 = 0, VH_BF16 = 1 };
 
+/* Rows sorted by group: which rows each adapter serves.  row_groups [rows]: a value outside [0, groups) is a row without an adapter.  The
+ * plan serves every call on the same rows (all layers of a pass, forward and backward), concurrent ones too. */
+int vh_rows_plan_size(int64_t rows, int64_t groups, int64_t* plan_words, int64_t* scratch_words);
+int vh_rows_plan(const int32_t* row_groups, int64_t rows, int64_t groups, int32_t* plan /* 16-byte aligned */, int32_t* scratch, void* stream);
 
+/* The shared weight [n][k] (row stride ld) and its bias [n] (or NULL), laid out once for both directions (16-byte aligned). */
+int vh_adapt_weight_size(int64_t n, int64_t k, int dtype, int64_t* bytes);
+int vh_adapt_weight_pack(const void* weight, int64_t ld, const void* bias, int64_t n, int64_t k, int dtype, void* packed, void* stream);
+
+typedef struct {
+    int32_t dtype;               /* of x, y, down, up, their gradients and the weight that was packed */
+    int32_t activation;          /* 0: f = identity, 1: LeakyReLU(negative_slope) */
+    int64_t n, k, rank, groups;
+    const void* packed;          /* vh_adapt_weight_pack */
+    const void* down;            /* A [groups][rank][k] */
+    const void* up;              /* B [groups][n][rank] */
+    float scale, negative_slope;
+} vh_adapt_layer;
+
+/* A tensor that waits for the backward pass: elements (data, ld), or a checkpoint (codes, exponents; data NULL).  A checkpoint of `cols`
+ * columns has ceil(cols / 32) * 32 codes (8-byte aligned) and ceil(cols / 32) exponents per row, dense.  code = e4m3 bits of x 2^-e, rounded to
+ * nearest even, e the least with the block's largest finite magnitude <= 448 * 2^e, in [-117, 120]; the exponent byte is
+ * e + 127; a code's sign bit is set iff x > 0 does not hold; a non-finite x is 0xff (NaN); at e = 120 the code's
+ * magnitude is at most 240 (256 * 2^120 is no float32).  Codes behind `cols` are 0x80. */
+typedef struct {
+    const void* data;
+    int64_t ld;
+    const uint8_t* codes;
+    const uint8_t* exponents;
+} vh_held;
+
+/* y [rows][ldy]; optional: low = u [rows][rank] and the checkpoint of y, for the backward pass */
+int vh_adapt_forward(const vh_adapt_layer* layer, const void* x, int64_t ldx, int64_t rows, const int32_t* plan, void* y, int64_t ldy, float* low,
+                     uint8_t* codes, uint8_t* exponents, void* stream);
+/* the same y for a few rows, in one launch without a plan (any number of rows is right; from about a hundred on the plan is faster) */
+int vh_adapt_forward_few(const vh_adapt_layer* layer, const void* x, int64_t ldx, int64_t rows, const int32_t* row_groups, void* y, int64_t ldy,
+                         void* stream);
+/* y (elements or checkpoint) may be NULL without an activation.  dx [rows][lddx] may be NULL (not wanted).  ddown, dup: dense, like
+ * down and up; a group without rows gets zeros.  The sums over a group's rows have one order: equal inputs give equal bits. */
+int vh_adapt_backward_size(int64_t rows, int64_t groups, int64_t n, int64_t k, int64_t rank, int64_t* scratch_words);
+int vh_adapt_backward(const vh_adapt_layer* layer, const void* dy, int64_t lddy, const vh_held* x, const vh_held* y, const float* low, int64_t rows,
+                      const int32_t* plan, void* dx, int64_t lddx, void* ddown, void* dup, float* scratch, void* stream);
+
+int vh_checkpoint8(const void* x, int64_t ld, int64_t rows, int64_t cols, int dtype, uint8_t* codes, uint8_t* exponents, void* stream);
+/* out [rows][cols], dense */
+int vh_checkpoint8_restore(const uint8_t* codes, const uint8_t* exponents, int64_t rows, int64_t cols, int dtype, void* out, void* stream);
+/* gradient of a projection whose input waited as a checkpoint: dweight = p^T x [n][k], dbias = sum p [n] (or NULL); y NULL: p = dy */
+int vh_checkpoint8_weight_grad_size(int64_t rows, int64_t n, int64_t k, int64_t* scratch_words);
+int vh_checkpoint8_weight_grad(const void* dy, int64_t lddy, const vh_held* x, const vh_held* y, float negative_slope, int64_t rows, int64_t n,
+                               int64_t k, int dtype, void* dweight, void* dbias, float* scratch, void* stream);
 
 #ifdef __cplusplus
 }

@@ -38,6 +38,16 @@ class ClusterInfo(ctypes.Structure):                                    # vh_clu
                 ("attempts_after", ctypes.c_int64), ("order_index_after", ctypes.c_int64)]
 
 
+class AdaptLayer(ctypes.Structure):                                     # vh_adapt_layer
+    _fields_ = [("dtype", ctypes.c_int32), ("activation", ctypes.c_int32), ("n", ctypes.c_int64), ("k", ctypes.c_int64),
+                ("rank", ctypes.c_int64), ("groups", ctypes.c_int64), ("packed", ctypes.c_void_p), ("down", ctypes.c_void_p),
+                ("up", ctypes.c_void_p), ("scale", ctypes.c_float), ("negative_slope", ctypes.c_float)]
+
+
+class Held(ctypes.Structure):                                           # vh_held
+    _fields_ = [("data", ctypes.c_void_p), ("ld", ctypes.c_int64), ("codes", ctypes.c_void_p), ("exponents", ctypes.c_void_p)]
+
+
 _lib = None
 
 _i64 = ctypes.c_int64
@@ -160,6 +170,19 @@ SIGNATURES = {
     "vh_vaevae_train_step": (_int, [_vp, _vp, _i64, _vp, _vp, _vp]),
     "vh_vaevae_train_epoch": (_int, [_vp, _vp, _i64, _i64, _vp]),
     "vh_vaevae_get_grad": (_int, [_vp, _int, ctypes.c_char_p, _vp, _i64]),
+    "vh_rows_plan_size": (_int, [_i64, _i64, ctypes.POINTER(_i64), ctypes.POINTER(_i64)]),
+    "vh_rows_plan": (_int, [_vp, _i64, _i64, _vp, _vp, _vp]),
+    "vh_adapt_weight_size": (_int, [_i64, _i64, _int, ctypes.POINTER(_i64)]),
+    "vh_adapt_weight_pack": (_int, [_vp, _i64, _vp, _i64, _i64, _int, _vp, _vp]),
+    "vh_adapt_forward": (_int, [ctypes.POINTER(AdaptLayer), _vp, _i64, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _vp]),
+    "vh_adapt_forward_few": (_int, [ctypes.POINTER(AdaptLayer), _vp, _i64, _i64, _vp, _vp, _i64, _vp]),
+    "vh_adapt_backward_size": (_int, [_i64, _i64, _i64, _i64, _i64, ctypes.POINTER(_i64)]),
+    "vh_adapt_backward": (_int, [ctypes.POINTER(AdaptLayer), _vp, _i64, ctypes.POINTER(Held), ctypes.POINTER(Held), _vp, _i64, _vp, _vp, _i64, _vp, _vp,
+                                 _vp, _vp]),
+    "vh_checkpoint8": (_int, [_vp, _i64, _i64, _i64, _int, _vp, _vp, _vp]),
+    "vh_checkpoint8_restore": (_int, [_vp, _vp, _i64, _i64, _int, _vp, _vp]),
+    "vh_checkpoint8_weight_grad_size": (_int, [_i64, _i64, _i64, ctypes.POINTER(_i64)]),
+    "vh_checkpoint8_weight_grad": (_int, [_vp, _i64, ctypes.POINTER(Held), ctypes.POINTER(Held), _f32, _i64, _i64, _i64, _int, _vp, _vp, _vp, _vp]),
 }
 
 

@@ -1,0 +1,401 @@
+"""Low-rank adapters of many samples beside a trained VAE's layers, and 8-bit activation checkpoints (``csrc/adapt*.hip``).
+
+One VAE is trained on the contigs of many samples (``vamb_amd.encode.VAE``); an adapter is a small correction of a layer for the
+contigs of ONE sample -- a batch effect of its library, its depth, its host.  A batch holds contigs of many samples, so every call
+serves all adapters at once.  With ``x [rows, k]``, the shared weight ``W [n, k]`` and bias ``b``, ``down = A [groups, rank, k]``, ``up = B
+[groups, n, rank]`` and the group ``g`` of a row (a row whose group is outside ``[0, groups)``, -1 say, has no adapter)::
+
+    u = x A_g^T     y = f(x W^T + b + scale u B_g^T)          f: identity, or LeakyReLU(negative_slope)
+    p = dy f'(y)    v = scale p B_g     dx = p W + v A_g      dA_g = sum v^T x     dB_g = scale sum p^T u     dW = p^T x     db = sum p
+
+What the backward pass needs of the forward pass waits as a :class:`Checkpoint8`: one byte per activation.
+
+The functions take and return tensors of one GPU (float32 or bfloat16, all tensors of a call in one type; ``u`` is always float32), run on the current
+stream of that GPU, do not synchronise and may be captured into a graph.  Memory comes from torch's allocator, so a tensor (a plan, a
+packed weight, a checkpoint) that is used on another stream than the one that made it has to be ordered as any other
+tensor has.  They stand outside of autograd: gradients come from :func:`adapted_linear_backward` and :func:`checkpoint_weight_grad`.
+Sums are float32; gradients have the type of their parameters.  Equal inputs give equal bits.
+
+:class:`VAEAdapters` trains adapters for a VAE's encoder and encodes with them.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from functools import lru_cache
+from typing import Optional, Union
+
+import torch as _torch
+
+from . import _lib
+
+MAX_RANK = 64
+MAX_GROUPS = 16384
+BLOCK = 32   # columns of a checkpoint that share an exponent
+# up to so many rows adapted_linear goes without a plan: one launch, W read once per 16 rows
+FEW_ROWS = 64
+
+_DTYPES = {_torch.float32: 0, _torch.bfloat16: 1}
+
+
+def _dtype_of(t: _torch.Tensor, what: str) -> int:
+    try:
+        return _DTYPES[t.dtype]
+    except KeyError:
+        raise ValueError(f"{what} must be float32 or bfloat16, not {t.dtype}") from None
+
+
+def _matrix(t, what: str, rows: Optional[int] = None, cols: Optional[int] = None) -> int:
+    """Check a [rows, cols] tensor whose rows are contiguous; returns its row stride."""
+    if not isinstance(t, _torch.Tensor) or t.dim() != 2:
+        raise ValueError(f"{what} must be a two-dimensional tensor")
+    if (rows is not None and t.shape[0] != rows) or (cols is not None and t.shape[1] != cols):
+        raise ValueError(f"{what} must be [{'rows' if rows is None else rows}, {'columns' if cols is None else cols}], not {list(t.shape)}")
+    if t.shape[1] > 1 and t.stride(1) != 1:
+        raise ValueError(f"the rows of {what} must be contiguous")
+    if t.shape[0] <= 1:
+        return t.shape[1]
+    if t.stride(0) < t.shape[1]:
+        raise ValueError(f"the rows of {what} overlap (row stride {t.stride(0)}, {t.shape[1]} columns)")
+    return t.stride(0)
+
+
+def _dense(t, what: str, shape) -> None:
+    if not isinstance(t, _torch.Tensor) or tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{what} must be {list(shape)}, not {list(getattr(t, 'shape', ()))}")
+    if not t.is_contiguous():
+        raise ValueError(f"{what} must be contiguous")
+
+
+class _On:
+    """The device of a call: checks that all tensors are there, makes it current for the library, gives its stream."""
+
+    __slots__ = ("device", "_before")
+
+    def __init__(self, first, *others):
+        self.device = first.device
+        if self.device.type != "cuda":
+            raise ValueError(f"the tensors must be on a GPU, not on {self.device}")
+        for t in others:
+            if t is not None and t.device != self.device:
+                raise ValueError(f"the tensors of a call must be on one device: {self.device} and {t.device}")
+
+    def __enter__(self):
+        self._before = _torch.cuda.current_device()
+        if self._before != self.device.index:
+            _torch.cuda.set_device(self.device)
+        return _torch.cuda.current_stream(self.device).cuda_stream
+
+    def __exit__(self, *exc):
+        if self._before != self.device.index:
+            _torch.cuda.set_device(self._before)
+        return False
+
+
+@lru_cache(maxsize=4096)
+def _plan_words(rows: int, groups: int):
+    a, b = ctypes.c_int64(), ctypes.c_int64()
+    _lib.check(_lib.load().vh_rows_plan_size(rows, groups, ctypes.byref(a), ctypes.byref(b)))
+    return a.value, b.value
+
+
+@lru_cache(maxsize=4096)
+def _backward_words(rows: int, groups: int, n: int, k: int, rank: int) -> int:
+    a = ctypes.c_int64()
+    _lib.check(_lib.load().vh_adapt_backward_size(rows, groups, n, k, rank, ctypes.byref(a)))
+    return a.value
+
+
+@lru_cache(maxsize=4096)
+def _weight_grad_words(rows: int, n: int, k: int) -> int:
+    a = ctypes.c_int64()
+    _lib.check(_lib.load().vh_checkpoint8_weight_grad_size(rows, n, k, ctypes.byref(a)))
+    return a.value
+
+
+# ---- which rows an adapter serves -----------------------------------------------------------------------------------------------
+class RowGroups:
+    """The rows of a batch sorted by group (:func:`group_rows`): made once per batch, read by every layer's forward and backward."""
+
+    __slots__ = ("rows", "groups", "plan")
+
+    def __init__(self, rows: int, groups: int, plan: Optional[_torch.Tensor]):
+        self.rows, self.groups, self.plan = rows, groups, plan
+
+
+def _check_groups(groups, n_groups: int) -> None:
+    if not isinstance(groups, _torch.Tensor) or groups.dim() != 1 or groups.dtype != _torch.int32:
+        raise ValueError("groups must be a one-dimensional int32 tensor (or what group_rows made of one)")
+    if not groups.is_contiguous():
+        raise ValueError("groups must be contiguous")
+    if not 1 <= n_groups <= MAX_GROUPS:
+        raise ValueError(f"the number of groups must be in [1, {MAX_GROUPS}], not {n_groups}")
+
+
+def group_rows(groups: _torch.Tensor, n_groups: int) -> RowGroups:
+    """Sort the rows of a batch by their group: ``groups`` int32 ``[rows]``; values outside ``[0, n_groups)`` are rows without an adapter."""
+    _check_groups(groups, n_groups)
+    rows = groups.shape[0]
+    if rows == 0:
+        return RowGroups(0, n_groups, None)
+    lib = _lib.load()
+    with _On(groups) as stream:
+        words, scratch_words = _plan_words(rows, n_groups)
+        plan = _torch.empty(words, dtype=_torch.int32, device=groups.device)
+        scratch = _torch.empty(scratch_words, dtype=_torch.int32, device=groups.device) if scratch_words else None
+        _lib.check(lib.vh_rows_plan(groups.data_ptr(), rows, n_groups, plan.data_ptr(), scratch.data_ptr() if scratch is not None else None, stream))
+    return RowGroups(rows, n_groups, plan)
+
+
+# ---- the shared projection ------------------------------------------------------------------------------------------------------
+class SharedProjection:
+    """``weight [n, k]`` and ``bias [n]`` of a layer that all adapters share, laid out once for both directions (a copy: later
+    changes of ``weight`` are not seen; make another)."""
+
+    def __init__(self, weight: _torch.Tensor, bias: Optional[_torch.Tensor] = None):
+        ld = _matrix(weight, "weight")
+        self.dtype = weight.dtype
+        code = _dtype_of(weight, "weight")
+        self.n, self.k = weight.shape
+        if self.n < 1 or self.k < 1:
+            raise ValueError("weight must not be empty")
+        if bias is not None:
+            _dense(bias, "bias", (self.n,))
+            if bias.dtype != weight.dtype:
+                raise ValueError(f"bias must have the weight's type {weight.dtype}, not {bias.dtype}")
+        self.device = weight.device
+        lib = _lib.load()
+        with _On(weight, bias) as stream:
+            size = ctypes.c_int64()
+            _lib.check(lib.vh_adapt_weight_size(self.n, self.k, code, ctypes.byref(size)))
+            self.packed = _torch.empty(size.value, dtype=_torch.uint8, device=weight.device)
+            _lib.check(lib.vh_adapt_weight_pack(weight.data_ptr(), ld, bias.data_ptr() if bias is not None else None, self.n, self.k, code,
+                                                self.packed.data_ptr(), stream))
+
+
+def _layer(shared, down, up, n_groups, scale, negative_slope):
+    """Check a layer's adapters and describe it to the library."""
+    if not isinstance(shared, SharedProjection):
+        raise ValueError("shared must be a SharedProjection")
+    if not isinstance(down, _torch.Tensor) or down.dim() != 3:
+        raise ValueError("down must be a tensor [groups, rank, k]")
+    groups, rank = down.shape[:2]
+    if groups != n_groups:
+        raise ValueError(f"down holds {groups} adapters, the rows' groups are {n_groups}")
+    if not 1 <= rank <= MAX_RANK:
+        raise ValueError(f"the rank must be in [1, {MAX_RANK}], not {rank}")
+    _dense(down, "down", (groups, rank, shared.k))
+    _dense(up, "up", (groups, shared.n, rank))
+    if down.dtype != shared.dtype or up.dtype != shared.dtype:
+        raise ValueError(f"down and up must have the weight's type {shared.dtype}, not {down.dtype} and {up.dtype}")
+    if not math.isfinite(scale):
+        raise ValueError(f"scale must be finite, not {scale}")
+    _check_slope(negative_slope)
+    return _lib.AdaptLayer(_DTYPES[shared.dtype], int(negative_slope is not None), shared.n, shared.k, rank, groups, shared.packed.data_ptr(),
+                           down.data_ptr(), up.data_ptr(), scale, 0.0 if negative_slope is None else negative_slope)
+
+
+def _check_slope(negative_slope) -> None:
+    if negative_slope is not None and not (0.0 <= negative_slope < math.inf):
+        raise ValueError(f"negative_slope must be finite and >= 0 (the derivative is read from the sign of the result), not {negative_slope}")
+
+
+def _input(x, shared) -> int:
+    if not isinstance(shared, SharedProjection):
+        raise ValueError("shared must be a SharedProjection")
+    ld = _matrix(x, "x", None, shared.k)
+    if x.dtype != shared.dtype:
+        raise ValueError(f"x must have the weight's type {shared.dtype}, not {x.dtype}")
+    return ld
+
+
+def adapted_linear(x, shared: SharedProjection, down, up, groups: Union[_torch.Tensor, RowGroups], scale: float = 1.0,
+                   negative_slope: Optional[float] = None) -> _torch.Tensor:
+    """``f(x W^T + b + scale u B_g^T)``, ``[rows, n]``: the layer with every row's own adapter.
+
+    ``groups``: an int32 tensor ``[rows]``, or the :class:`RowGroups` of these rows where several layers use it.  ``x`` may have any row stride."""
+    ld = _input(x, shared)
+    rows = x.shape[0]
+    planned = isinstance(groups, RowGroups)
+    n_groups = groups.groups if planned else (down.shape[0] if isinstance(down, _torch.Tensor) and down.dim() == 3 else 0)
+    layer = _layer(shared, down, up, n_groups, scale, negative_slope)
+    if not planned:
+        _check_groups(groups, n_groups)
+    if (groups.rows if planned else groups.shape[0]) != rows:
+        raise ValueError(f"x has {rows} rows, groups {groups.rows if planned else groups.shape[0]}")
+    lib = _lib.load()
+    with _On(x, shared.packed, down, up, groups.plan if planned else groups) as stream:
+        y = _torch.empty((rows, shared.n), dtype=x.dtype, device=x.device)
+        if rows == 0:
+            return y
+        if not planned and rows <= FEW_ROWS:
+            _lib.check(lib.vh_adapt_forward_few(layer, x.data_ptr(), ld, rows, groups.data_ptr(), y.data_ptr(), shared.n, stream))
+            return y
+        if not planned:
+            groups = group_rows(groups, n_groups)
+        _lib.check(lib.vh_adapt_forward(layer, x.data_ptr(), ld, rows, groups.plan.data_ptr(), y.data_ptr(), shared.n, None, None, None, stream))
+    return y
+
+
+def adapted_linear_train(x, shared: SharedProjection, down, up, groups: RowGroups, scale: float = 1.0, negative_slope: Optional[float] = None):
+    """``(y, u, checkpoint of y)``: :func:`adapted_linear` with what the backward pass needs -- the small product ``u [rows, rank]`` in
+    float32, and ``y`` as a :class:`Checkpoint8`, written by the same launch."""
+    ld = _input(x, shared)
+    rows = x.shape[0]
+    if not isinstance(groups, RowGroups):
+        raise ValueError("groups must come from group_rows")
+    layer = _layer(shared, down, up, groups.groups, scale, negative_slope)
+    if groups.rows != rows:
+        raise ValueError(f"x has {rows} rows, groups {groups.rows}")
+    lib = _lib.load()
+    with _On(x, shared.packed, down, up, groups.plan) as stream:
+        y = _torch.empty((rows, shared.n), dtype=x.dtype, device=x.device)
+        low = _torch.empty((rows, down.shape[1]), dtype=_torch.float32, device=x.device)
+        held = Checkpoint8._empty(rows, shared.n, x.device)
+        if rows:
+            _lib.check(lib.vh_adapt_forward(layer, x.data_ptr(), ld, rows, groups.plan.data_ptr(), y.data_ptr(), shared.n, low.data_ptr(),
+                                            held.codes.data_ptr(), held.exponents.data_ptr(), stream))
+    return y, low, held
+
+
+def adapted_linear_backward(dy, x, y, low, shared: SharedProjection, down, up, groups: RowGroups, scale: float = 1.0,
+                            negative_slope: Optional[float] = None, need_dx: bool = True):
+    """``(dx, ddown, dup)`` of :func:`adapted_linear_train`; ``dx`` is None with ``need_dx=False`` (a first layer).
+
+    ``x`` and ``y`` are the layer's input and output, as tensors or checkpoints (``y`` may be None without an activation: it gives
+    the derivative); ``low`` is its ``u``.  The gradients of a group without rows are zero."""
+    if not isinstance(groups, RowGroups):
+        raise ValueError("groups must come from group_rows")
+    layer = _layer(shared, down, up, groups.groups, scale, negative_slope)
+    ld = _matrix(dy, "dy", groups.rows, shared.n)
+    rows, rank = groups.rows, down.shape[1]
+    if dy.dtype != shared.dtype:
+        raise ValueError(f"dy must have the weight's type {shared.dtype}, not {dy.dtype}")
+    if negative_slope is not None and y is None:
+        raise ValueError("y is needed for the derivative of the activation")
+    held_x, tx = _held(x, "x", rows, shared.k, dy.dtype)
+    held_y, ty = _held(y, "y", rows, shared.n, dy.dtype) if y is not None else (None, None)
+    _dense(low, "low", (rows, rank))
+    if low.dtype != _torch.float32:
+        raise ValueError(f"low must be float32, not {low.dtype}")
+    lib = _lib.load()
+    with _On(dy, shared.packed, down, up, groups.plan, tx, ty, low) as stream:
+        dx = _torch.empty((rows, shared.k), dtype=dy.dtype, device=dy.device) if need_dx else None
+        if rows == 0:
+            return dx, _torch.zeros_like(down), _torch.zeros_like(up)
+        ddown, dup = _torch.empty_like(down), _torch.empty_like(up)
+        scratch = _torch.empty(_backward_words(rows, groups.groups, shared.n, shared.k, rank), dtype=_torch.float32, device=dy.device)
+        _lib.check(lib.vh_adapt_backward(layer, dy.data_ptr(), ld, held_x, held_y, low.data_ptr(), rows, groups.plan.data_ptr(),
+                                         dx.data_ptr() if need_dx else None, shared.k, ddown.data_ptr(), dup.data_ptr(), scratch.data_ptr(), stream))
+    return dx, ddown, dup
+
+
+# ---- checkpoints ----------------------------------------------------------------------------------------------------------------
+class Checkpoint8:
+    """A matrix ``[rows, columns]`` held in one byte per element: ``codes`` uint8 ``[rows, columns rounded up to 32]``, e4m3 bits of
+    ``x 2^-e``, and ``exponents`` uint8 ``[rows, columns / 32 rounded up]``, ``e + 127`` of every 32 columns.
+
+    ``e`` is the least with ``amax <= 448 * 2^e`` over the block's finite magnitudes, kept in [-117, 120]; codes are rounded to nearest even
+    (2^-4 relative to the value, 2^-10 of the block's scale near zero), their sign bit is set where ``x > 0`` does not hold (the derivative
+    of LeakyReLU can be read from it), a non-finite element is NaN, and magnitudes that would round to
+    2^128 become 240 * 2^120.  Every value is exact in bfloat16."""
+
+    __slots__ = ("codes", "exponents", "columns")
+
+    def __init__(self, codes: _torch.Tensor, exponents: _torch.Tensor, columns: int):
+        if columns < 1:
+            raise ValueError(f"a checkpoint has at least one column, not {columns}")
+        if not isinstance(codes, _torch.Tensor) or codes.dim() != 2 or codes.dtype != _torch.uint8:
+            raise ValueError("codes must be a uint8 tensor [rows, columns rounded up to 32]")
+        blocks = -(-columns // BLOCK)
+        _dense(codes, "codes", (codes.shape[0], BLOCK * blocks))
+        _dense(exponents, "exponents", (codes.shape[0], blocks))
+        if exponents.dtype != _torch.uint8:
+            raise ValueError("exponents must be uint8")
+        if exponents.device != codes.device:
+            raise ValueError("codes and exponents must be on one device")
+        if codes.numel() and codes.data_ptr() % 8:
+            raise ValueError("codes must be 8-byte aligned")
+        self.codes, self.exponents, self.columns = codes, exponents, columns
+
+    @classmethod
+    def _empty(cls, rows: int, columns: int, device):
+        blocks = -(-columns // BLOCK)
+        self = cls.__new__(cls)
+        self.codes = _torch.empty((rows, BLOCK * blocks), dtype=_torch.uint8, device=device)
+        self.exponents = _torch.empty((rows, blocks), dtype=_torch.uint8, device=device)
+        self.columns = columns
+        return self
+
+    @property
+    def shape(self):
+        return _torch.Size((self.codes.shape[0], self.columns))
+
+    def restore(self, dtype: _torch.dtype = _torch.float32) -> _torch.Tensor:
+        """The values that the codes stand for, ``[rows, columns]`` (exact in either type)."""
+        if dtype not in _DTYPES:
+            raise ValueError(f"a checkpoint is restored to float32 or bfloat16, not {dtype}")
+        rows = self.codes.shape[0]
+        lib = _lib.load()
+        with _On(self.codes) as stream:
+            out = _torch.empty((rows, self.columns), dtype=dtype, device=self.codes.device)
+            if rows:
+                _lib.check(lib.vh_checkpoint8_restore(self.codes.data_ptr(), self.exponents.data_ptr(), rows, self.columns, _DTYPES[dtype],
+                                                      out.data_ptr(), stream))
+        return out
+
+
+def checkpoint8(x: _torch.Tensor) -> Checkpoint8:
+    """Hold ``x [rows, columns]`` for the backward pass in one byte per element."""
+    ld = _matrix(x, "x")
+    code = _dtype_of(x, "x")
+    rows, columns = x.shape
+    if columns < 1:
+        raise ValueError("x must have at least one column")
+    lib = _lib.load()
+    with _On(x) as stream:
+        held = Checkpoint8._empty(rows, columns, x.device)
+        if rows:
+            _lib.check(lib.vh_checkpoint8(x.data_ptr(), ld, rows, columns, code, held.codes.data_ptr(), held.exponents.data_ptr(), stream))
+    return held
+
+
+def _held(t, what: str, rows: int, cols: int, dtype):
+    if isinstance(t, Checkpoint8):
+        if tuple(t.shape) != (rows, cols):
+            raise ValueError(f"the checkpoint {what} must be [{rows}, {cols}], not {list(t.shape)}")
+        return _lib.Held(None, 0, t.codes.data_ptr(), t.exponents.data_ptr()), t.codes
+    ld = _matrix(t, what, rows, cols)
+    if t.dtype != dtype:
+        raise ValueError(f"{what} must be {dtype}, not {t.dtype}")
+    return _lib.Held(t.data_ptr(), ld, None, None), t
+
+
+def checkpoint_weight_grad(dy, x: Checkpoint8, y=None, negative_slope: Optional[float] = None):
+    """``(dW, db)`` of a layer whose input waited as a checkpoint: ``p^T x [n, k]`` and ``sum p [n]`` with ``p = dy f'(y)``.
+
+    ``y`` (tensor or checkpoint) and ``negative_slope`` come together for a layer with LeakyReLU; without them ``p = dy``."""
+    if not isinstance(x, Checkpoint8):
+        raise ValueError("x must be a Checkpoint8")
+    rows, k = x.shape
+    ld = _matrix(dy, "dy", rows)
+    code = _dtype_of(dy, "dy")
+    n = dy.shape[1]
+    if n < 1:
+        raise ValueError("dy must have at least one column")
+    _check_slope(negative_slope)
+    if negative_slope is not None and y is None:
+        raise ValueError("y is needed for the derivative of the activation")
+    held_x, tx = _held(x, "x", rows, k, dy.dtype)
+    # (without an activation y plays no part, as in adapted_linear_backward)
+    held_y, ty = _held(y, "y", rows, n, dy.dtype) if y is not None else (None, None)
+    lib = _lib.load()
+    with _On(dy, tx, ty) as stream:
+        if rows == 0:
+            return _torch.zeros((n, k), dtype=dy.dtype, device=dy.device), _torch.zeros(n, dtype=dy.dtype, device=dy.device)
+        dweight = _torch.empty((n, k), dtype=dy.dtype, device=dy.device)
+        dbias = _torch.empty(n, dtype=dy.dtype, device=dy.device)
+        scratch = _torch.empty(_weight_grad_words(rows, n, k), dtype=_torch.float32, device=dy.device)
+        _lib.check(lib.vh_checkpoint8_weight_grad(dy.data_ptr(), ld, held_x, held_y if negative_slope is not None else None,
+                                                  negative_slope or 0.0, rows, n, k, code, dweight.data_ptr(), dbias.data_ptr(), scratch.data_ptr(), stream))
+    return dweight, dbias

@@ -1,0 +1,1121 @@
+// adapt.hip -- low-rank adapters of many groups of rows beside a shared projection, and 8-bit activation checkpoints: the C entry
+// points of include/vambhip.h and every kernel of them but the projection itself (adapt_linear.hpp).  gfx950.
+//
+// All pointers of these entry points are DEVICE pointers of the calling thread's current device; the calls enqueue on `stream` and
+// return; scratch memory is the caller's, so that two streams or two captured graphs never share any.  Nothing is
+// allocated, cleared by memset or synchronised.
+#include "adapt_common.hpp"
+#include "common.hpp"
+
+namespace vh {
+namespace adapt {
+
+// =====================================================================================================================
+// Row plan: a stable counting sort of the rows by group.  Rows per wave are consecutive; 64 keys at a time are ranked among
+// themselves by ballots over the key's bits, the LDS counter of the wave gives the base.
+// =====================================================================================================================
+__device__ __forceinline__ unsigned long long same_key(int key, int bits) {
+    unsigned long long m = ~0ull;
+    for (int b = 0; b < bits; ++b) {
+        const unsigned long long v = __ballot((key >> b) & 1);
+        m &= ((key >> b) & 1) ? v : ~v;
+    }
+    return m;
+}
+__device__ __forceinline__ int key_of(const int* groups, int64_t row, int64_t rows, int n_groups) {
+    if (row >= rows) return n_groups + 1;   // no row
+    const int g = groups[row];
+    return (unsigned)g < (unsigned)n_groups ? g : n_groups;
+}
+
+// exclusive scan over a workgroup of 1024; *total = the sum
+__device__ __forceinline__ int3 block_scan3(int3 v, int3* total, int* lds /* 3 * 16 */) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int3 s = v;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const int x = __shfl_up(s.x, d), y = __shfl_up(s.y, d), z = __shfl_up(s.z, d);
+        if (lane >= d) { s.x += x; s.y += y; s.z += z; }
+    }
+    __syncthreads();
+    if (lane == 63) { lds[wave] = s.x; lds[16 + wave] = s.y; lds[32 + wave] = s.z; }
+    __syncthreads();
+    int3 base = {0, 0, 0}, all = {0, 0, 0};
+    for (int w = 0; w < 16; ++w) {
+        if (w == wave) base = all;
+        all.x += lds[w];
+        all.y += lds[16 + w];
+        all.z += lds[32 + w];
+    }
+    *total = all;
+    return int3{base.x + s.x - v.x, base.y + s.y - v.y, base.z + s.z - v.z};
+}
+
+// One workgroup of 1024: rows per group `count(g)` -> run starts (handed to `start(g, first slot)`), filling slots, items, multis, header.
+template <class Count, class Start>
+__device__ __forceinline__ void plan_offsets(int* plan, const PlanShape& ps, int* lds, Count count, Start start) {
+    const int G = (int)ps.groups, ir = (int)ps.item_rows;
+    int slot0 = 0, item0 = 0, multi0 = 0, part0 = 0;
+    for (int base = 0; base <= G; base += 1024) {
+        const int g = base + (int)threadIdx.x;
+        const int m = g <= G ? count(g) : 0;
+        const int filled = (m + 15) & ~15;
+        const int pieces = g < G ? max(1, (m + ir - 1) / ir) : 0;
+        const int multi = pieces > 1;
+        // the two small counts share a word: multis <= rows / item_rows + 1 <= 513, parts <= 2 multis-worth of pieces <= 1100
+        int3 total;
+        const int3 at = block_scan3(int3{filled, pieces, multi | ((multi ? pieces : 0) << 16)}, &total, lds);
+        if (g <= G) {
+            const int first = slot0 + at.x;
+            start(g, first);
+            for (int i = m; i < filled; ++i) plan[ps.o_row + first + i] = -1;
+            const int part = part0 + (at.z >> 16);
+            for (int i = 0; i < pieces; ++i) {
+                int* it = plan + ps.o_item + 4 * (int64_t)(item0 + at.y + i);
+                it[0] = g;
+                it[1] = first + i * ir;
+                it[2] = min(ir, m - i * ir);
+                it[3] = multi ? part + i : -1;
+            }
+            if (multi) {
+                int* mu = plan + ps.o_multi + 4 * (int64_t)(multi0 + (at.z & 0xffff));
+                mu[0] = g;
+                mu[1] = part;
+                mu[2] = pieces;
+            }
+        }
+        slot0 += total.x;
+        item0 += total.y;
+        multi0 += total.z & 0xffff;
+        part0 += total.z >> 16;
+    }
+    if (threadIdx.x == 0) {
+        plan[kPlanSubs] = slot0 / 16;
+        plan[kPlanItems] = item0;
+        plan[kPlanMultis] = multi0;
+        plan[kPlanParts] = part0;
+    }
+}
+
+__device__ __forceinline__ void place_rows(const int* groups, int64_t lo, int64_t hi, int64_t rows, int G, int bits, int* counter, int* plan,
+                                           const PlanShape& ps) {
+    const int lane = threadIdx.x & 63;
+    for (int64_t row0 = lo; row0 < hi; row0 += 64) {
+        const int64_t row = row0 + lane;
+        const int key = key_of(groups, row < hi ? row : rows, rows, G);
+        const unsigned long long same = same_key(key, bits);
+        const int rank = __popcll(same & ((1ull << lane) - 1));
+        if (key <= G) {
+            const int slot = counter[key] + rank;
+            plan[ps.o_row + slot] = (int)row;
+            if ((slot & 15) == 0) plan[ps.o_sub + slot / 16] = key < G ? key : -1;
+        }
+        __builtin_amdgcn_wave_barrier();   // every lane has read its counter (LDS operations of a wave complete in order)
+        if (key <= G && rank == 0) counter[key] += __popcll(same);
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+__device__ __forceinline__ void count_rows(const int* groups, int64_t lo, int64_t hi, int64_t rows, int G, int* counter) {
+    for (int64_t row = lo + (threadIdx.x & 63); row < hi; row += 64) atomicAdd(&counter[key_of(groups, row, rows, G)], 1);   // integers: any order
+}
+
+constexpr int kSmallRows = 16384, kSmallCounters = 16 * 1024;   // one workgroup: 16 waves' counters in 64 KB
+
+__global__ __launch_bounds__(1024) void plan_small_kernel(const int* groups, int* plan, PlanShape ps, int bits) {
+    extern __shared__ int counters[];   // [16][G + 1]
+    __shared__ int lds[48];
+    const int G = (int)ps.groups, wave = threadIdx.x >> 6;
+    for (int i = threadIdx.x; i < 16 * (G + 1); i += 1024) counters[i] = 0;
+    __syncthreads();
+    const int64_t seg = (ps.rows + 1023) / 1024 * 64, lo = min(wave * seg, ps.rows), hi = min(lo + seg, ps.rows);
+    count_rows(groups, lo, hi, ps.rows, G, counters + wave * (G + 1));
+    __syncthreads();
+    plan_offsets(plan, ps, lds,
+                 [&](int g) {
+                     int m = 0;
+                     for (int w = 0; w < 16; ++w) m += counters[w * (G + 1) + g];
+                     return m;
+                 },
+                 [&](int g, int first) {
+                     for (int w = 0; w < 16; ++w) {
+                         const int c = counters[w * (G + 1) + g];
+                         counters[w * (G + 1) + g] = first;
+                         first += c;
+                     }
+                 });
+    __syncthreads();
+    place_rows(groups, lo, hi, ps.rows, G, bits, counters + wave * (G + 1), plan, ps);
+}
+
+// Larger: one wave per piece of rows; counts [G + 1][pieces], then run totals [G + 1] behind them
+__global__ __launch_bounds__(64) void plan_count_kernel(const int* groups, int* scratch, PlanShape ps, int64_t seg, int pieces) {
+    extern __shared__ int counters[];
+    const int G = (int)ps.groups;
+    for (int i = threadIdx.x; i <= G; i += 64) counters[i] = 0;
+    __syncthreads();
+    const int64_t lo = min(blockIdx.x * seg, ps.rows), hi = min(lo + seg, ps.rows);
+    count_rows(groups, lo, hi, ps.rows, G, counters);
+    __syncthreads();
+    for (int i = threadIdx.x; i <= G; i += 64) scratch[(int64_t)i * pieces + blockIdx.x] = counters[i];
+}
+__global__ __launch_bounds__(64) void plan_scan_kernel(int* scratch, int G, int pieces) {
+    const int g = blockIdx.x, lane = threadIdx.x;
+    int* c = scratch + (int64_t)g * pieces;
+    int carry = 0;
+    for (int i0 = 0; i0 < pieces; i0 += 64) {
+        const int i = i0 + lane, v = i < pieces ? c[i] : 0;
+        int s = v;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const int u = __shfl_up(s, d);
+            if (lane >= d) s += u;
+        }
+        if (i < pieces) c[i] = carry + s - v;
+        carry += __shfl(s, 63);
+    }
+    if (lane == 0) scratch[(int64_t)(G + 1) * pieces + g] = carry;
+}
+__global__ __launch_bounds__(1024) void plan_offsets_kernel(int* plan, int* totals, PlanShape ps) {
+    __shared__ int lds[48];
+    plan_offsets(plan, ps, lds, [&](int g) { return totals[g]; }, [&](int g, int first) { totals[g] = first; });
+}
+__global__ __launch_bounds__(64) void plan_place_kernel(const int* groups, const int* scratch, int* plan, PlanShape ps, int64_t seg, int pieces, int bits) {
+    extern __shared__ int counters[];
+    const int G = (int)ps.groups;
+    for (int i = threadIdx.x; i <= G; i += 64) counters[i] = scratch[(int64_t)(G + 1) * pieces + i] + scratch[(int64_t)i * pieces + blockIdx.x];
+    __syncthreads();
+    const int64_t lo = min(blockIdx.x * seg, ps.rows), hi = min(lo + seg, ps.rows);
+    place_rows(groups, lo, hi, ps.rows, G, bits, counters, plan, ps);
+}
+
+static bool plan_is_small(int64_t rows, int64_t groups) { return rows <= kSmallRows && 16 * (groups + 1) <= kSmallCounters; }
+static int64_t plan_pieces(int64_t rows) { return rows < 512 ? 1 : (rows / 512 < 1024 ? rows / 512 : 1024); }
+
+// =====================================================================================================================
+// Shared weight: both orientations, zero-filled to multiples of 128 rows and 64 columns, cut into planes
+// =====================================================================================================================
+struct WeightShape {
+    int64_t np, kp, nq, kq, fwd, bwd, bias_off, bytes;   // fwd: [P][np][kq], bwd: [P][kp][nq]
+    int planes;
+};
+static WeightShape weight_shape(int64_t n, int64_t k, int dtype) {
+    WeightShape w{};
+    w.planes = dtype == VH_BF16 ? 1 : 3;
+    w.np = round_up(n, 128);
+    w.kq = round_up(k, 64);
+    w.kp = round_up(k, 128);
+    w.nq = round_up(n, 64);
+    w.fwd = w.np * w.kq;
+    w.bwd = w.kp * w.nq;
+    w.bias_off = 2 * w.planes * (w.fwd + w.bwd);
+    w.bytes = w.bias_off + 4 * w.np;
+    return w;
+}
+template <class T>
+__global__ __launch_bounds__(256) void pack_weight_kernel(const T* w, int64_t ld, const T* bias, int n, int k, bf16_t* out, float* out_bias, WeightShape ws) {
+    const int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x;
+    const bool second = i >= ws.fwd;
+    const int64_t j = second ? i - ws.fwd : i;
+    if (j < (second ? ws.bwd : ws.fwd)) {
+        const int64_t stride = second ? ws.nq : ws.kq, a = j / stride, b = j % stride;
+        const int64_t row = second ? b : a, col = second ? a : b;
+        const bool in = row < n && col < k;
+        bf16_t* dst = out + (second ? ws.planes * ws.fwd : 0) + j;
+        const int64_t plane = second ? ws.bwd : ws.fwd;
+        if constexpr (sizeof(T) == 2) {
+            dst[0] = in ? w[row * ld + col] : (T)0;
+        } else {
+            unsigned h, m, l;
+            split3(in ? w[row * ld + col] : 0.f, h, m, l);
+            dst[0] = (bf16_t)(h >> 16);
+            dst[plane] = (bf16_t)(m >> 16);
+            dst[2 * plane] = (bf16_t)(l >> 16);
+        }
+    }
+    if (i < ws.np) out_bias[i] = bias != nullptr && i < n ? to_f<T>(bias[i]) : 0.f;
+}
+
+// =====================================================================================================================
+// Checkpoints
+// =====================================================================================================================
+// four lanes share a block of 32 columns, eight each
+template <class T>
+__global__ __launch_bounds__(256) void checkpoint_kernel(const T* x, int64_t ldx, int64_t rows, int cols, uint8_t* codes, uint8_t* exps) {
+    const int chunks = (cols + kBlockCols - 1) / kBlockCols * 4;
+    const int64_t total = rows * chunks;
+    const int64_t first = blockIdx.x * (int64_t)256 + threadIdx.x, step = (int64_t)gridDim.x * 256;   // multiples of four: a block's lanes stay together
+    for (int64_t i = first; i < total; i += step) {
+        const int64_t row = i / chunks;
+        const int ch = (int)(i - row * chunks);
+        const Raw8<T> v = load8<T>(x + row * ldx + 8 * ch, cols - 8 * ch);
+        float f[8], amax = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            f[e] = v.get(e);
+            amax = fmaxf(amax, finite_size(f[e]));
+        }
+        amax = fmaxf(amax, __shfl_xor(amax, 1));
+        amax = fmaxf(amax, __shfl_xor(amax, 2));
+        const int k = block_exp(amax);
+        const u32x2 o = {encode4(f[0], f[1], f[2], f[3], k), encode4(f[4], f[5], f[6], f[7], k)};
+        *reinterpret_cast<u32x2*>(codes + 8 * i) = o;   // codes are dense: [rows][8 * chunks]
+        if ((ch & 3) == 0) exps[i >> 2] = (uint8_t)(k + 127);
+    }
+}
+template <class T>
+__global__ __launch_bounds__(256) void restore_kernel(const uint8_t* codes, const uint8_t* exps, int64_t rows, int cols, T* out) {
+    const int chunks = (cols + kBlockCols - 1) / kBlockCols * 4;
+    const int64_t total = rows * chunks, step = (int64_t)gridDim.x * 256;
+    const bool wide = cols % 8 == 0 && (uintptr_t)out % 16 == 0;
+    for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < total; i += step) {
+        const int64_t row = i / chunks;
+        const int c0 = 8 * (int)(i - row * chunks);
+        const u32x2 w = *reinterpret_cast<const u32x2*>(codes + 8 * i);
+        const float scale = __uint_as_float((unsigned)exps[i >> 2] << 23);
+        float f[8];
+        decode4(w[0], scale, reinterpret_cast<float(&)[4]>(f[0]));
+        decode4(w[1], scale, reinterpret_cast<float(&)[4]>(f[4]));
+        T* dst = out + row * cols + c0;
+        if (wide && c0 + 8 <= cols) {
+            struct __attribute__((aligned(16))) Eight { T e[8]; };
+            Eight o;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o.e[e] = from_f<T>(f[e]);
+            *reinterpret_cast<Eight*>(dst) = o;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (c0 + e < cols) dst[e] = from_f<T>(f[e]);
+        }
+    }
+}
+
+// A tensor that a backward pass reads: elements of T, or checkpoint codes
+struct Source {
+    const void* p;         // elements or codes
+    const uint8_t* exps;   // nullptr: elements
+    int64_t ld;            // in elements / bytes
+};
+template <class T>
+struct Eight {             // eight columns of a row as read
+    Raw8<T> raw;
+    u32x2 code;
+    unsigned exp;
+};
+template <class T>
+__device__ __forceinline__ void read8(const Source& s, int64_t row, int col, int valid, Eight<T>& o) {
+    if (s.exps == nullptr) {
+        o.raw = load8<T>((const T*)s.p + row * s.ld + col, valid);
+    } else {
+        o.code = u32x2{0, 0};
+        o.exp = 0;
+        if (valid > 0) {   // rows are filled up to a multiple of 32 codes (of value zero)
+            o.code = *reinterpret_cast<const u32x2*>((const uint8_t*)s.p + row * s.ld + col);
+            o.exp = s.exps[row * (s.ld / kBlockCols) + col / kBlockCols];
+        }
+    }
+}
+template <class T>
+__device__ __forceinline__ void values8(const Source& s, const Eight<T>& v, float (&f)[8]) {
+    if (s.exps == nullptr) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = v.raw.get(e);
+    } else {
+        const float scale = __uint_as_float(v.exp << 23);
+        decode4(v.code[0], scale, reinterpret_cast<float(&)[4]>(f[0]));
+        decode4(v.code[1], scale, reinterpret_cast<float(&)[4]>(f[4]));
+    }
+}
+// f'(y) of eight columns applied to f
+template <class T>
+__device__ __forceinline__ void masked8(const Source& s, const Eight<T>& v, float slope, float (&f)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const bool pos = s.exps == nullptr ? v.raw.get(e) > 0.f : !((v.code[e >> 2] >> (8 * (e & 3) + 7)) & 1);
+        f[e] = pos ? f[e] : f[e] * slope;
+    }
+}
+
+// =====================================================================================================================
+// Gradients of the adapters:  down_g = sum v^T x  [rank][K],  up_g = s sum p^T u  [N][rank]
+// One workgroup = one item (at most item_rows rows of one group) and 128 columns of x or of p.  v_mfma_f32_16x16x4_f32: its operands
+// are one element per lane, so eight consecutive columns that a lane has read are the operands of eight instructions and nothing is
+// transposed; products and sums are fp32 whatever the tensors' type.
+// =====================================================================================================================
+struct AdapterGradArgs {
+    Source x, mask;            // mask.p == nullptr: f' = 1
+    const void* dy;
+    int64_t ldy;
+    const float* low;          // u [rows][rank], from the forward pass
+    const float* v;            // [rows][rank], s included
+    void *ddown, *dup;
+    float* parts;
+    int K, N, rank;
+    float scale, slope;
+    const int* plan;
+    PlanShape ps;
+    int down_tiles;
+};
+
+template <class T, int RT>
+__global__ __launch_bounds__(256) void adapter_grad_kernel(AdapterGradArgs a) {
+    __shared__ __attribute__((aligned(16))) f32x4 red[2][RT * 8][64];
+    if ((int)blockIdx.x >= a.plan[kPlanItems]) return;
+    const int* it = a.plan + a.ps.o_item + 4 * (int64_t)blockIdx.x;
+    const int g = it[0], first = it[1], count = it[2], part = it[3];
+    const int* slot_row = a.plan + a.ps.o_row;
+    const bool up = (int)blockIdx.y >= a.down_tiles;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, quad = lane >> 4;
+    const int C = up ? a.N : a.K, c0 = ((int)blockIdx.y - (up ? a.down_tiles : 0)) * 128 + 8 * l15, valid = C - c0, r = a.rank;
+    const float* small = up ? a.low : a.v;
+    const Source wide = up ? Source{a.dy, nullptr, a.ldy} : a.x;
+
+    f32x4 acc[RT][8];
+#pragma unroll
+    for (int j = 0; j < RT; ++j)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[j][e] = f32x4{0, 0, 0, 0};
+
+    const bool masked = up && a.mask.p != nullptr;
+    Eight<T> w, m;
+    float s[RT];
+    auto row_of = [&](int i) { return i < count ? slot_row[first + i] : -1; };
+    auto fetch = [&](int rid) {
+        read8<T>(wide, max(rid, 0), c0, rid >= 0 ? valid : 0, w);
+        if (masked) read8<T>(a.mask, max(rid, 0), c0, rid >= 0 ? valid : 0, m);
+#pragma unroll
+        for (int j = 0; j < RT; ++j) s[j] = rid >= 0 && 16 * j + l15 < r ? small[(int64_t)rid * r + 16 * j + l15] : 0.f;
+    };
+    const int i0 = 4 * wave + quad;
+    fetch(row_of(i0));
+    int next = row_of(i0 + 16);
+    for (int i = 4 * wave; i < count; i += 16) {
+        float f[8], sc[RT];
+        values8<T>(wide, w, f);
+        if (masked) masked8<T>(a.mask, m, a.slope, f);
+#pragma unroll
+        for (int j = 0; j < RT; ++j) sc[j] = s[j];
+        fetch(next);
+        next = row_of(i + quad + 32);
+#pragma unroll
+        for (int j = 0; j < RT; ++j)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[j][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(sc[j], f[e], acc[j][e], 0, 0, 0);
+    }
+    // waves 2, 3 -> 0, 1 -> 0
+    if (wave >= 2) {
+#pragma unroll
+        for (int q = 0; q < RT * 8; ++q) red[wave - 2][q][lane] = acc[q / 8][q % 8];
+    }
+    __syncthreads();
+    if (wave < 2) {
+#pragma unroll
+        for (int q = 0; q < RT * 8; ++q) acc[q / 8][q % 8] += red[wave][q][lane];
+    }
+    __syncthreads();
+    if (wave == 1) {
+#pragma unroll
+        for (int q = 0; q < RT * 8; ++q) red[0][q][lane] = acc[q / 8][q % 8];
+    }
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int q = 0; q < RT * 8; ++q) acc[q / 8][q % 8] += red[0][q][lane];
+
+    const float scale = up ? a.scale : 1.f;   // (v has it)
+    const int64_t pair = (int64_t)r * (a.K + a.N);
+    float* po = part >= 0 ? a.parts + part * pair + (up ? (int64_t)r * a.K : 0) : nullptr;
+#pragma unroll
+    for (int j = 0; j < RT; ++j) {
+        const int rank = 16 * j + 4 * quad;
+        if (up) {
+            T* dst = (T*)a.dup + (int64_t)g * a.N * r;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (e < valid) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (rank + i < r) {
+                            const int64_t at = (int64_t)(c0 + e) * r + rank + i;
+                            if (po) po[at] = acc[j][e][i] * scale; else dst[at] = from_f<T>(acc[j][e][i] * scale);
+                        }
+                }
+        } else {
+            T* dst = (T*)a.ddown + (int64_t)g * r * a.K;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (rank + i < r) {
+                    const int64_t at = (int64_t)(rank + i) * a.K + c0;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (e < valid) {
+                            if (po) po[at + e] = acc[j][e][i]; else dst[at + e] = from_f<T>(acc[j][e][i]);
+                        }
+                }
+        }
+    }
+}
+template <class T>
+__global__ __launch_bounds__(256) void adapter_join_kernel(AdapterGradArgs a) {
+    if ((int)blockIdx.x >= a.plan[kPlanMultis]) return;
+    const int* mu = a.plan + a.ps.o_multi + 4 * (int64_t)blockIdx.x;
+    const int g = mu[0], part = mu[1], n = mu[2];
+    const int64_t half = (int64_t)a.rank * a.K, pair = (int64_t)a.rank * (a.K + a.N);
+    const int64_t i = blockIdx.y * (int64_t)256 + threadIdx.x;
+    if (i >= pair) return;
+    float s = 0.f;
+    for (int p = 0; p < n; ++p) s += a.parts[(part + p) * pair + i];
+    if (i < half) ((T*)a.ddown)[(int64_t)g * half + i] = from_f<T>(s);
+    else ((T*)a.dup)[(int64_t)g * a.N * a.rank + i - half] = from_f<T>(s);
+}
+
+// =====================================================================================================================
+// Few rows: no plan.  A workgroup = 16 rows x 16 columns; eight waves share the depth of the projection and, one distinct adapter at a
+// time, the u of the rows; the last 256 products with B_g are plain fused multiply-adds in float32.
+// =====================================================================================================================
+struct FewArgs {
+    const void* x;
+    int64_t ldx;
+    const int* groups;
+    const bf16_t* w;
+    int64_t w_plane;
+    int ldw;
+    const float* bias;
+    const void *down, *up;
+    int K, N, rank, n_groups, activation;
+    int64_t rows;
+    float scale, slope;
+    void* y;
+    int64_t ldy;
+};
+template <class T, int RT>
+__global__ __launch_bounds__(512) void few_kernel(FewArgs a) {
+    constexpr int P = Elem<T>::planes;
+    __shared__ float part[8][16][17];
+    __shared__ float low[16][16 * RT + 1];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l15 = lane & 15, quad = lane >> 4;
+    const int n0 = blockIdx.x * 16, r = a.rank, K = a.K;
+    const int64_t row0 = blockIdx.y * (int64_t)16;
+    const int64_t my = min(row0 + l15, a.rows - 1);
+    int g = row0 + l15 < a.rows ? a.groups[my] : -1;
+    if ((unsigned)g >= (unsigned)a.n_groups) g = -1;
+    const T* xr = (const T*)a.x + my * a.ldx;
+
+    f32x4 acc = {0, 0, 0, 0};
+    const bf16_t* wr = a.w + (int64_t)(n0 + l15) * a.ldw;
+    for (int k0 = 32 * wave; k0 < K; k0 += 256) {
+        const int k = k0 + 8 * quad;
+        const Planes8<T> xp = to_planes(load8<T>(xr + k, K - k));
+        s16x8 wf[P];
+#pragma unroll
+        for (int p = 0; p < P; ++p) wf[p] = __builtin_bit_cast(s16x8, *reinterpret_cast<const u32x4*>(wr + p * a.w_plane + k));
+        acc = mma(wf, xp.p, acc);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) part[wave][l15][4 * quad + i] = acc[i];
+
+    unsigned pending = (unsigned)__ballot(g >= 0) & 0xffffu;
+    for (int at = 0; pending; ++at) {
+        const int one = __builtin_amdgcn_readfirstlane(__shfl(g, __builtin_ctz(pending)));
+        const unsigned same = (unsigned)__ballot(g == one) & 0xffffu;
+        pending &= ~same;
+        if ((at & 7) != wave) continue;
+        f32x4 u[RT];
+#pragma unroll
+        for (int j = 0; j < RT; ++j) u[j] = f32x4{0, 0, 0, 0};
+        for (int k0 = 0; k0 < K; k0 += 32) {
+            const int k = k0 + 8 * quad;
+            const Planes8<T> xp = to_planes(load8<T>(xr + k, K - k));
+#pragma unroll
+            for (int j = 0; j < RT; ++j) {
+                const int rank = 16 * j + l15;
+                const Planes8<T> ap = to_planes(load8<T>((const T*)a.down + ((int64_t)one * r + rank) * K + k, rank < r ? K - k : 0));
+                u[j] = mma(ap.p, xp.p, u[j]);
+            }
+        }
+        if (g == one) {
+#pragma unroll
+            for (int j = 0; j < RT; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) low[l15][16 * j + 4 * quad + i] = u[j][i];
+        }
+    }
+    __syncthreads();
+    if (tid >= 256) return;
+    // thread = (row, column)
+    const int row = tid >> 4, col = n0 + (tid & 15);
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) v += part[w][row][tid & 15];
+    if (row0 + row >= a.rows || col >= a.N) return;
+    const int gr = a.groups[row0 + row];
+    if ((unsigned)gr < (unsigned)a.n_groups) {
+        const T* b = (const T*)a.up + ((int64_t)gr * a.N + col) * r;
+        float s = 0.f;
+        for (int j0 = 0; j0 < r; j0 += 8) {
+            const Raw8<T> w = load8<T>(b + j0, r - j0);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s = fmaf(j0 + e < r ? low[row][min(j0 + e, 16 * RT - 1)] : 0.f, w.get(e), s);
+        }
+        v = fmaf(s, a.scale, v);
+    }
+    if (a.bias != nullptr) v += a.bias[col];
+    if (a.activation) v = v > 0.f ? v : v * a.slope;
+    ((T*)a.y)[(row0 + row) * a.ldy + col] = from_f<T>(v);
+}
+
+// =====================================================================================================================
+// Gradient of the shared projection from checkpoints:  dW = p^T x  [N][K],  db = sum p  [N]
+// Tile 128 x 128, split over the rows; both operands are contracted along their slow dimension: row-major LDS tiles [32 rows][128
+// columns] read by the transposing LDS instruction.  x's values are exact in bf16 (one plane), so float32 dy costs three products, not
+// six.  256-byte tile rows: the 32-byte pieces are XOR-permuted by the row so that the eight rows of half a read differ in their banks.
+// =====================================================================================================================
+struct WeightGradArgs {
+    Source x, mask;
+    const void* dy;
+    int64_t ldy, rows;
+    int N, K, k_tiles;
+    int64_t split_rows;
+    float slope;
+    float* parts;      // [splits][N * K + N]
+};
+typedef short tr_v4s __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ s16x4 read_tr(const unsigned char* p) {
+    return __builtin_bit_cast(s16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) tr_v4s*)p));
+}
+__device__ __forceinline__ int tr_swz(int row) { return (row & 3) | ((row >> 1) & 4); }
+
+template <class T>
+__global__ __launch_bounds__(256) void weight_grad_kernel(WeightGradArgs a) {
+    constexpr int P = Elem<T>::planes, BR = 32, TB = BR * 256;
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];   // [2][P + 1][TB]: planes of p, then x
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l15 = lane & 15, quad = lane >> 4;
+    const int n0 = ((int)blockIdx.x / a.k_tiles) * 128, k0 = ((int)blockIdx.x % a.k_tiles) * 128;
+    const int64_t lo = blockIdx.y * a.split_rows, hi = min(lo + a.split_rows, a.rows);
+    const int wn = wave >> 1, wk = wave & 1;
+    const bool masked = a.mask.p != nullptr, sums = k0 == 0;
+    const Source dy = {a.dy, nullptr, a.ldy};
+
+    // pieces of eight columns: thread t has column piece t % 16 of rows t / 16 and t / 16 + 16
+    const int pc = tid & 15, pr = tid >> 4;
+    Eight<T> pw[2], mw[2], xw[2];
+    auto fetch = [&](int64_t row0) {
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            const int64_t row = row0 + pr + 16 * q;
+            const bool in = row < hi;
+            const int64_t at = in ? row : lo;
+            read8<T>(dy, at, n0 + 8 * pc, in ? a.N - n0 - 8 * pc : 0, pw[q]);
+            if (masked) read8<T>(a.mask, at, n0 + 8 * pc, in ? a.N - n0 - 8 * pc : 0, mw[q]);
+            read8<T>(a.x, at, k0 + 8 * pc, in ? a.K - k0 - 8 * pc : 0, xw[q]);
+        }
+    };
+    float bsum[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) bsum[e] = 0.f;
+    auto keep = [&](unsigned char* buf) {
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            const int row = pr + 16 * q, at = row * 256 + (((pc >> 1) ^ tr_swz(row)) * 32 + (pc & 1) * 16);
+            float f[8];
+            values8<T>(dy, pw[q], f);
+            if (masked) masked8<T>(a.mask, mw[q], a.slope, f);
+            Raw8<T> o;
+            o.zero();
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                bsum[e] += f[e];
+                o.set(e, from_f<T>(f[e]));
+            }
+            const Planes8<T> pl = to_planes(o);
+#pragma unroll
+            for (int p = 0; p < P; ++p) *reinterpret_cast<s16x8*>(buf + p * TB + at) = pl.p[p];
+            values8<T>(a.x, xw[q], f);
+            u32x4 xv;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) xv[e] = (__float_as_uint(f[2 * e]) >> 16) | (__float_as_uint(f[2 * e + 1]) & 0xffff0000u);   // exact
+            *reinterpret_cast<u32x4*>(buf + P * TB + at) = xv;
+        }
+    };
+    f32x4 acc[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+
+    // lane's share of a transposed operand: rows 8 quad + l15 / 4 (+ 4), columns 4 (l15 % 4) of the 16
+    const int fr = 8 * quad + (l15 >> 2);
+    auto frag = [&](const unsigned char* buf, int col0) {
+        const int piece = (col0 >> 4), off = 8 * (l15 & 3);
+        const s16x4 a0 = read_tr(buf + fr * 256 + ((piece ^ tr_swz(fr)) * 32) + off);
+        const s16x4 a1 = read_tr(buf + (fr + 4) * 256 + ((piece ^ tr_swz(fr + 4)) * 32) + off);
+        return __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    fetch(lo);
+    keep(smem);
+    __syncthreads();
+    int cur = 0;
+    for (int64_t row0 = lo; row0 < hi; row0 += BR) {
+        const unsigned char* buf = smem + cur * (P + 1) * TB;
+        unsigned char* nxt = smem + (cur ^ 1) * (P + 1) * TB;
+        const bool more = row0 + BR < hi;
+        if (more) fetch(row0 + BR);
+        s16x8 xf[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) xf[j] = frag(buf + P * TB, wk * 64 + 16 * j);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            s16x8 pf[P];
+#pragma unroll
+            for (int p = 0; p < P; ++p) pf[p] = frag(buf + p * TB, wn * 64 + 16 * i);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int p = P - 1; p >= 0; --p) acc[i][j] = mfma32(xf[j], pf[p], acc[i][j]);   // D[k column][n column]
+        }
+        if (more) keep(nxt);
+        __syncthreads();
+        cur ^= 1;
+    }
+    float* out = a.parts + blockIdx.y * ((int64_t)a.N * a.K + a.N);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int n = n0 + wn * 64 + 16 * i + l15;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int k = k0 + wk * 64 + 16 * j + 4 * quad;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (n < a.N && k + e < a.K) out[(int64_t)n * a.K + k + e] = acc[i][j][e];
+        }
+    }
+    if (sums) {
+        float* s = reinterpret_cast<float*>(smem);   // [16 rows][128]: the tiles are done with (barrier above)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[pr * 128 + 8 * pc + e] = bsum[e];
+        __syncthreads();
+        if (tid < 128 && n0 + tid < a.N) {
+            float v = 0.f;
+            for (int i = 0; i < 16; ++i) v += s[i * 128 + tid];
+            out[(int64_t)a.N * a.K + n0 + tid] = v;
+        }
+    }
+}
+template <class T>
+__global__ __launch_bounds__(256) void weight_join_kernel(const float* parts, int splits, int64_t n_weight, int64_t total, T* dw, T* db) {
+    const int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x;
+    if (i >= total) return;
+    float s = 0.f;
+    for (int p = 0; p < splits; ++p) s += parts[p * total + i];
+    if (i < n_weight) dw[i] = from_f<T>(s);
+    else if (db != nullptr) db[i - n_weight] = from_f<T>(s);
+}
+// about 512 workgroups, at least 64 rows each
+static int64_t weight_splits(int64_t rows, int64_t n, int64_t k, int64_t* split_rows) {
+    const int64_t tiles = ceil_div(n, 128) * ceil_div(k, 128);
+    int64_t want = ceil_div(512, tiles);
+    const int64_t most = ceil_div(rows, 64);
+    want = want < most ? want : most;
+    *split_rows = round_up(ceil_div(rows, want), 32);
+    return ceil_div(rows, *split_rows);
+}
+
+// =====================================================================================================================
+// Checks that every entry shares
+// =====================================================================================================================
+static void check_dtype(int dtype) { VH_REQUIRE(dtype == VH_F32 || dtype == VH_BF16, "dtype must be VH_F32 or VH_BF16, not %d", dtype); }
+static void check_rows(int64_t rows) { VH_REQUIRE(rows >= 1 && rows <= (int64_t(1) << 30), "rows must be in [1, 2^30], not %lld", (long long)rows); }
+static void check_width(int64_t w, const char* what) { VH_REQUIRE(w >= 1 && w <= (1 << 20), "%s must be in [1, 2^20], not %lld", what, (long long)w); }
+static void check_groups(int64_t g) { VH_REQUIRE(g >= 1 && g <= kMaxGroups, "the number of groups must be in [1, %d], not %lld", kMaxGroups, (long long)g); }
+static void check_rank(int64_t r) { VH_REQUIRE(r >= 1 && r <= kMaxRank, "the rank must be in [1, %d], not %lld", kMaxRank, (long long)r); }
+static void check_ptr(const void* p, const char* what) { VH_REQUIRE(p != nullptr, "%s is NULL", what); }
+static void check_slope(int activation, float slope) {
+    // the derivative is taken from the sign of the value, which a negative slope would lose
+    VH_REQUIRE(!activation || (slope >= 0.f && slope < __builtin_inff()), "the negative slope must be finite and >= 0");
+}
+static void check_held(const uint8_t* codes, const uint8_t* exps, const char* what) {
+    VH_REQUIRE((codes == nullptr) == (exps == nullptr), "%s: codes and exponents come together", what);
+    VH_REQUIRE((uintptr_t)codes % 8 == 0, "%s: codes must be 8-byte aligned", what);
+}
+static int64_t code_cols(int64_t c) { return round_up(c, kBlockCols); }
+
+static Source source_of(const vh_held* t, int64_t cols, const char* what) {
+    check_held(t->codes, t->exponents, what);
+    VH_REQUIRE((t->data != nullptr) != (t->codes != nullptr), "%s: either elements or codes", what);
+    if (t->codes != nullptr) return {t->codes, t->exponents, code_cols(cols)};
+    VH_REQUIRE(t->ld >= cols, "%s: row stride %lld below the %lld columns", what, (long long)t->ld, (long long)cols);
+    return {t->data, nullptr, t->ld};
+}
+static void check_layer(const vh_adapt_layer* l) {
+    check_ptr(l, "layer");
+    check_dtype(l->dtype);
+    check_width(l->n, "n");
+    check_width(l->k, "k");
+    check_groups(l->groups);
+    check_rank(l->rank);
+    check_ptr(l->packed, "packed weight");
+    VH_REQUIRE((uintptr_t)l->packed % 16 == 0, "packed weight must be 16-byte aligned");
+    check_ptr(l->down, "down");
+    check_ptr(l->up, "up");
+    check_slope(l->activation, l->negative_slope);
+    VH_REQUIRE(l->scale == l->scale && fabsf(l->scale) < __builtin_inff(), "scale must be finite");
+}
+static void run_linear(const LinArgs& a, int dtype, bool backward, hipStream_t s) {
+    if (dtype == VH_BF16) launch_linear_bf16(a, backward, s);
+    else launch_linear_f32(a, backward, s);
+}
+template <class T, int RT>
+static void launch_few(const FewArgs& a, hipStream_t s) {
+    few_kernel<T, RT><<<dim3((unsigned)ceil_div(a.N, 16), (unsigned)ceil_div(a.rows, 16)), 512, 0, s>>>(a);
+    VH_HIP(hipGetLastError());
+}
+template <class T>
+static void few_rank(const FewArgs& a, hipStream_t s) {
+    if (a.rank <= 16) launch_few<T, 1>(a, s);
+    else if (a.rank <= 32) launch_few<T, 2>(a, s);
+    else launch_few<T, 4>(a, s);
+}
+template <class T>
+static void adapter_grads(const AdapterGradArgs& a, hipStream_t s) {
+    const dim3 grid((unsigned)a.ps.items, (unsigned)(a.down_tiles + ceil_div(a.N, 128)));
+    if (a.rank <= 16) adapter_grad_kernel<T, 1><<<grid, 256, 0, s>>>(a);
+    else if (a.rank <= 32) adapter_grad_kernel<T, 2><<<grid, 256, 0, s>>>(a);
+    else adapter_grad_kernel<T, 4><<<grid, 256, 0, s>>>(a);
+    VH_HIP(hipGetLastError());
+    if (a.ps.rows > a.ps.item_rows) {
+        const int64_t multis = a.ps.rows / a.ps.item_rows < a.ps.groups ? a.ps.rows / a.ps.item_rows : a.ps.groups;
+        adapter_join_kernel<T><<<dim3((unsigned)multis, (unsigned)ceil_div((int64_t)a.rank * (a.K + a.N), 256)), 256, 0, s>>>(a);
+        VH_HIP(hipGetLastError());
+    }
+}
+static int64_t grad_parts(const PlanShape& ps) { return ps.rows > ps.item_rows ? 2 * (ps.rows / ps.item_rows) : 0; }
+
+}  // namespace adapt
+}  // namespace vh
+
+using namespace vh;
+using namespace vh::adapt;
+
+extern "C" {
+
+int vh_rows_plan_size(int64_t rows, int64_t groups, int64_t* plan_words, int64_t* scratch_words) {
+    return guarded([&] {
+        check_rows(rows);
+        check_groups(groups);
+        check_ptr(plan_words, "plan_words");
+        check_ptr(scratch_words, "scratch_words");
+        *plan_words = plan_shape(rows, groups).words;
+        *scratch_words = plan_is_small(rows, groups) ? 0 : (groups + 1) * (plan_pieces(rows) + 1);
+    });
+}
+
+int vh_rows_plan(const int32_t* row_groups, int64_t rows, int64_t groups, int32_t* plan, int32_t* scratch, void* stream) {
+    return guarded([&] {
+        check_rows(rows);
+        check_groups(groups);
+        check_ptr(row_groups, "row_groups");
+        check_ptr(plan, "plan");
+        VH_REQUIRE((uintptr_t)plan % 16 == 0, "plan must be 16-byte aligned");
+        const PlanShape ps = plan_shape(rows, groups);
+        hipStream_t s = (hipStream_t)stream;
+        int bits = 1;
+        while ((1 << bits) < groups + 2) ++bits;   // keys 0 .. groups + 1
+        if (plan_is_small(rows, groups)) {
+            plan_small_kernel<<<1, 1024, 16 * (groups + 1) * sizeof(int), s>>>(row_groups, plan, ps, bits);
+            VH_HIP(hipGetLastError());
+            return;
+        }
+        check_ptr(scratch, "scratch");
+        const int pieces = (int)plan_pieces(rows);
+        const int64_t seg = round_up(ceil_div(rows, pieces), 64);
+        const size_t lds = (groups + 1) * sizeof(int);
+        int* totals = scratch + (groups + 1) * pieces;
+        if (lds > 65536) {
+            VH_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(plan_count_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+            VH_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(plan_place_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+        }
+        plan_count_kernel<<<pieces, 64, lds, s>>>(row_groups, scratch, ps, seg, pieces);
+        VH_HIP(hipGetLastError());
+        plan_scan_kernel<<<(unsigned)(groups + 1), 64, 0, s>>>(scratch, (int)groups, pieces);
+        VH_HIP(hipGetLastError());
+        plan_offsets_kernel<<<1, 1024, 0, s>>>(plan, totals, ps);
+        VH_HIP(hipGetLastError());
+        plan_place_kernel<<<pieces, 64, lds, s>>>(row_groups, scratch, plan, ps, seg, pieces, bits);
+        VH_HIP(hipGetLastError());
+    });
+}
+
+int vh_adapt_weight_size(int64_t n, int64_t k, int dtype, int64_t* bytes) {
+    return guarded([&] {
+        check_dtype(dtype);
+        check_width(n, "n");
+        check_width(k, "k");
+        check_ptr(bytes, "bytes");
+        *bytes = weight_shape(n, k, dtype).bytes;
+    });
+}
+
+int vh_adapt_weight_pack(const void* weight, int64_t ld, const void* bias, int64_t n, int64_t k, int dtype, void* packed, void* stream) {
+    return guarded([&] {
+        check_dtype(dtype);
+        check_width(n, "n");
+        check_width(k, "k");
+        check_ptr(weight, "weight");
+        check_ptr(packed, "packed");
+        VH_REQUIRE(ld >= k, "row stride %lld below the %lld columns", (long long)ld, (long long)k);
+        VH_REQUIRE((uintptr_t)packed % 16 == 0, "packed weight must be 16-byte aligned");
+        const WeightShape ws = weight_shape(n, k, dtype);
+        float* out_bias = reinterpret_cast<float*>((char*)packed + ws.bias_off);
+        const unsigned blocks = (unsigned)ceil_div(ws.fwd + ws.bwd, 256);
+        if (dtype == VH_BF16)
+            pack_weight_kernel<bf16_t><<<blocks, 256, 0, (hipStream_t)stream>>>((const bf16_t*)weight, ld, (const bf16_t*)bias, (int)n, (int)k,
+                                                                                (bf16_t*)packed, out_bias, ws);
+        else
+            pack_weight_kernel<float><<<blocks, 256, 0, (hipStream_t)stream>>>((const float*)weight, ld, (const float*)bias, (int)n, (int)k,
+                                                                               (bf16_t*)packed, out_bias, ws);
+        VH_HIP(hipGetLastError());
+    });
+}
+
+int vh_adapt_forward(const vh_adapt_layer* l, const void* x, int64_t ldx, int64_t rows, const int32_t* plan, void* y, int64_t ldy, float* low,
+                     uint8_t* codes, uint8_t* exponents, void* stream) {
+    return guarded([&] {
+        check_layer(l);
+        check_rows(rows);
+        check_ptr(x, "x");
+        check_ptr(y, "y");
+        check_ptr(plan, "plan");
+        VH_REQUIRE(ldx >= l->k && ldy >= l->n, "row strides below the number of columns");
+        check_held(codes, exponents, "checkpoint of y");
+        const WeightShape ws = weight_shape(l->n, l->k, l->dtype);
+        const int es = l->dtype == VH_BF16 ? 2 : 4;
+        LinArgs a{};
+        a.x = x;
+        a.ldx = ldx;
+        a.slope = l->negative_slope;
+        a.activation = l->activation;
+        a.w = (const bf16_t*)l->packed;
+        a.w_plane = ws.fwd;
+        a.ldw = (int)ws.kq;
+        a.bias = reinterpret_cast<const float*>((const char*)l->packed + ws.bias_off);
+        a.inner = l->down;
+        a.outer = l->up;
+        a.K = (int)l->k;
+        a.N = (int)l->n;
+        a.rank = (int)l->rank;
+        a.scale = l->scale;
+        a.low_scale = 1.f;
+        a.low = low;
+        a.y = y;
+        a.ldy = ldy;
+        a.codes = codes;
+        a.ldc = code_cols(l->n);
+        a.exps = exponents;
+        a.plan = plan;
+        a.ps = plan_shape(rows, l->groups);
+        a.dma = es == 2 && l->k % 8 == 0 && ldx % 8 == 0 && (uintptr_t)x % 16 == 0;
+        run_linear(a, l->dtype, false, (hipStream_t)stream);
+    });
+}
+
+int vh_adapt_forward_few(const vh_adapt_layer* l, const void* x, int64_t ldx, int64_t rows, const int32_t* row_groups, void* y, int64_t ldy, void* stream) {
+    return guarded([&] {
+        check_layer(l);
+        check_rows(rows);
+        check_ptr(x, "x");
+        check_ptr(y, "y");
+        check_ptr(row_groups, "row_groups");
+        VH_REQUIRE(rows <= 65535 * 16, "too many rows for this entry");
+        VH_REQUIRE(ldx >= l->k && ldy >= l->n, "row strides below the number of columns");
+        const WeightShape ws = weight_shape(l->n, l->k, l->dtype);
+        FewArgs a{};
+        a.x = x;
+        a.ldx = ldx;
+        a.groups = row_groups;
+        a.w = (const bf16_t*)l->packed;
+        a.w_plane = ws.fwd;
+        a.ldw = (int)ws.kq;
+        a.bias = reinterpret_cast<const float*>((const char*)l->packed + ws.bias_off);
+        a.down = l->down;
+        a.up = l->up;
+        a.K = (int)l->k;
+        a.N = (int)l->n;
+        a.rank = (int)l->rank;
+        a.n_groups = (int)l->groups;
+        a.activation = l->activation;
+        a.rows = rows;
+        a.scale = l->scale;
+        a.slope = l->negative_slope;
+        a.y = y;
+        a.ldy = ldy;
+        if (l->dtype == VH_BF16) few_rank<bf16_t>(a, (hipStream_t)stream);
+        else few_rank<float>(a, (hipStream_t)stream);
+    });
+}
+
+int vh_adapt_backward_size(int64_t rows, int64_t groups, int64_t n, int64_t k, int64_t rank, int64_t* scratch_words) {
+    return guarded([&] {
+        check_rows(rows);
+        check_groups(groups);
+        check_width(n, "n");
+        check_width(k, "k");
+        check_rank(rank);
+        check_ptr(scratch_words, "scratch_words");
+        const PlanShape ps = plan_shape(rows, groups);
+        *scratch_words = round_up(rows * rank, 4) + grad_parts(ps) * rank * (n + k);
+    });
+}
+
+int vh_adapt_backward(const vh_adapt_layer* l, const void* dy, int64_t lddy, const vh_held* x, const vh_held* y, const float* low, int64_t rows,
+                      const int32_t* plan, void* dx, int64_t lddx, void* ddown, void* dup, float* scratch, void* stream) {
+    return guarded([&] {
+        check_layer(l);
+        check_rows(rows);
+        check_ptr(dy, "dy");
+        check_ptr(x, "x");
+        check_ptr(low, "low");
+        check_ptr(plan, "plan");
+        check_ptr(ddown, "ddown");
+        check_ptr(dup, "dup");
+        check_ptr(scratch, "scratch");
+        VH_REQUIRE(lddy >= l->n && (dx == nullptr || lddx >= l->k), "row strides below the number of columns");
+        VH_REQUIRE(!l->activation || y != nullptr, "the layer's output is needed for the derivative of its activation");
+        const Source xs = source_of(x, l->k, "x");
+        Source mask = {nullptr, nullptr, 0};
+        if (l->activation) mask = source_of(y, l->n, "y");
+        const PlanShape ps = plan_shape(rows, l->groups);
+        float* v = scratch;
+        const WeightShape ws = weight_shape(l->n, l->k, l->dtype);
+        LinArgs a{};
+        a.x = dy;
+        a.ldx = lddy;
+        a.mask = mask.p;
+        a.ldm = mask.ld;
+        a.mask_codes = mask.exps != nullptr;
+        a.slope = l->negative_slope;
+        a.w = (const bf16_t*)l->packed + ws.planes * ws.fwd;
+        a.w_plane = ws.bwd;
+        a.ldw = (int)ws.nq;
+        a.inner = l->up;
+        a.outer = l->down;
+        a.K = (int)l->n;
+        a.N = (int)l->k;
+        a.rank = (int)l->rank;
+        a.scale = a.low_scale = l->scale;
+        a.low = v;
+        a.y = dx;
+        a.ldy = lddx;
+        a.plan = plan;
+        a.ps = ps;
+        run_linear(a, l->dtype, true, (hipStream_t)stream);
+        AdapterGradArgs g{};
+        g.x = xs;
+        g.mask = mask;
+        g.dy = dy;
+        g.ldy = lddy;
+        g.low = low;
+        g.v = v;
+        g.ddown = ddown;
+        g.dup = dup;
+        g.parts = scratch + round_up(rows * l->rank, 4);
+        g.K = (int)l->k;
+        g.N = (int)l->n;
+        g.rank = (int)l->rank;
+        g.scale = l->scale;
+        g.slope = l->negative_slope;
+        g.plan = plan;
+        g.ps = ps;
+        g.down_tiles = (int)ceil_div(l->k, 128);
+        if (l->dtype == VH_BF16) adapter_grads<bf16_t>(g, (hipStream_t)stream);
+        else adapter_grads<float>(g, (hipStream_t)stream);
+    });
+}
+
+int vh_checkpoint8(const void* x, int64_t ld, int64_t rows, int64_t cols, int dtype, uint8_t* codes, uint8_t* exponents, void* stream) {
+    return guarded([&] {
+        check_dtype(dtype);
+        check_rows(rows);
+        check_width(cols, "cols");
+        check_ptr(x, "x");
+        check_ptr(codes, "codes");
+        check_held(codes, exponents, "checkpoint");
+        VH_REQUIRE(ld >= cols, "row stride %lld below the %lld columns", (long long)ld, (long long)cols);
+        const int64_t blocks = ceil_div(rows * (code_cols(cols) / 8), 256);
+        const unsigned grid = (unsigned)(blocks < 8192 ? blocks : 8192);
+        if (dtype == VH_BF16) checkpoint_kernel<bf16_t><<<grid, 256, 0, (hipStream_t)stream>>>((const bf16_t*)x, ld, rows, (int)cols, codes, exponents);
+        else checkpoint_kernel<float><<<grid, 256, 0, (hipStream_t)stream>>>((const float*)x, ld, rows, (int)cols, codes, exponents);
+        VH_HIP(hipGetLastError());
+    });
+}
+
+int vh_checkpoint8_restore(const uint8_t* codes, const uint8_t* exponents, int64_t rows, int64_t cols, int dtype, void* out, void* stream) {
+    return guarded([&] {
+        check_dtype(dtype);
+        check_rows(rows);
+        check_width(cols, "cols");
+        check_ptr(codes, "codes");
+        check_ptr(out, "out");
+        check_held(codes, exponents, "checkpoint");
+        const int64_t blocks = ceil_div(rows * (code_cols(cols) / 8), 256);
+        const unsigned grid = (unsigned)(blocks < 8192 ? blocks : 8192);
+        if (dtype == VH_BF16) restore_kernel<bf16_t><<<grid, 256, 0, (hipStream_t)stream>>>(codes, exponents, rows, (int)cols, (bf16_t*)out);
+        else restore_kernel<float><<<grid, 256, 0, (hipStream_t)stream>>>(codes, exponents, rows, (int)cols, (float*)out);
+        VH_HIP(hipGetLastError());
+    });
+}
+
+int vh_checkpoint8_weight_grad_size(int64_t rows, int64_t n, int64_t k, int64_t* scratch_words) {
+    return guarded([&] {
+        check_rows(rows);
+        check_width(n, "n");
+        check_width(k, "k");
+        check_ptr(scratch_words, "scratch_words");
+        int64_t split_rows;
+        *scratch_words = weight_splits(rows, n, k, &split_rows) * (n * k + n);
+    });
+}
+
+int vh_checkpoint8_weight_grad(const void* dy, int64_t lddy, const vh_held* x, const vh_held* y, float negative_slope, int64_t rows, int64_t n, int64_t k,
+                               int dtype, void* dweight, void* dbias, float* scratch, void* stream) {
+    return guarded([&] {
+        check_dtype(dtype);
+        check_rows(rows);
+        check_width(n, "n");
+        check_width(k, "k");
+        check_ptr(dy, "dy");
+        check_ptr(x, "x");
+        check_ptr(dweight, "dweight");
+        check_ptr(scratch, "scratch");
+        VH_REQUIRE(lddy >= n, "row stride %lld below the %lld columns", (long long)lddy, (long long)n);
+        check_slope(y != nullptr, negative_slope);
+        WeightGradArgs a{};
+        a.x = source_of(x, k, "x");
+        VH_REQUIRE(a.x.exps != nullptr, "x must be a checkpoint");
+        if (y != nullptr) a.mask = source_of(y, n, "y");
+        a.dy = dy;
+        a.ldy = lddy;
+        a.rows = rows;
+        a.N = (int)n;
+        a.K = (int)k;
+        a.k_tiles = (int)ceil_div(k, 128);
+        a.slope = negative_slope;
+        a.parts = scratch;
+        const int64_t splits = weight_splits(rows, n, k, &a.split_rows);
+        const int64_t tiles = ceil_div(n, 128) * a.k_tiles, total = n * k + n;
+        VH_REQUIRE(tiles < (int64_t(1) << 31) && splits < 65536, "too many tiles for one launch");
+        const dim3 grid((unsigned)tiles, (unsigned)splits);
+        hipStream_t s = (hipStream_t)stream;
+        if (dtype == VH_BF16) {
+            weight_grad_kernel<bf16_t><<<grid, 256, 2 * 2 * 32 * 256, s>>>(a);
+            VH_HIP(hipGetLastError());
+            weight_join_kernel<bf16_t><<<(unsigned)ceil_div(total, 256), 256, 0, s>>>(scratch, (int)splits, n * k, total, (bf16_t*)dweight, (bf16_t*)dbias);
+        } else {
+            weight_grad_kernel<float><<<grid, 256, 2 * 4 * 32 * 256, s>>>(a);
+            VH_HIP(hipGetLastError());
+            weight_join_kernel<float><<<(unsigned)ceil_div(total, 256), 256, 0, s>>>(scratch, (int)splits, n * k, total, (float*)dweight, (float*)dbias);
+        }
+        VH_HIP(hipGetLastError());
+    });
+}
+
+}  // extern "C"

@@ -1,0 +1,250 @@
+// adapt_common.hpp -- element types, 8-bit checkpoints and the row plan shared by the adapter kernels (adapt*.hip), gfx950.
+//
+// Operands of the matrix products.  v_mfma_f32_16x16x32_bf16 is the only matrix instruction of the wide products: bf16 tensors are
+// one operand plane, float32 tensors three (x = x0 + x1 + x2, each the next 8 significant bits cut off: exact, 3 x 8 = 24 bits), and of
+// the nine products of two such splits the six with i + j <= 2 are taken; the three dropped ones are below 2^-23 of the
+// product.  Six bf16 products run at 2.5 PF / 6 = 420 TF, the fp32 instruction at 157 TF.
+//
+// 8-bit checkpoints.  One byte per element (e4m3: 1 + 4 + 3 bits) and one exponent byte per 32 columns of a row.  The
+// exponent k is the least with amax <= 448 * 2^k, kept in [-117, 120], so that (a) no code saturates, (b) every value code * 2^k has 4
+// significant bits and is a normal bf16: the backward products read it without a further rounding.  The sign
+// bit is set iff !(x > 0), zeros included: that bit IS the derivative of LeakyReLU, whose argument is positive iff its value is.
+// A non-finite element becomes the NaN code (0xff) and does not enter amax.  At k = 120 the code is kept to 240: 256 * 2^120 would be an
+// infinity in both types.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+namespace vh {
+namespace adapt {
+
+typedef unsigned short bf16_t;   // raw bits
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bfx2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bfx8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+// the same at any element alignment (rows of 107 or 154 columns start anywhere); gfx950 serves unaligned 16-byte loads
+typedef unsigned u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+typedef unsigned u32x2_any __attribute__((ext_vector_type(2), aligned(2)));
+
+constexpr int kBlockCols = 32;   // columns that share an exponent
+constexpr int kMinExp = -117, kMaxExp = 120;
+constexpr int kMaxRank = 64;
+constexpr int kMaxGroups = 16384;
+
+template <class T> struct Elem;
+template <> struct Elem<bf16_t> { static constexpr int planes = 1; };
+template <> struct Elem<float> { static constexpr int planes = 3; };
+
+__device__ __forceinline__ float bf_to_f(bf16_t h) { return __uint_as_float((unsigned)h << 16); }
+__device__ __forceinline__ bf16_t f_to_bf(float x) { return __builtin_bit_cast(bf16_t, (__bf16)x); }   // nearest even
+
+template <class T> __device__ __forceinline__ float to_f(T x);
+template <> __device__ __forceinline__ float to_f<float>(float x) { return x; }
+template <> __device__ __forceinline__ float to_f<bf16_t>(bf16_t x) { return bf_to_f(x); }
+template <class T> __device__ __forceinline__ T from_f(float x);
+template <> __device__ __forceinline__ float from_f<float>(float x) { return x; }
+template <> __device__ __forceinline__ bf16_t from_f<bf16_t>(float x) { return f_to_bf(x); }
+
+// ---- eight consecutive elements as they were read -------------------------------------------------------------------------
+template <class T> struct Raw8;
+template <> struct Raw8<bf16_t> {
+    u32x4 v;
+    __device__ __forceinline__ void zero() { v = u32x4{0, 0, 0, 0}; }
+    __device__ __forceinline__ void load(const bf16_t* p) { v = *reinterpret_cast<const u32x4_any*>(p); }
+    __device__ __forceinline__ void set(int e, bf16_t x) {   // e: a constant after unrolling; the element's bits are zero before
+        v[e >> 1] |= (unsigned)x << (16 * (e & 1));
+    }
+    __device__ __forceinline__ float get(int e) const { return __uint_as_float((e & 1) ? (v[e >> 1] & 0xffff0000u) : (v[e >> 1] << 16)); }
+};
+template <> struct Raw8<float> {
+    f32x4 a, b;
+    __device__ __forceinline__ void zero() { a = f32x4{0, 0, 0, 0}; b = a; }
+    __device__ __forceinline__ void load(const float* p) {
+        a = *reinterpret_cast<const f32x4_any*>(p);
+        b = *reinterpret_cast<const f32x4_any*>(p + 4);
+    }
+    __device__ __forceinline__ void set(int e, float x) {
+        if (e < 4) a[e] = x; else b[e - 4] = x;
+    }
+    __device__ __forceinline__ float get(int e) const { return e < 4 ? a[e] : b[e - 4]; }
+};
+
+// p[0 .. 7], zeros behind the first `valid` (nothing is read behind them)
+template <class T>
+__device__ __forceinline__ Raw8<T> load8(const T* p, int valid) {
+    Raw8<T> r;
+    r.zero();
+    if (valid >= 8) {
+        r.load(p);
+    } else if (valid > 0) {
+#pragma unroll
+        for (int e = 0; e < 7; ++e)
+            if (e < valid) r.set(e, p[e]);
+    }
+    return r;
+}
+template <class T>
+__device__ __forceinline__ Raw8<T> load8_strided(const T* p, int64_t stride, int valid) {
+    Raw8<T> r;
+    r.zero();
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (e < valid) r.set(e, p[e * stride]);
+    return r;
+}
+
+// ---- operand planes ---------------------------------------------------------------------------------------------------------
+// the three cuts of a float32; an infinity stays whole in the first (inf - inf would make a NaN of it), a NaN stays one
+__device__ __forceinline__ void split3(float x, unsigned& h, unsigned& m, unsigned& l) {
+    const unsigned b = __float_as_uint(x);
+    h = b & 0xffff0000u;
+    float r = x - __uint_as_float(h);
+    r = __builtin_isinf(x) ? 0.f : r;
+    m = __float_as_uint(r) & 0xffff0000u;
+    const float q = r - __uint_as_float(m);
+    l = __float_as_uint(q);   // at most 8 significant bits: its low half is zero
+}
+
+template <class T> struct Planes8 { s16x8 p[Elem<T>::planes]; };
+
+__device__ __forceinline__ Planes8<bf16_t> to_planes(const Raw8<bf16_t>& r) {
+    Planes8<bf16_t> o;
+    o.p[0] = __builtin_bit_cast(s16x8, r.v);
+    return o;
+}
+__device__ __forceinline__ Planes8<float> to_planes(const Raw8<float>& r) {
+    u32x4 w[3];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        unsigned h0, m0, l0, h1, m1, l1;
+        split3(r.get(2 * e), h0, m0, l0);
+        split3(r.get(2 * e + 1), h1, m1, l1);
+        w[0][e] = (h0 >> 16) | (h1 & 0xffff0000u);
+        w[1][e] = (m0 >> 16) | (m1 & 0xffff0000u);
+        w[2][e] = (l0 >> 16) | (l1 & 0xffff0000u);
+    }
+    Planes8<float> o;
+#pragma unroll
+    for (int p = 0; p < 3; ++p) o.p[p] = __builtin_bit_cast(s16x8, w[p]);
+    return o;
+}
+
+__device__ __forceinline__ f32x4 mfma32(s16x8 a, s16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bfx8, a), __builtin_bit_cast(bfx8, b), c, 0, 0, 0);
+}
+template <int PA, int PB>
+__device__ __forceinline__ f32x4 mma(const s16x8 (&a)[PA], const s16x8 (&b)[PB], f32x4 c) {
+#pragma unroll
+    for (int s = 2; s >= 0; --s)   // smallest products first
+#pragma unroll
+        for (int i = 0; i < PA; ++i)
+#pragma unroll
+            for (int j = 0; j < PB; ++j)
+                if (i + j == s) c = mfma32(a[i], b[j], c);
+    return c;
+}
+
+// ---- 8-bit checkpoints ------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ float finite_size(float x) {
+    const float a = fabsf(x);
+    return a < __builtin_inff() ? a : 0.f;   // (a NaN compares false)
+}
+// least k with amax <= 448 * 2^k (448 = 1.75 * 2^8: the mantissa above 1.75 carries into the exponent), kept in range
+__device__ __forceinline__ int block_exp(float amax) {
+    const int k = (int)((__float_as_uint(amax) + 0x1fffffu) >> 23) - 127 - 8;
+    return min(max(k, kMinExp), kMaxExp);
+}
+__device__ __forceinline__ float exp2i(int k) { return __uint_as_float((unsigned)(k + 127) << 23); }   // -126 <= k <= 127
+// four elements -> four codes
+__device__ __forceinline__ unsigned encode4(float x0, float x1, float x2, float x3, int k) {
+    const float inv = exp2i(-k), top = k == kMaxExp ? 240.f : 448.f;
+    auto y = [&](float x) { return __builtin_amdgcn_fmed3f(x * inv, -top, top); };
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(y(x0), y(x1), 0, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(y(x2), y(x3), w, true);
+    unsigned s = 0, n = 0;
+    const float x[4] = {x0, x1, x2, x3};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (!(x[e] > 0.f)) s |= 0x80u << (8 * e);
+        if (!(fabsf(x[e]) < __builtin_inff())) n |= 0xffu << (8 * e);
+    }
+    return ((unsigned)w & 0x7f7f7f7fu) | s | n;
+}
+__device__ __forceinline__ void decode4(unsigned codes, float scale, float (&o)[4]) {
+    const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, true);
+    o[0] = a[0] * scale;
+    o[1] = a[1] * scale;
+    o[2] = b[0] * scale;
+    o[3] = b[1] * scale;
+}
+
+// ---- the row plan -----------------------------------------------------------------------------------------------------------
+// Rows sorted by group (stably: sums over a group's rows have one order), every group's run filled up to a multiple of 16 slots, so that
+// a 16-row MFMA operand has ONE adapter.  Rows whose group is not in [0, groups) stand last, without an adapter.  An "item" is
+// a piece of at most item_rows rows of one group: a workgroup of the gradient kernel; a group of several items ("multi") writes parts
+// that the join kernel adds in their order.  A group without rows has one empty item, which writes its zeros.
+struct PlanShape {
+    int64_t rows, groups;
+    int64_t slots, subs, items, multis, item_rows;
+    int64_t o_row, o_sub, o_item, o_multi, words;
+};
+inline PlanShape plan_shape(int64_t rows, int64_t groups) {
+    PlanShape s{};
+    s.rows = rows;
+    s.groups = groups;
+    const int64_t runs = groups + 1 < rows ? groups + 1 : rows;
+    s.subs = rows / 16 + runs;
+    s.slots = 16 * s.subs;
+    int64_t ir = (rows / 512 + 15) / 16 * 16;
+    s.item_rows = ir < 256 ? 256 : ir;
+    s.items = groups + rows / s.item_rows;
+    s.multis = rows / s.item_rows + 1;
+    s.o_row = 16;
+    s.o_sub = s.o_row + s.slots;
+    s.o_item = (s.o_sub + s.subs + 3) / 4 * 4;
+    s.o_multi = s.o_item + 4 * s.items;
+    s.words = s.o_multi + 4 * s.multis;
+    return s;
+}
+enum { kPlanSubs = 0, kPlanItems = 1, kPlanMultis = 2, kPlanParts = 3 };
+
+// ---- arguments of the shared-projection kernel (adapt_linear.hpp) -----------------------------------------------------------------
+struct LinArgs {
+    const void* x;            // [rows][ldx]: the layer's input, or dy
+    int64_t ldx;
+    const void* mask;         // backward: the layer's output whose sign selects f' (nullptr: f' = 1) ...
+    int64_t ldm;              // ... its row stride in elements / bytes
+    int mask_codes;           // ... as checkpoint codes
+    float slope;
+    int activation;           // forward: LeakyReLU(slope) on the result
+    const bf16_t* w;          // packed operand [planes][.][ldw]
+    int64_t w_plane;          // elements of a plane
+    int ldw;
+    const float* bias;        // padded, or nullptr
+    const void* inner;        // adapters contracted with x (forward: down, backward: up)
+    const void* outer;        // adapters of the result (forward: up, backward: down)
+    int K, N, rank;
+    float scale, low_scale;   // on the expanded part; on `low` as it is written
+    float* low;               // [rows][rank] or nullptr
+    void* y;                  // [rows][ldy]; nullptr: only `low` is wanted
+    int64_t ldy;
+    uint8_t* codes;           // checkpoint of y (nullptr: none), row stride ldc
+    int64_t ldc;
+    uint8_t* exps;            // row stride ldc / 32
+    const int* plan;
+    PlanShape ps;
+    int dma;                  // x rows are 16-byte aligned and K is a multiple of 8
+};
+void launch_linear_bf16(const LinArgs& a, bool backward, hipStream_t s);
+void launch_linear_f32(const LinArgs& a, bool backward, hipStream_t s);
+
+}  // namespace adapt
+}  // namespace vh

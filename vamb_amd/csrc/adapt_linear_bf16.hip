@@ -1,0 +1,12 @@
+// Instantiations of the shared-projection kernel on bf16 tensors (adapt_linear.hpp).
+#include "adapt_linear.hpp"
+
+namespace vh {
+namespace adapt {
+void launch_linear_bf16(const LinArgs& a, bool backward, hipStream_t s) {
+    if (backward) launch_rank<bf16_t, true, false>(a, s);
+    else if (a.dma) launch_rank<bf16_t, false, true>(a, s);
+    else launch_rank<bf16_t, false, false>(a, s);
+}
+}  // namespace adapt
+}  // namespace vh
