@@ -492,9 +492,10 @@ int vh_vae_train_epoch_dp(vh_vae* h, const int64_t* perm, int64_t n_batches, int
  *
  * Unlike the handles above, these entry points take DEVICE pointers (of the calling thread's current device), enqueue on `stream`
  * (a hipStream_t; NULL: the null stream) and return without synchronising; they allocate nothing, so that they may be captured
- * into a graph.  Scratch memory is the caller's, of the size that the *_size entry gives; calls that may run at the same
+ * into a graph.  Scratch memory is the caller's, 16-byte aligned and of the size that the *_size entry gives; calls that may run at the same
  * time need scratch of their own.  Tensors are float32 or bf16 (`dtype`), unit stride along a row, `ld*` elements between rows, any
- * alignment of the element type.  Widths up to 2^20, rows up to 2^30, ranks up to 64, groups up to 16384.
+ * alignment of the element type.  Widths up to 2^20, weights (padded to 128 x 64) below 4 GB in each
+ * direction (bf16: 2 bytes, float32: 6 bytes an element), rows up to 2^30, ranks up to 64, groups up to 16384.
  * ============================================================================================= */
 enum { VH_F32 = 0, VH_BF16 = 1 };
 
@@ -537,7 +538,7 @@ int vh_adapt_forward_few(const vh_adapt_layer* layer, const void* x, int64_t ldx
                          void* stream);
 /* y (elements or checkpoint) may be NULL without an activation.  dx [rows][lddx] may be NULL (not wanted).  ddown, dup: dense, like
  * down and up; a group without rows gets zeros.  The sums over a group's rows have one order: equal inputs give equal bits. */
-int vh_adapt_backward_size(int64_t rows, int64_t groups, int64_t n, int64_t k, int64_t rank, int64_t* scratch_words);
+int vh_adapt_backward_size(int64_t rows, int64_t groups, int64_t n, int64_t k, int64_t rank, int dtype, int64_t* scratch_words);
 int vh_adapt_backward(const vh_adapt_layer* layer, const void* dy, int64_t lddy, const vh_held* x, const vh_held* y, const float* low, int64_t rows,
                       const int32_t* plan, void* dx, int64_t lddx, void* ddown, void* dup, float* scratch, void* stream);
 

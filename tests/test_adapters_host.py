@@ -155,7 +155,7 @@ def test_c_entries_refuse():
         lambda: lib.vh_adapt_forward(layer, some, K, 5, some, some, N, None, some, None, None),     # codes without exponents
         lambda: lib.vh_adapt_forward(layer, some, K, 2 ** 31, some, some, N, None, None, None, None),
         lambda: lib.vh_adapt_forward_few(layer, some, K, 5, None, some, N, None),
-        lambda: lib.vh_adapt_backward_size(5, 5, N, K, 0, a),
+        lambda: lib.vh_adapt_backward_size(5, 5, N, K, 0, 0, a),
         lambda: lib.vh_adapt_backward(layer, some, N, _lib.Held(None, 0, None, None), None, some, 5, some, some, K, some, some, some, None),
         lambda: lib.vh_adapt_backward(layer, some, N, _lib.Held(some, K, some, some), None, some, 5, some, some, K, some, some, some, None),
         lambda: lib.vh_adapt_backward(layer, some, N, _lib.Held(some, K - 1, None, None), None, some, 5, some, some, K, some, some, some, None),

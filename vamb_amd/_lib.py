@@ -176,7 +176,7 @@ SIGNATURES = {
     "vh_adapt_weight_pack": (_int, [_vp, _i64, _vp, _i64, _i64, _int, _vp, _vp]),
     "vh_adapt_forward": (_int, [ctypes.POINTER(AdaptLayer), _vp, _i64, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _vp]),
     "vh_adapt_forward_few": (_int, [ctypes.POINTER(AdaptLayer), _vp, _i64, _i64, _vp, _vp, _i64, _vp]),
-    "vh_adapt_backward_size": (_int, [_i64, _i64, _i64, _i64, _i64, ctypes.POINTER(_i64)]),
+    "vh_adapt_backward_size": (_int, [_i64, _i64, _i64, _i64, _i64, _int, ctypes.POINTER(_i64)]),
     "vh_adapt_backward": (_int, [ctypes.POINTER(AdaptLayer), _vp, _i64, ctypes.POINTER(Held), ctypes.POINTER(Held), _vp, _i64, _vp, _vp, _i64, _vp, _vp,
                                  _vp, _vp]),
     "vh_checkpoint8": (_int, [_vp, _i64, _i64, _i64, _int, _vp, _vp, _vp]),

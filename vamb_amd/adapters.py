@@ -100,9 +100,9 @@ def _plan_words(rows: int, groups: int):
 
 
 @lru_cache(maxsize=4096)
-def _backward_words(rows: int, groups: int, n: int, k: int, rank: int) -> int:
+def _backward_words(rows: int, groups: int, n: int, k: int, rank: int, dtype: int) -> int:
     a = ctypes.c_int64()
-    _lib.check(_lib.load().vh_adapt_backward_size(rows, groups, n, k, rank, ctypes.byref(a)))
+    _lib.check(_lib.load().vh_adapt_backward_size(rows, groups, n, k, rank, dtype, ctypes.byref(a)))
     return a.value
 
 
@@ -196,8 +196,8 @@ def _layer(shared, down, up, n_groups, scale, negative_slope):
 
 
 def _check_slope(negative_slope) -> None:
-    if negative_slope is not None and not (0.0 <= negative_slope < math.inf):
-        raise ValueError(f"negative_slope must be finite and >= 0 (the derivative is read from the sign of the result), not {negative_slope}")
+    if negative_slope is not None and not 0.0 <= negative_slope <= 1.0:
+        raise ValueError(f"negative_slope must be in [0, 1] (the derivative is read from the sign of the result), not {negative_slope}")
 
 
 def _input(x, shared) -> int:
@@ -284,7 +284,7 @@ def adapted_linear_backward(dy, x, y, low, shared: SharedProjection, down, up, g
         if rows == 0:
             return dx, _torch.zeros_like(down), _torch.zeros_like(up)
         ddown, dup = _torch.empty_like(down), _torch.empty_like(up)
-        scratch = _torch.empty(_backward_words(rows, groups.groups, shared.n, shared.k, rank), dtype=_torch.float32, device=dy.device)
+        scratch = _torch.empty(_backward_words(rows, groups.groups, shared.n, shared.k, rank, layer.dtype), dtype=_torch.float32, device=dy.device)
         _lib.check(lib.vh_adapt_backward(layer, dy.data_ptr(), ld, held_x, held_y, low.data_ptr(), rows, groups.plan.data_ptr(),
                                          dx.data_ptr() if need_dx else None, shared.k, ddown.data_ptr(), dup.data_ptr(), scratch.data_ptr(), stream))
     return dx, ddown, dup

@@ -22,12 +22,6 @@ __device__ __forceinline__ unsigned long long same_key(int key, int bits) {
     }
     return m;
 }
-__device__ __forceinline__ int key_of(const int* groups, int64_t row, int64_t rows, int n_groups) {
-    if (row >= rows) return n_groups + 1;   // no row
-    const int g = groups[row];
-    return (unsigned)g < (unsigned)n_groups ? g : n_groups;
-}
-
 // exclusive scan over a workgroup of 1024; *total = the sum
 __device__ __forceinline__ int3 block_scan3(int3 v, int3* total, int* lds /* 3 * 16 */) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -97,26 +91,49 @@ __device__ __forceinline__ void plan_offsets(int* plan, const PlanShape& ps, int
     }
 }
 
-__device__ __forceinline__ void place_rows(const int* groups, int64_t lo, int64_t hi, int64_t rows, int G, int bits, int* counter, int* plan,
-                                           const PlanShape& ps) {
+// 64 PB rows of a wave at a time, their keys requested together: what a key's load takes is paid once per batch
+constexpr int PB = 8;
+__device__ __forceinline__ void load_keys(const int* groups, int64_t row0, int64_t hi, int G, int (&key)[PB]) {
     const int lane = threadIdx.x & 63;
-    for (int64_t row0 = lo; row0 < hi; row0 += 64) {
-        const int64_t row = row0 + lane;
-        const int key = key_of(groups, row < hi ? row : rows, rows, G);
-        const unsigned long long same = same_key(key, bits);
-        const int rank = __popcll(same & ((1ull << lane) - 1));
-        if (key <= G) {
-            const int slot = counter[key] + rank;
-            plan[ps.o_row + slot] = (int)row;
-            if ((slot & 15) == 0) plan[ps.o_sub + slot / 16] = key < G ? key : -1;
-        }
-        __builtin_amdgcn_wave_barrier();   // every lane has read its counter (LDS operations of a wave complete in order)
-        if (key <= G && rank == 0) counter[key] += __popcll(same);
-        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int b = 0; b < PB; ++b) {
+        const int64_t row = row0 + 64 * b + lane;
+        key[b] = groups[min(row, hi - 1)];
+    }
+#pragma unroll
+    for (int b = 0; b < PB; ++b) {
+        const int64_t row = row0 + 64 * b + lane;
+        key[b] = row < hi ? ((unsigned)key[b] < (unsigned)G ? key[b] : G) : G + 1;   // G + 1: no row
     }
 }
-__device__ __forceinline__ void count_rows(const int* groups, int64_t lo, int64_t hi, int64_t rows, int G, int* counter) {
-    for (int64_t row = lo + (threadIdx.x & 63); row < hi; row += 64) atomicAdd(&counter[key_of(groups, row, rows, G)], 1);   // integers: any order
+__device__ __forceinline__ void place_rows(const int* groups, int64_t lo, int64_t hi, int G, int bits, int* counter, int* plan, const PlanShape& ps) {
+    const int lane = threadIdx.x & 63;
+    for (int64_t row0 = lo; row0 < hi; row0 += 64 * PB) {
+        int key[PB];
+        load_keys(groups, row0, hi, G, key);
+#pragma unroll
+        for (int b = 0; b < PB; ++b) {
+            const unsigned long long same = same_key(key[b], bits);
+            const int rank = __popcll(same & ((1ull << lane) - 1));
+            if (key[b] <= G) {
+                const int slot = counter[key[b]] + rank;
+                plan[ps.o_row + slot] = (int)(row0 + 64 * b + lane);
+                if ((slot & 15) == 0) plan[ps.o_sub + slot / 16] = key[b] < G ? key[b] : -1;
+            }
+            __builtin_amdgcn_wave_barrier();   // every lane has read its counter (LDS operations of a wave complete in order)
+            if (key[b] <= G && rank == 0) counter[key[b]] += __popcll(same);
+            __builtin_amdgcn_wave_barrier();
+        }
+    }
+}
+__device__ __forceinline__ void count_rows(const int* groups, int64_t lo, int64_t hi, int G, int* counter) {
+    for (int64_t row0 = lo; row0 < hi; row0 += 64 * PB) {
+        int key[PB];
+        load_keys(groups, row0, hi, G, key);
+#pragma unroll
+        for (int b = 0; b < PB; ++b)
+            if (key[b] <= G) atomicAdd(&counter[key[b]], 1);   // integers: any order
+    }
 }
 
 constexpr int kSmallRows = 16384, kSmallCounters = 16 * 1024;   // one workgroup: 16 waves' counters in 64 KB
@@ -128,7 +145,7 @@ __global__ __launch_bounds__(1024) void plan_small_kernel(const int* groups, int
     for (int i = threadIdx.x; i < 16 * (G + 1); i += 1024) counters[i] = 0;
     __syncthreads();
     const int64_t seg = (ps.rows + 1023) / 1024 * 64, lo = min(wave * seg, ps.rows), hi = min(lo + seg, ps.rows);
-    count_rows(groups, lo, hi, ps.rows, G, counters + wave * (G + 1));
+    count_rows(groups, lo, hi, G, counters + wave * (G + 1));
     __syncthreads();
     plan_offsets(plan, ps, lds,
                  [&](int g) {
@@ -144,7 +161,7 @@ __global__ __launch_bounds__(1024) void plan_small_kernel(const int* groups, int
                      }
                  });
     __syncthreads();
-    place_rows(groups, lo, hi, ps.rows, G, bits, counters + wave * (G + 1), plan, ps);
+    place_rows(groups, lo, hi, G, bits, counters + wave * (G + 1), plan, ps);
 }
 
 // Larger: one wave per piece of rows; counts [G + 1][pieces], then run totals [G + 1] behind them
@@ -154,7 +171,7 @@ __global__ __launch_bounds__(64) void plan_count_kernel(const int* groups, int* 
     for (int i = threadIdx.x; i <= G; i += 64) counters[i] = 0;
     __syncthreads();
     const int64_t lo = min(blockIdx.x * seg, ps.rows), hi = min(lo + seg, ps.rows);
-    count_rows(groups, lo, hi, ps.rows, G, counters);
+    count_rows(groups, lo, hi, G, counters);
     __syncthreads();
     for (int i = threadIdx.x; i <= G; i += 64) scratch[(int64_t)i * pieces + blockIdx.x] = counters[i];
 }
@@ -185,7 +202,7 @@ __global__ __launch_bounds__(64) void plan_place_kernel(const int* groups, const
     for (int i = threadIdx.x; i <= G; i += 64) counters[i] = scratch[(int64_t)(G + 1) * pieces + i] + scratch[(int64_t)i * pieces + blockIdx.x];
     __syncthreads();
     const int64_t lo = min(blockIdx.x * seg, ps.rows), hi = min(lo + seg, ps.rows);
-    place_rows(groups, lo, hi, ps.rows, G, bits, counters, plan, ps);
+    place_rows(groups, lo, hi, G, bits, counters, plan, ps);
 }
 
 static bool plan_is_small(int64_t rows, int64_t groups) { return rows <= kSmallRows && 16 * (groups + 1) <= kSmallCounters; }
@@ -198,6 +215,7 @@ struct WeightShape {
     int64_t np, kp, nq, kq, fwd, bwd, bias_off, bytes;   // fwd: [P][np][kq], bwd: [P][kp][nq]
     int planes;
 };
+// (a packed orientation stays below 2^32 - 16 bytes, so that its planes are one buffer)
 static WeightShape weight_shape(int64_t n, int64_t k, int dtype) {
     WeightShape w{};
     w.planes = dtype == VH_BF16 ? 1 : 3;
@@ -209,6 +227,7 @@ static WeightShape weight_shape(int64_t n, int64_t k, int dtype) {
     w.bwd = w.kp * w.nq;
     w.bias_off = 2 * w.planes * (w.fwd + w.bwd);
     w.bytes = w.bias_off + 4 * w.np;
+    VH_REQUIRE(2 * w.planes * (w.fwd > w.bwd ? w.fwd : w.bwd) < 0xfffffff0ll, "a weight of %lld x %lld is too large", (long long)n, (long long)k);
     return w;
 }
 template <class T>
@@ -326,6 +345,25 @@ __device__ __forceinline__ void values8(const Source& s, const Eight<T>& v, floa
         decode4(v.code[1], scale, reinterpret_cast<float(&)[4]>(f[4]));
     }
 }
+// the first n of eight neighbouring results (at any alignment)
+template <class T>
+__device__ __forceinline__ void store8(T* p, const float (&v)[8], int n) {
+    if (n >= 8) {
+        if constexpr (sizeof(T) == 2) {
+            u32x4 o;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = f_to_bf(v[2 * e]) | (unsigned)f_to_bf(v[2 * e + 1]) << 16;
+            *reinterpret_cast<u32x4_any*>(p) = o;
+        } else {
+            *reinterpret_cast<f32x4_any*>(p) = f32x4{v[0], v[1], v[2], v[3]};
+            *reinterpret_cast<f32x4_any*>(p + 4) = f32x4{v[4], v[5], v[6], v[7]};
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (e < n) p[e] = from_f<T>(v[e]);
+    }
+}
 // f'(y) of eight columns applied to f
 template <class T>
 __device__ __forceinline__ void masked8(const Source& s, const Eight<T>& v, float slope, float (&f)[8]) {
@@ -357,18 +395,15 @@ struct AdapterGradArgs {
     int down_tiles;
 };
 
-template <class T, int RT>
-__global__ __launch_bounds__(256) void adapter_grad_kernel(AdapterGradArgs a) {
-    __shared__ __attribute__((aligned(16))) f32x4 red[2][RT * 8][64];
-    if ((int)blockIdx.x >= a.plan[kPlanItems]) return;
-    const int* it = a.plan + a.ps.o_item + 4 * (int64_t)blockIdx.x;
-    const int g = it[0], first = it[1], count = it[2], part = it[3];
+// `whole`: the tile's 128 columns exist (the same for the workgroup), so that its loads need no branch
+template <class T, int RT, bool UP, bool WHOLE>
+__device__ __forceinline__ void adapter_grad_tile(const AdapterGradArgs& a, int g, int first, int count, int part, int tile0, f32x4 (*red)[8][64]) {
     const int* slot_row = a.plan + a.ps.o_row;
-    const bool up = (int)blockIdx.y >= a.down_tiles;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, quad = lane >> 4;
-    const int C = up ? a.N : a.K, c0 = ((int)blockIdx.y - (up ? a.down_tiles : 0)) * 128 + 8 * l15, valid = C - c0, r = a.rank;
-    const float* small = up ? a.low : a.v;
-    const Source wide = up ? Source{a.dy, nullptr, a.ldy} : a.x;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l15 = lane & 15, quad = lane >> 4;
+    const int C = UP ? a.N : a.K, c0 = tile0 + 8 * l15, valid = WHOLE ? 8 : C - c0, r = a.rank;
+    const float* small = UP ? a.low : a.v;
+    const Source wide = UP ? Source{a.dy, nullptr, a.ldy} : a.x;
+    const bool masked = UP && a.mask.p != nullptr;
 
     f32x4 acc[RT][8];
 #pragma unroll
@@ -376,83 +411,106 @@ __global__ __launch_bounds__(256) void adapter_grad_kernel(AdapterGradArgs a) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) acc[j][e] = f32x4{0, 0, 0, 0};
 
-    const bool masked = up && a.mask.p != nullptr;
-    Eight<T> w, m;
-    float s[RT];
+    // a wave takes eight rows a step (two of each quad), the workgroup 32
+    Eight<T> w[2], m[2];
+    float s[2][RT];
     auto row_of = [&](int i) { return i < count ? slot_row[first + i] : -1; };
-    auto fetch = [&](int rid) {
-        read8<T>(wide, max(rid, 0), c0, rid >= 0 ? valid : 0, w);
-        if (masked) read8<T>(a.mask, max(rid, 0), c0, rid >= 0 ? valid : 0, m);
+    auto fetch = [&](const int (&rid)[2]) {
 #pragma unroll
-        for (int j = 0; j < RT; ++j) s[j] = rid >= 0 && 16 * j + l15 < r ? small[(int64_t)rid * r + 16 * j + l15] : 0.f;
+        for (int h = 0; h < 2; ++h) {
+            const int row = max(rid[h], 0);   // (a row that is not there is read as row 0 and counts with a factor of zero ...)
+            read8<T>(wide, row, c0, valid, w[h]);
+            if (masked) read8<T>(a.mask, row, c0, valid, m[h]);
+#pragma unroll
+            for (int j = 0; j < RT; ++j) s[h][j] = small[(int64_t)row * r + min(16 * j + l15, r - 1)];
+        }
     };
-    const int i0 = 4 * wave + quad;
-    fetch(row_of(i0));
-    int next = row_of(i0 + 16);
-    for (int i = 4 * wave; i < count; i += 16) {
-        float f[8], sc[RT];
-        values8<T>(wide, w, f);
-        if (masked) masked8<T>(a.mask, m, a.slope, f);
+    int rid[2], nxt[2];
+    const int i0 = 8 * wave + quad;
 #pragma unroll
-        for (int j = 0; j < RT; ++j) sc[j] = s[j];
-        fetch(next);
-        next = row_of(i + quad + 32);
+    for (int h = 0; h < 2; ++h) rid[h] = row_of(i0 + 4 * h);
+    fetch(rid);
 #pragma unroll
-        for (int j = 0; j < RT; ++j)
+    for (int h = 0; h < 2; ++h) nxt[h] = row_of(i0 + 32 + 4 * h);
+    for (int i = 8 * wave; i < count; i += 32) {
+        float f[2][8], sc[2][RT];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) acc[j][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(sc[j], f[e], acc[j][e], 0, 0, 0);
+        for (int h = 0; h < 2; ++h) {
+            values8<T>(wide, w[h], f[h]);
+            if (masked) masked8<T>(a.mask, m[h], a.slope, f[h]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[h][e] = rid[h] >= 0 ? f[h][e] : 0.f;   // (... on zeros: row 0 may hold anything)
+#pragma unroll
+            for (int j = 0; j < RT; ++j) sc[h][j] = rid[h] >= 0 && 16 * j + l15 < r ? s[h][j] : 0.f;
+            rid[h] = nxt[h];
+        }
+        if (i + 32 < count) {
+            fetch(rid);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) nxt[h] = row_of(i + quad + 64 + 4 * h);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < RT; ++j)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) acc[j][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(sc[h][j], f[h][e], acc[j][e], 0, 0, 0);
     }
-    // waves 2, 3 -> 0, 1 -> 0
-    if (wave >= 2) {
-#pragma unroll
-        for (int q = 0; q < RT * 8; ++q) red[wave - 2][q][lane] = acc[q / 8][q % 8];
-    }
-    __syncthreads();
-    if (wave < 2) {
-#pragma unroll
-        for (int q = 0; q < RT * 8; ++q) acc[q / 8][q % 8] += red[wave][q][lane];
-    }
-    __syncthreads();
-    if (wave == 1) {
-#pragma unroll
-        for (int q = 0; q < RT * 8; ++q) red[0][q][lane] = acc[q / 8][q % 8];
-    }
-    __syncthreads();
-    if (wave != 0) return;
-#pragma unroll
-    for (int q = 0; q < RT * 8; ++q) acc[q / 8][q % 8] += red[0][q][lane];
-
-    const float scale = up ? a.scale : 1.f;   // (v has it)
+    // the four waves' sums, in their order; 16 ranks x 128 columns at a time, every thread eight neighbouring results
     const int64_t pair = (int64_t)r * (a.K + a.N);
-    float* po = part >= 0 ? a.parts + part * pair + (up ? (int64_t)r * a.K : 0) : nullptr;
+    float* po = part >= 0 ? a.parts + part * pair + (UP ? (int64_t)r * a.K : 0) : nullptr;
+    T* dst = UP ? (T*)a.dup + (int64_t)g * a.N * r : (T*)a.ddown + (int64_t)g * r * a.K;
 #pragma unroll
     for (int j = 0; j < RT; ++j) {
-        const int rank = 16 * j + 4 * quad;
-        if (up) {
-            T* dst = (T*)a.dup + (int64_t)g * a.N * r;
+        if (j) __syncthreads();
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (e < valid) {
+        for (int e = 0; e < 8; ++e) red[wave][e][lane] = acc[j][e];
+        __syncthreads();
+        float v[8];
+        int64_t at;
+        int n;
+        if constexpr (UP) {   // up [N][rank]: thread = column, eight ranks
+            const int col = tid >> 1, rank = 16 * j + 8 * (tid & 1), q = 2 * (tid & 1);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (rank + i < r) {
-                            const int64_t at = (int64_t)(c0 + e) * r + rank + i;
-                            if (po) po[at] = acc[j][e][i] * scale; else dst[at] = from_f<T>(acc[j][e][i] * scale);
-                        }
-                }
-        } else {
-            T* dst = (T*)a.ddown + (int64_t)g * r * a.K;
+            for (int h = 0; h < 2; ++h) {
+                f32x4 t = red[0][col & 7][16 * (q + h) + (col >> 3)];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (rank + i < r) {
-                    const int64_t at = (int64_t)(rank + i) * a.K + c0;
+                for (int wv = 1; wv < 4; ++wv) t += red[wv][col & 7][16 * (q + h) + (col >> 3)];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (e < valid) {
-                            if (po) po[at + e] = acc[j][e][i]; else dst[at + e] = from_f<T>(acc[j][e][i]);
-                        }
-                }
+                for (int i = 0; i < 4; ++i) v[4 * h + i] = t[i] * a.scale;
+            }
+            at = (int64_t)(tile0 + col) * r + rank;
+            n = tile0 + col < C ? r - rank : 0;
+        } else {              // down [rank][K]: thread = rank, eight columns
+            const int rk = tid >> 4, cc = tid & 15;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                float t = 0.f;
+#pragma unroll
+                for (int wv = 0; wv < 4; ++wv) t += red[wv][e][16 * (rk >> 2) + cc][rk & 3];
+                v[e] = t;   // (v has the scale)
+            }
+            at = (int64_t)(16 * j + rk) * a.K + tile0 + 8 * cc;
+            n = 16 * j + rk < r ? C - tile0 - 8 * cc : 0;
         }
+        if (po) store8<float>(po + at, v, n);
+        else store8<T>(dst + at, v, n);
+    }
+}
+template <class T, int RT>
+__global__ __launch_bounds__(256) void adapter_grad_kernel(AdapterGradArgs a) {
+    __shared__ __attribute__((aligned(16))) f32x4 red[4][8][64];
+    if ((int)blockIdx.x >= a.plan[kPlanItems]) return;
+    const int* it = a.plan + a.ps.o_item + 4 * (int64_t)blockIdx.x;
+    const int g = it[0], first = it[1], count = it[2], part = it[3];
+    const bool up = (int)blockIdx.y >= a.down_tiles;
+    const int tile0 = 128 * ((int)blockIdx.y - (up ? a.down_tiles : 0));
+    if (up) {
+        if (tile0 + 128 <= a.N) adapter_grad_tile<T, RT, true, true>(a, g, first, count, part, tile0, red);
+        else adapter_grad_tile<T, RT, true, false>(a, g, first, count, part, tile0, red);
+    } else {
+        if (tile0 + 128 <= a.K) adapter_grad_tile<T, RT, false, true>(a, g, first, count, part, tile0, red);
+        else adapter_grad_tile<T, RT, false, false>(a, g, first, count, part, tile0, red);
     }
 }
 template <class T>
@@ -467,6 +525,24 @@ __global__ __launch_bounds__(256) void adapter_join_kernel(AdapterGradArgs a) {
     for (int p = 0; p < n; ++p) s += a.parts[(part + p) * pair + i];
     if (i < half) ((T*)a.ddown)[(int64_t)g * half + i] = from_f<T>(s);
     else ((T*)a.dup)[(int64_t)g * a.N * a.rank + i - half] = from_f<T>(s);
+}
+
+// up [N][rank] of the adapters that some row asks for -> [rank][N], the orientation that dy is contracted with: the projection
+// reads its inner operands 16 bytes at a time along the depth
+template <class T>
+__global__ __launch_bounds__(256) void turn_up_kernel(const T* up, T* out, int N, int r, const int* plan, PlanShape ps) {
+    __shared__ T tile[64][kMaxRank + 1];
+    if ((int)blockIdx.x >= plan[kPlanItems]) return;
+    const int* it = plan + ps.o_item + 4 * (int64_t)blockIdx.x;
+    if (it[2] == 0 || (blockIdx.x > 0 && it[-4] == it[0])) return;   // no rows; a later piece of the same group
+    const int64_t base = (int64_t)it[0] * N * r;
+    const int n0 = blockIdx.y * 64, n = min(64, N - n0);
+    for (int i = threadIdx.x; i < n * r; i += 256) tile[i / r][i % r] = up[base + (int64_t)n0 * r + i];
+    __syncthreads();
+    for (int i = threadIdx.x; i < 64 * r; i += 256) {
+        const int j = i >> 6, c = i & 63;
+        if (c < n) out[base + (int64_t)j * N + n0 + c] = tile[c][j];
+    }
 }
 
 // =====================================================================================================================
@@ -566,7 +642,7 @@ __global__ __launch_bounds__(512) void few_kernel(FewArgs a) {
 
 // =====================================================================================================================
 // Gradient of the shared projection from checkpoints:  dW = p^T x  [N][K],  db = sum p  [N]
-// Tile 128 x 128, split over the rows; both operands are contracted along their slow dimension: row-major LDS tiles [32 rows][128
+// Tile 128 x 128, split over the rows; both operands are contracted along their slow dimension: row-major LDS tiles [64 rows][128
 // columns] read by the transposing LDS instruction.  x's values are exact in bf16 (one plane), so float32 dy costs three products, not
 // six.  256-byte tile rows: the 32-byte pieces are XOR-permuted by the row so that the eight rows of half a read differ in their banks.
 // =====================================================================================================================
@@ -585,38 +661,35 @@ __device__ __forceinline__ s16x4 read_tr(const unsigned char* p) {
 }
 __device__ __forceinline__ int tr_swz(int row) { return (row & 3) | ((row >> 1) & 4); }
 
-template <class T>
-__global__ __launch_bounds__(256) void weight_grad_kernel(WeightGradArgs a) {
-    constexpr int P = Elem<T>::planes, BR = 32, TB = BR * 256;
-    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];   // [2][P + 1][TB]: planes of p, then x
+template <class T, bool WHOLE>
+__device__ __forceinline__ void weight_grad_tile(const WeightGradArgs& a, int n0, int k0, unsigned char* smem) {
+    constexpr int P = Elem<T>::planes, BR = 64, TB = BR * 256;   // smem: [2][P + 1][TB]: planes of p, then x
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l15 = lane & 15, quad = lane >> 4;
-    const int n0 = ((int)blockIdx.x / a.k_tiles) * 128, k0 = ((int)blockIdx.x % a.k_tiles) * 128;
     const int64_t lo = blockIdx.y * a.split_rows, hi = min(lo + a.split_rows, a.rows);
-    const int wn = wave >> 1, wk = wave & 1;
-    const bool masked = a.mask.p != nullptr, sums = k0 == 0;
+    const int half = wave >> 2, wn = (wave >> 1) & 1, wk = wave & 1;   // waves 0-3 take rows 0-31 of a tile, waves 4-7 rows 32-63
+    const bool masked = a.mask.p != nullptr;
     const Source dy = {a.dy, nullptr, a.ldy};
 
-    // pieces of eight columns: thread t has column piece t % 16 of rows t / 16 and t / 16 + 16
+    // pieces of eight columns: thread t has column piece t % 16 of rows t / 16 and t / 16 + 32
     const int pc = tid & 15, pr = tid >> 4;
     Eight<T> pw[2], mw[2], xw[2];
     auto fetch = [&](int64_t row0) {
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-            const int64_t row = row0 + pr + 16 * q;
-            const bool in = row < hi;
-            const int64_t at = in ? row : lo;
-            read8<T>(dy, at, n0 + 8 * pc, in ? a.N - n0 - 8 * pc : 0, pw[q]);
-            if (masked) read8<T>(a.mask, at, n0 + 8 * pc, in ? a.N - n0 - 8 * pc : 0, mw[q]);
-            read8<T>(a.x, at, k0 + 8 * pc, in ? a.K - k0 - 8 * pc : 0, xw[q]);
+            const int64_t at = min(row0 + pr + 32 * q, hi - 1);   // (behind the last row: read again, and set to zero in keep)
+            read8<T>(dy, at, n0 + 8 * pc, WHOLE ? 8 : a.N - n0 - 8 * pc, pw[q]);
+            if (masked) read8<T>(a.mask, at, n0 + 8 * pc, WHOLE ? 8 : a.N - n0 - 8 * pc, mw[q]);
+            read8<T>(a.x, at, k0 + 8 * pc, WHOLE ? 8 : a.K - k0 - 8 * pc, xw[q]);
         }
     };
     float bsum[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) bsum[e] = 0.f;
-    auto keep = [&](unsigned char* buf) {
+    auto keep = [&](unsigned char* buf, int64_t row0) {
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-            const int row = pr + 16 * q, at = row * 256 + (((pc >> 1) ^ tr_swz(row)) * 32 + (pc & 1) * 16);
+            const int row = pr + 32 * q, at = row * 256 + (((pc >> 1) ^ tr_swz(row)) * 32 + (pc & 1) * 16);
+            const bool in = row0 + row < hi;
             float f[8];
             values8<T>(dy, pw[q], f);
             if (masked) masked8<T>(a.mask, mw[q], a.slope, f);
@@ -624,6 +697,7 @@ __global__ __launch_bounds__(256) void weight_grad_kernel(WeightGradArgs a) {
             o.zero();
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
+                f[e] = in ? f[e] : 0.f;
                 bsum[e] += f[e];
                 o.set(e, from_f<T>(f[e]));
             }
@@ -633,7 +707,10 @@ __global__ __launch_bounds__(256) void weight_grad_kernel(WeightGradArgs a) {
             values8<T>(a.x, xw[q], f);
             u32x4 xv;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) xv[e] = (__float_as_uint(f[2 * e]) >> 16) | (__float_as_uint(f[2 * e + 1]) & 0xffff0000u);   // exact
+            for (int e = 0; e < 4; ++e) {
+                const unsigned both = (__float_as_uint(f[2 * e]) >> 16) | (__float_as_uint(f[2 * e + 1]) & 0xffff0000u);   // exact
+                xv[e] = in ? both : 0u;
+            }
             *reinterpret_cast<u32x4*>(buf + P * TB + at) = xv;
         }
     };
@@ -643,8 +720,8 @@ __global__ __launch_bounds__(256) void weight_grad_kernel(WeightGradArgs a) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
 
-    // lane's share of a transposed operand: rows 8 quad + l15 / 4 (+ 4), columns 4 (l15 % 4) of the 16
-    const int fr = 8 * quad + (l15 >> 2);
+    // lane's share of a transposed operand: rows 8 quad + l15 / 4 (+ 4) of the wave's 32, columns 4 (l15 % 4) of the 16
+    const int fr = 32 * half + 8 * quad + (l15 >> 2);
     auto frag = [&](const unsigned char* buf, int col0) {
         const int piece = (col0 >> 4), off = 8 * (l15 & 3);
         const s16x4 a0 = read_tr(buf + fr * 256 + ((piece ^ tr_swz(fr)) * 32) + off);
@@ -652,7 +729,7 @@ __global__ __launch_bounds__(256) void weight_grad_kernel(WeightGradArgs a) {
         return __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
     };
     fetch(lo);
-    keep(smem);
+    keep(smem, lo);
     __syncthreads();
     int cur = 0;
     for (int64_t row0 = lo; row0 < hi; row0 += BR) {
@@ -660,6 +737,7 @@ __global__ __launch_bounds__(256) void weight_grad_kernel(WeightGradArgs a) {
         unsigned char* nxt = smem + (cur ^ 1) * (P + 1) * TB;
         const bool more = row0 + BR < hi;
         if (more) fetch(row0 + BR);
+        __builtin_amdgcn_sched_barrier(0);
         s16x8 xf[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) xf[j] = frag(buf + P * TB, wk * 64 + 16 * j);
@@ -673,33 +751,56 @@ __global__ __launch_bounds__(256) void weight_grad_kernel(WeightGradArgs a) {
 #pragma unroll
                 for (int p = P - 1; p >= 0; --p) acc[i][j] = mfma32(xf[j], pf[p], acc[i][j]);   // D[k column][n column]
         }
-        if (more) keep(nxt);
+        __builtin_amdgcn_sched_barrier(0);
+        if (more) keep(nxt, row0 + BR);
         __syncthreads();
         cur ^= 1;
     }
+    // the two halves' sums
+    f32x4* red = reinterpret_cast<f32x4*>(smem);   // [4 waves][16][64]: the tiles are done with (barrier above)
+    if (half) {
+#pragma unroll
+        for (int q = 0; q < 16; ++q) red[((wave & 3) * 16 + q) * 64 + lane] = acc[q / 4][q % 4];
+    }
+    __syncthreads();
     float* out = a.parts + blockIdx.y * ((int64_t)a.N * a.K + a.N);
+    if (!half) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int n = n0 + wn * 64 + 16 * i + l15;
+        for (int i = 0; i < 4; ++i) {
+            const int n = n0 + wn * 64 + 16 * i + l15;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int k = k0 + wk * 64 + 16 * j + 4 * quad;
+            for (int j = 0; j < 4; ++j) {
+                const int k = k0 + wk * 64 + 16 * j + 4 * quad;
+                const f32x4 v = acc[i][j] + red[(wave * 16 + 4 * i + j) * 64 + lane];
+                if (WHOLE) {
+                    *reinterpret_cast<f32x4_any*>(out + (int64_t)n * a.K + k) = v;
+                } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (n < a.N && k + e < a.K) out[(int64_t)n * a.K + k + e] = acc[i][j][e];
+                    for (int e = 0; e < 4; ++e)
+                        if (n < a.N && k + e < a.K) out[(int64_t)n * a.K + k + e] = v[e];
+                }
+            }
         }
     }
-    if (sums) {
-        float* s = reinterpret_cast<float*>(smem);   // [16 rows][128]: the tiles are done with (barrier above)
+    if (k0 == 0) {
+        __syncthreads();
+        float* s = reinterpret_cast<float*>(smem);   // [32 rows][128]
 #pragma unroll
         for (int e = 0; e < 8; ++e) s[pr * 128 + 8 * pc + e] = bsum[e];
         __syncthreads();
         if (tid < 128 && n0 + tid < a.N) {
             float v = 0.f;
-            for (int i = 0; i < 16; ++i) v += s[i * 128 + tid];
+            for (int i = 0; i < 32; ++i) v += s[i * 128 + tid];
             out[(int64_t)a.N * a.K + n0 + tid] = v;
         }
     }
+}
+template <class T>
+__global__ __launch_bounds__(512) void weight_grad_kernel(WeightGradArgs a) {
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    const int n0 = ((int)blockIdx.x / a.k_tiles) * 128, k0 = ((int)blockIdx.x % a.k_tiles) * 128;
+    if (n0 + 128 <= a.N && k0 + 128 <= a.K) weight_grad_tile<T, true>(a, n0, k0, smem);
+    else weight_grad_tile<T, false>(a, n0, k0, smem);
 }
 template <class T>
 __global__ __launch_bounds__(256) void weight_join_kernel(const float* parts, int splits, int64_t n_weight, int64_t total, T* dw, T* db) {
@@ -710,13 +811,13 @@ __global__ __launch_bounds__(256) void weight_join_kernel(const float* parts, in
     if (i < n_weight) dw[i] = from_f<T>(s);
     else if (db != nullptr) db[i - n_weight] = from_f<T>(s);
 }
-// about 512 workgroups, at least 64 rows each
+// about 256 workgroups, at least 128 rows each
 static int64_t weight_splits(int64_t rows, int64_t n, int64_t k, int64_t* split_rows) {
     const int64_t tiles = ceil_div(n, 128) * ceil_div(k, 128);
-    int64_t want = ceil_div(512, tiles);
-    const int64_t most = ceil_div(rows, 64);
+    int64_t want = ceil_div(256, tiles);
+    const int64_t most = ceil_div(rows, 128);
     want = want < most ? want : most;
-    *split_rows = round_up(ceil_div(rows, want), 32);
+    *split_rows = round_up(ceil_div(rows, want), 64);
     return ceil_div(rows, *split_rows);
 }
 
@@ -730,8 +831,8 @@ static void check_groups(int64_t g) { VH_REQUIRE(g >= 1 && g <= kMaxGroups, "the
 static void check_rank(int64_t r) { VH_REQUIRE(r >= 1 && r <= kMaxRank, "the rank must be in [1, %d], not %lld", kMaxRank, (long long)r); }
 static void check_ptr(const void* p, const char* what) { VH_REQUIRE(p != nullptr, "%s is NULL", what); }
 static void check_slope(int activation, float slope) {
-    // the derivative is taken from the sign of the value, which a negative slope would lose
-    VH_REQUIRE(!activation || (slope >= 0.f && slope < __builtin_inff()), "the negative slope must be finite and >= 0");
+    // below 0 the sign of the value would not tell the derivative; up to 1 the activation is max(v, slope v)
+    VH_REQUIRE(!activation || (slope >= 0.f && slope <= 1.f), "the negative slope must be in [0, 1]");
 }
 static void check_held(const uint8_t* codes, const uint8_t* exps, const char* what) {
     VH_REQUIRE((codes == nullptr) == (exps == nullptr), "%s: codes and exponents come together", what);
@@ -787,6 +888,14 @@ static void adapter_grads(const AdapterGradArgs& a, hipStream_t s) {
         adapter_join_kernel<T><<<dim3((unsigned)multis, (unsigned)ceil_div((int64_t)a.rank * (a.K + a.N), 256)), 256, 0, s>>>(a);
         VH_HIP(hipGetLastError());
     }
+}
+static int64_t turned_words(int64_t groups, int64_t n, int64_t rank, int dtype) {
+    return round_up(dtype == VH_BF16 ? ceil_div(groups * n * rank, 2) : groups * n * rank, 4);
+}
+template <class T>
+static void turn_up(const void* up, void* out, int64_t n, int64_t r, const int* plan, const PlanShape& ps, hipStream_t s) {
+    turn_up_kernel<T><<<dim3((unsigned)ps.items, (unsigned)ceil_div(n, 64)), 256, 0, s>>>((const T*)up, (T*)out, (int)n, (int)r, plan, ps);
+    VH_HIP(hipGetLastError());
 }
 static int64_t grad_parts(const PlanShape& ps) { return ps.rows > ps.item_rows ? 2 * (ps.rows / ps.item_rows) : 0; }
 
@@ -913,7 +1022,9 @@ int vh_adapt_forward(const vh_adapt_layer* l, const void* x, int64_t ldx, int64_
         a.exps = exponents;
         a.plan = plan;
         a.ps = plan_shape(rows, l->groups);
-        a.dma = es == 2 && l->k % 8 == 0 && ldx % 8 == 0 && (uintptr_t)x % 16 == 0;
+        const int64_t x_bytes = ((rows - 1) * ldx + l->k) * es;
+        a.dma = es == 2 && l->k % 8 == 0 && ldx % 8 == 0 && (uintptr_t)x % 16 == 0 && x_bytes < 0xfffffff0ll;   // (down is read at any alignment)
+        a.x_bytes = a.dma ? (unsigned)x_bytes : 0;
         run_linear(a, l->dtype, false, (hipStream_t)stream);
     });
 }
@@ -953,7 +1064,7 @@ int vh_adapt_forward_few(const vh_adapt_layer* l, const void* x, int64_t ldx, in
     });
 }
 
-int vh_adapt_backward_size(int64_t rows, int64_t groups, int64_t n, int64_t k, int64_t rank, int64_t* scratch_words) {
+int vh_adapt_backward_size(int64_t rows, int64_t groups, int64_t n, int64_t k, int64_t rank, int dtype, int64_t* scratch_words) {
     return guarded([&] {
         check_rows(rows);
         check_groups(groups);
@@ -962,7 +1073,8 @@ int vh_adapt_backward_size(int64_t rows, int64_t groups, int64_t n, int64_t k, i
         check_rank(rank);
         check_ptr(scratch_words, "scratch_words");
         const PlanShape ps = plan_shape(rows, groups);
-        *scratch_words = round_up(rows * rank, 4) + grad_parts(ps) * rank * (n + k);
+        check_dtype(dtype);
+        *scratch_words = round_up(rows * rank, 4) + turned_words(groups, n, rank, dtype) + grad_parts(ps) * rank * (n + k);
     });
 }
 
@@ -996,7 +1108,11 @@ int vh_adapt_backward(const vh_adapt_layer* l, const void* dy, int64_t lddy, con
         a.w = (const bf16_t*)l->packed + ws.planes * ws.fwd;
         a.w_plane = ws.bwd;
         a.ldw = (int)ws.nq;
-        a.inner = l->up;
+        float* turned = scratch + round_up(rows * l->rank, 4);
+        VH_REQUIRE((uintptr_t)scratch % 16 == 0, "scratch must be 16-byte aligned");
+        if (l->dtype == VH_BF16) turn_up<bf16_t>(l->up, turned, l->n, l->rank, plan, ps, (hipStream_t)stream);
+        else turn_up<float>(l->up, turned, l->n, l->rank, plan, ps, (hipStream_t)stream);
+        a.inner = turned;
         a.outer = l->down;
         a.K = (int)l->n;
         a.N = (int)l->k;
@@ -1017,7 +1133,7 @@ int vh_adapt_backward(const vh_adapt_layer* l, const void* dy, int64_t lddy, con
         g.v = v;
         g.ddown = ddown;
         g.dup = dup;
-        g.parts = scratch + round_up(rows * l->rank, 4);
+        g.parts = turned + turned_words(l->groups, l->n, l->rank, l->dtype);
         g.K = (int)l->k;
         g.N = (int)l->n;
         g.rank = (int)l->rank;
@@ -1106,11 +1222,13 @@ int vh_checkpoint8_weight_grad(const void* dy, int64_t lddy, const vh_held* x, c
         const dim3 grid((unsigned)tiles, (unsigned)splits);
         hipStream_t s = (hipStream_t)stream;
         if (dtype == VH_BF16) {
-            weight_grad_kernel<bf16_t><<<grid, 256, 2 * 2 * 32 * 256, s>>>(a);
+            weight_grad_kernel<bf16_t><<<grid, 512, 2 * 2 * 64 * 256, s>>>(a);
             VH_HIP(hipGetLastError());
             weight_join_kernel<bf16_t><<<(unsigned)ceil_div(total, 256), 256, 0, s>>>(scratch, (int)splits, n * k, total, (bf16_t*)dweight, (bf16_t*)dbias);
         } else {
-            weight_grad_kernel<float><<<grid, 256, 2 * 4 * 32 * 256, s>>>(a);
+            constexpr int bytes = 2 * 4 * 64 * 256;
+            VH_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(weight_grad_kernel<float>), hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+            weight_grad_kernel<float><<<grid, 512, bytes, s>>>(a);
             VH_HIP(hipGetLastError());
             weight_join_kernel<float><<<(unsigned)ceil_div(total, 256), 256, 0, s>>>(scratch, (int)splits, n * k, total, (float*)dweight, (float*)dbias);
         }

@@ -53,12 +53,15 @@ template <class T> __device__ __forceinline__ T from_f(float x);
 template <> __device__ __forceinline__ float from_f<float>(float x) { return x; }
 template <> __device__ __forceinline__ bf16_t from_f<bf16_t>(float x) { return f_to_bf(x); }
 
+// (global memory said aloud: a pointer chosen between two objects would be read by flat loads, which also count as LDS accesses)
+#define VH_GLOBAL(type, p) (const __attribute__((address_space(1))) type*)(p)
+
 // ---- eight consecutive elements as they were read -------------------------------------------------------------------------
 template <class T> struct Raw8;
 template <> struct Raw8<bf16_t> {
     u32x4 v;
     __device__ __forceinline__ void zero() { v = u32x4{0, 0, 0, 0}; }
-    __device__ __forceinline__ void load(const bf16_t* p) { v = *reinterpret_cast<const u32x4_any*>(p); }
+    __device__ __forceinline__ void load(const bf16_t* p) { v = *(VH_GLOBAL(u32x4_any, p)); }
     __device__ __forceinline__ void set(int e, bf16_t x) {   // e: a constant after unrolling; the element's bits are zero before
         v[e >> 1] |= (unsigned)x << (16 * (e & 1));
     }
@@ -68,8 +71,8 @@ template <> struct Raw8<float> {
     f32x4 a, b;
     __device__ __forceinline__ void zero() { a = f32x4{0, 0, 0, 0}; b = a; }
     __device__ __forceinline__ void load(const float* p) {
-        a = *reinterpret_cast<const f32x4_any*>(p);
-        b = *reinterpret_cast<const f32x4_any*>(p + 4);
+        a = *(VH_GLOBAL(f32x4_any, p));
+        b = *(VH_GLOBAL(f32x4_any, p + 4));
     }
     __device__ __forceinline__ void set(int e, float x) {
         if (e < 4) a[e] = x; else b[e - 4] = x;
@@ -87,20 +90,10 @@ __device__ __forceinline__ Raw8<T> load8(const T* p, int valid) {
     } else if (valid > 0) {
 #pragma unroll
         for (int e = 0; e < 7; ++e)
-            if (e < valid) r.set(e, p[e]);
+            if (e < valid) r.set(e, *(VH_GLOBAL(T, p + e)));
     }
     return r;
 }
-template <class T>
-__device__ __forceinline__ Raw8<T> load8_strided(const T* p, int64_t stride, int valid) {
-    Raw8<T> r;
-    r.zero();
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-        if (e < valid) r.set(e, p[e * stride]);
-    return r;
-}
-
 // ---- operand planes ---------------------------------------------------------------------------------------------------------
 // the three cuts of a float32; an infinity stays whole in the first (inf - inf would make a NaN of it), a NaN stays one
 __device__ __forceinline__ void split3(float x, unsigned& h, unsigned& m, unsigned& l) {
@@ -241,7 +234,8 @@ struct LinArgs {
     uint8_t* exps;            // row stride ldc / 32
     const int* plan;
     PlanShape ps;
-    int dma;                  // x rows are 16-byte aligned and K is a multiple of 8
+    int dma;                  // x rows are 16-byte aligned, K is a multiple of 8 and x ends below 2^32 - 16 bytes: ...
+    unsigned x_bytes;         // ... its size, as a buffer
 };
 void launch_linear_bf16(const LinArgs& a, bool backward, hipStream_t s);
 void launch_linear_f32(const LinArgs& a, bool backward, hipStream_t s);

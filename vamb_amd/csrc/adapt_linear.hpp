@@ -18,14 +18,23 @@
 #include "adapt_common.hpp"
 #include "common.hpp"
 
+#include <type_traits>
+
 namespace vh {
 namespace adapt {
 
-__device__ __forceinline__ void dma16(const void* src, unsigned char* lds_wave_base) {
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
-                                     (__attribute__((address_space(3))) void*)lds_wave_base, 16, 0, 0);
+// 16 bytes per lane from base + offset to the LDS.  Buffer loads, not global_load_lds: that one is a flat instruction to the compiler, which
+// then turns every wait on an LDS read or a register load into a drain of all of them (seen in the ISA: vmcnt(0) in the middle of a
+// tile).  An offset at or behind the buffer's end reads zeros.
+typedef __amdgpu_buffer_rsrc_t Buffer;
+__device__ __forceinline__ Buffer buffer_of(const void* p, unsigned bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)bytes, 0x00020000);
 }
-static __device__ const uint4 g_zero16 = {0, 0, 0, 0};
+__device__ __forceinline__ void dma16(Buffer b, unsigned offset, unsigned char* lds_wave_base) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(b, (__attribute__((address_space(3))) void*)lds_wave_base, 16, (int)offset, 0, 0, 0);
+}
+constexpr unsigned kBehind = 0xfffffff0u;   // behind every buffer (their sizes are below it)
+static __device__ const uint4 g_zero32[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
 
 template <int PU>
 __device__ __forceinline__ void cut4(const f32x4 v, s16x4 (&o)[PU]) {
@@ -44,89 +53,137 @@ __device__ __forceinline__ void cut4(const f32x4 v, s16x4 (&o)[PU]) {
 }
 __device__ __forceinline__ f32x4 mfma16(s16x4 a, s16x4 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a, b, c, 0, 0, 0); }
 
-// four consecutive elements at p (valid of them) as operand planes
-__device__ __forceinline__ void load4_planes(const bf16_t* p, int64_t stride, int valid, s16x4 (&o)[1]) {
-    if (stride == 1 && valid >= 4) {
-        o[0] = __builtin_bit_cast(s16x4, (u32x2)*reinterpret_cast<const u32x2_any*>(p));
+// Four elements, `stride` apart, the first `valid` of them (zeros behind): no branch on lanes, what is not there is read from the
+// block of zeros.  `vec`: stride 1, and valid is four or none (the same for the whole wave).
+__device__ __forceinline__ void load4(const bf16_t* p, int64_t stride, int valid, bool vec, u32x2& o) {
+    if (vec) {
+        o = (u32x2)*(VH_GLOBAL(u32x2_any, valid >= 4 ? p : (const bf16_t*)g_zero32));
         return;
     }
-    s16x4 r = {0, 0, 0, 0};
+    bf16_t e[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-        if (e < valid) r[e] = (short)p[e * stride];
-    o[0] = r;
+    for (int i = 0; i < 4; ++i) e[i] = *(VH_GLOBAL(bf16_t, i < valid ? p + i * stride : (const bf16_t*)g_zero32));
+    o = u32x2{e[0] | (unsigned)e[1] << 16, e[2] | (unsigned)e[3] << 16};
 }
-__device__ __forceinline__ void load4_planes(const float* p, int64_t stride, int valid, s16x4 (&o)[3]) {
-    f32x4 r = {0, 0, 0, 0};
-    if (stride == 1 && valid >= 4) {
-        r = *reinterpret_cast<const f32x4_any*>(p);
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (e < valid) r[e] = p[e * stride];
+__device__ __forceinline__ void load4(const float* p, int64_t stride, int valid, bool vec, f32x4& o) {
+    if (vec) {
+        o = *(VH_GLOBAL(f32x4_any, valid >= 4 ? p : (const float*)g_zero32));
+        return;
     }
-    cut4<3>(r, o);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = *(VH_GLOBAL(float, i < valid ? p + i * stride : (const float*)g_zero32));
 }
+__device__ __forceinline__ void planes4(const u32x2& r, s16x4 (&o)[1]) { o[0] = __builtin_bit_cast(s16x4, r); }
+__device__ __forceinline__ void planes4(const f32x4& r, s16x4 (&o)[3]) { cut4<3>(r, o); }
+template <class T> struct Raw4;
+template <> struct Raw4<bf16_t> { typedef u32x2 type; };
+template <> struct Raw4<float> { typedef f32x4 type; };
 
-// NT = 0: only `low` is computed (a backward pass without dx)
-template <class T, int NT, int MS, int RT, bool TRANS, bool DMA>
-__global__ __launch_bounds__(256) void linear_kernel(LinArgs a) {
+// A tile shape: WM x WN waves, each MS x NT subtiles of 16 x 16; two tile buffers of depth BK in the LDS.
+// NT = 0: only `low` is computed (a backward pass without dx).
+template <int WM_, int WN_, int MS_, int NT_, int BK_>
+struct Shape {
+    static constexpr int WM = WM_, WN = WN_, MS = MS_, NT = NT_, BK = BK_;
+};
+
+template <class T, class S, int RT, bool TRANS, bool DMA>
+__global__ __launch_bounds__(64 * S::WM * S::WN) void linear_kernel(LinArgs a) {
+    constexpr int WM = S::WM, WN = S::WN, MS = S::MS, NT = S::NT, NW = WM * WN, THREADS = 64 * NW;
     constexpr int P = Elem<T>::planes;
     constexpr int PU = P == 1 ? 2 : 3;
-    constexpr int BK = P == 1 ? 64 : 32;
-    constexpr int CH = BK / 8;                     // 16-byte pieces of a tile row
-    constexpr int BM = 64 * MS, BN = 16 * NT;
+    constexpr int BK = S::BK;
+    constexpr int CH = BK / 8;                          // 16-byte pieces of a tile row
+    constexpr int BM = 16 * MS * WM, BN = 16 * NT * WN;
     constexpr int XB = BM * BK * 2, WB = BN * BK * 2;   // bytes of a plane
     constexpr int BUF = P * (XB + WB);
-    constexpr int PX = BM * CH / 256;              // x pieces per thread (and plane)
-    constexpr int NWI = P * BN * CH / 64;          // W pieces, one wave instruction each
-    constexpr int KC = BK / 32;                    // 32-deep products per tile
+    constexpr int PX = BM * CH / THREADS;               // x pieces per thread (and plane)
+    constexpr int NWI = P * BN * CH / 64;               // W pieces, one wave instruction each
+    constexpr int QW = NWI ? (NWI + NW - 1) / NW : 1;
+    constexpr int KC = BK / 32;                         // 32-deep products per tile
+    constexpr int MU = MS / WN;                         // subtiles whose u this wave computes (its share of the WN waves on the same rows)
+    static_assert(PX >= 1 && BM * CH % THREADS == 0 && MS % WN == 0 && (!DMA || P == 1), "tile shape");
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int l15 = lane & 15, quad = lane >> 4;
-    const int n_sub = a.plan[kPlanSubs];
-    const int row_tiles = (n_sub + 4 * MS - 1) / (4 * MS), col_tiles = NT ? (a.N + BN - 1) / (BN ? BN : 1) : 1;
-    // workgroup b runs on XCD b % 8: each XCD gets a contiguous run of tiles, the column tiles of a row tile beside each other (its
-    // x rows come from that XCD's L2 after the first)
-    const int total = row_tiles * col_tiles, xcd = blockIdx.x & 7, local = blockIdx.x >> 3;
-    if (local >= (total >> 3) + (xcd < (total & 7))) return;
-    const int t = __builtin_amdgcn_readfirstlane(xcd * (total >> 3) + min(xcd, total & 7) + local);
-    const int tile = t / col_tiles, n0 = (t % col_tiles) * BN;
+    const int l15 = lane & 15, quad = lane >> 4, wm = wave / WN, wn = wave % WN;
+    // workgroup b runs on XCD b % 8: a row tile's column tiles are eight apart, so that XCD's L2 has its x rows after the first
+    const int col_tiles = NT ? (a.N + BN - 1) / (BN ? BN : 1) : 1;
+    const int bid = blockIdx.x, tile = bid / (8 * col_tiles) * 8 + (bid & 7), n0 = (bid / 8 % col_tiles) * BN;
     const int* slot_row = a.plan + a.ps.o_row;
     const int* sub_group = a.plan + a.ps.o_sub;
     const int K = a.K, r = a.rank, nk = (K + BK - 1) / BK;
+    const int n_sub = a.plan[kPlanSubs];
 
-    auto swz = [](int row) { return P == 1 ? ((row >> 1) & 7) : ((row >> 2) & 3); };
+    // 16-byte pieces of a tile row are XOR-permuted by half the row's number within the operand: the 16 rows of an operand read then
+    // take the LDS's full 256 B a clock (measured; permuted by a quarter of it, rows of four pieces took 128).  Rows of W are read in another order: a lane's four results of the subtiles 2 i and
+    // 2 i + 1 are eight consecutive columns, 32 i + 8 (l15 / 4) + 4 (0 or 1) + l15 % 4 being the column of operand row l15.
+    auto swz = [](int row) { return (row >> 1) & (CH - 1); };
+    auto swz_w = [](int row) { return ((row >> 1) & 1) | ((row >> 2) & (CH - 2)); };
+    auto w_row = [&](int n) { return 32 * (n >> 1) + 8 * (l15 >> 2) + 4 * (n & 1) + (l15 & 3); };
 
     // ---- x pieces of this thread
     const T* x_src[PX];
     const char* m_src[PX];
-    int x_k[PX];
+    int x_k[PX], rids[PX];
+    unsigned x_off[PX];
+    const Buffer x_buf = buffer_of(a.x, a.x_bytes);
 #pragma unroll
     for (int q = 0; q < PX; ++q) {
-        const int idx = tid + 256 * q, row = idx / CH, slot = tile * BM + row;
-        int rid = slot < 16 * n_sub ? slot_row[slot] : -1;
-        rid = max(rid, 0);   // a filling slot takes row 0's values; its results are dropped
-        x_k[q] = 8 * ((idx % CH) ^ swz(row));
-        x_src[q] = (const T*)a.x + (int64_t)rid * a.ldx;
-        m_src[q] = a.mask ? (const char*)a.mask + (int64_t)rid * a.ldm * (a.mask_codes ? 1 : (int)sizeof(T)) : nullptr;
+        const int slot = tile * BM + (tid + THREADS * q) / CH;
+        rids[q] = slot < (int)a.ps.slots ? slot_row[slot] : -1;   // (slots behind the last run hold anything: n_sub decides below)
     }
-    int grp[MS];
+    int grp[MU];
+#pragma unroll
+    for (int m = 0; m < MU; ++m) {
+        const int sub = tile * (MS * WM) + wm * MS + wn * MU + m;
+        grp[m] = sub < (int)a.ps.subs ? sub_group[sub] : -1;
+    }
+    int out_row[MS], out_grp[MS];   // this lane's row of the wave's subtiles, and their adapters
 #pragma unroll
     for (int m = 0; m < MS; ++m) {
-        const int sub = tile * 4 * MS + wave * MS + m;
-        grp[m] = __builtin_amdgcn_readfirstlane(sub < n_sub ? sub_group[sub] : -1);
+        const int sub = min(tile * (MS * WM) + wm * MS + m, (int)a.ps.subs - 1);
+        out_row[m] = slot_row[16 * sub + l15];
+        out_grp[m] = sub_group[sub];
+    }
+    if (tile * (MS * WM) >= n_sub) return;
+#pragma unroll
+    for (int m = 0; m < MS; ++m) out_grp[m] = __builtin_amdgcn_readfirstlane(out_grp[m]);
+#pragma unroll
+    for (int q = 0; q < PX; ++q) {
+        const int idx = tid + THREADS * q, row = idx / CH, slot = tile * BM + row;
+        const int rid = max(slot < 16 * n_sub ? rids[q] : -1, 0);   // a filling slot takes row 0's values; its results are dropped
+        x_k[q] = 8 * ((idx % CH) ^ swz(row));
+        x_src[q] = (const T*)a.x + (int64_t)rid * a.ldx;
+        x_off[q] = (unsigned)(rid * a.ldx * (int64_t)sizeof(T));   // (DMA: all of x lies below kBehind)
+        m_src[q] = a.mask ? (const char*)a.mask + (int64_t)rid * a.ldm * (a.mask_codes ? 1 : (int)sizeof(T)) : nullptr;
+    }
+#pragma unroll
+    for (int m = 0; m < MU; ++m) {
+        const int sub = tile * (MS * WM) + wm * MS + wn * MU + m;
+        grp[m] = __builtin_amdgcn_readfirstlane(sub < n_sub ? grp[m] : -1);
     }
 
     Raw8<T> x_raw[PX], y_raw[PX];
     u32x2 c_raw[PX];
-    auto fetch_x = [&](int k0, unsigned char* buf) {
+    // WHOLE: the tile lies within K (no branch: a wait behind one would drain every load in flight)
+    auto fetch_x = [&](auto whole, int k0, unsigned char* buf) {
         if constexpr (DMA) {
 #pragma unroll
             for (int q = 0; q < PX; ++q) {
                 const int k = k0 + x_k[q];
-                dma16(k < K ? (const void*)(x_src[q] + k) : (const void*)&g_zero16, buf + (wave + 4 * q) * 1024);
+                dma16(x_buf, k < K ? x_off[q] + 2 * k : kBehind, buf + (wave + NW * q) * 1024);
+            }
+        } else if constexpr (decltype(whole)::value) {
+#pragma unroll
+            for (int q = 0; q < PX; ++q) x_raw[q].load(x_src[q] + k0 + x_k[q]);
+            if (TRANS && a.mask) {
+                if (a.mask_codes) {
+#pragma unroll
+                    for (int q = 0; q < PX; ++q) c_raw[q] = *(VH_GLOBAL(u32x2, m_src[q] + k0 + x_k[q]));
+                } else {
+#pragma unroll
+                    for (int q = 0; q < PX; ++q) y_raw[q].load((const T*)m_src[q] + k0 + x_k[q]);
+                }
             }
         } else {
 #pragma unroll
@@ -136,7 +193,7 @@ __global__ __launch_bounds__(256) void linear_kernel(LinArgs a) {
                 if (TRANS && a.mask) {
                     if (a.mask_codes) {
                         c_raw[q] = u32x2{0, 0};
-                        if (k < K) c_raw[q] = *reinterpret_cast<const u32x2*>(m_src[q] + k);
+                        if (k < K) c_raw[q] = *(VH_GLOBAL(u32x2, m_src[q] + k));
                     } else {
                         y_raw[q] = load8<T>((const T*)m_src[q] + k, K - k);
                     }
@@ -156,198 +213,281 @@ __global__ __launch_bounds__(256) void linear_kernel(LinArgs a) {
                     for (int e = 0; e < 8; ++e) {
                         const bool pos = a.mask_codes ? !((c_raw[q][e >> 2] >> (8 * (e & 3) + 7)) & 1) : y_raw[q].get(e) > 0.f;
                         const float d = v.get(e);
-                        // (bf16: the masked elements are rounded once more, to 8 bits: 2^-9 of terms that the slope made small)
+                        // (bf16: the masked elements are rounded once more, to 8 bits: 2^-8 of terms that the slope made small)
                         o.set(e, from_f<T>(pos ? d : d * a.slope));
                     }
                     v = o;
                 }
                 const Planes8<T> pl = to_planes(v);
 #pragma unroll
-                for (int p = 0; p < P; ++p) *reinterpret_cast<s16x8*>(buf + p * XB + (tid + 256 * q) * 16) = pl.p[p];
+                for (int p = 0; p < P; ++p) *reinterpret_cast<s16x8*>(buf + p * XB + (tid + THREADS * q) * 16) = pl.p[p];
             }
         }
     };
+    // (the workgroup's rows of W begin at a uniform address; within them 32 bits are enough: BN * 2^20 * 2 bytes)
+    const Buffer w_buf = buffer_of(a.w + (int64_t)n0 * a.ldw, kBehind);
+    unsigned w_off[QW];
+#pragma unroll
+    for (int q = 0; q < QW; ++q) {
+        const int idx = (wave + NW * q) * 64 + lane, p = idx / (BN * CH ? BN * CH : 1), rest = idx % (BN * CH ? BN * CH : 1), row = rest / CH;
+        w_off[q] = (unsigned)(2 * (p * a.w_plane + (int64_t)row * a.ldw + 8 * ((rest % CH) ^ swz_w(row))));
+    }
     auto fetch_w = [&](int k0, unsigned char* buf) {
         if constexpr (NT > 0) {
 #pragma unroll
-            for (int q = 0; q < (NWI + 3) / 4; ++q) {
-                const int wi = wave + 4 * q;
-                if (NWI % 4 == 0 || wi < NWI) {
-                    const int idx = wi * 64 + lane, p = idx / (BN * CH), rest = idx % (BN * CH), row = rest / CH;
-                    dma16(a.w + p * a.w_plane + (int64_t)(n0 + row) * a.ldw + k0 + 8 * ((rest % CH) ^ swz(row)), buf + wi * 1024);
-                }
-            }
+            for (int q = 0; q < QW; ++q)
+                if (NWI % NW == 0 || wave + NW * q < NWI) dma16(w_buf, w_off[q] + 2 * k0, buf + (wave + NW * q) * 1024);
         }
     };
-    // A_g operands: lane = rank l15 (+ 16 rt), depth 8 quad ..
-    Raw8<T> in_raw[MS][KC][RT];
-    auto fetch_in = [&](int k0) {
+    // inner operands: lane = rank l15 (+ 16 j), depth 8 quad ..; what lies outside is read from a block of zeros, so that the loads
+    // need no branch (only a ragged last tile of unaligned rows takes the elementwise way)
+    const T* in_src[MU][RT];
 #pragma unroll
-        for (int m = 0; m < MS; ++m)
+    for (int m = 0; m < MU; ++m)
 #pragma unroll
-            for (int c = 0; c < KC; ++c)
+        for (int j = 0; j < RT; ++j)
+            in_src[m][j] = grp[m] >= 0 && 16 * j + l15 < r ? (const T*)a.inner + ((int64_t)grp[m] * r + 16 * j + l15) * K : nullptr;
+    auto fetch_in = [&](auto whole, int k0, Raw8<T> (&in)[MU][KC][RT]) {
+        if constexpr (DMA || decltype(whole)::value) {
 #pragma unroll
-                for (int j = 0; j < RT; ++j) {
-                    const int rank = 16 * j + l15, k = k0 + 32 * c + 8 * quad;
-                    const int valid = (grp[m] >= 0 && rank < r) ? K - k : 0;
-                    if constexpr (TRANS)
-                        in_raw[m][c][j] = load8_strided<T>((const T*)a.inner + ((int64_t)grp[m] * K + k) * r + rank, r, valid);
-                    else
-                        in_raw[m][c][j] = load8<T>((const T*)a.inner + ((int64_t)grp[m] * r + rank) * K + k, valid);
-                }
+            for (int m = 0; m < MU; ++m)
+#pragma unroll
+                for (int c = 0; c < KC; ++c)
+#pragma unroll
+                    for (int j = 0; j < RT; ++j) {
+                        const int k = k0 + 32 * c + 8 * quad;
+                        in[m][c][j].load(in_src[m][j] != nullptr && (!DMA || k < K) ? in_src[m][j] + k : (const T*)g_zero32);
+                    }
+        } else {
+#pragma unroll
+            for (int m = 0; m < MU; ++m)
+#pragma unroll
+                for (int c = 0; c < KC; ++c)
+#pragma unroll
+                    for (int j = 0; j < RT; ++j) {
+                        const int k = k0 + 32 * c + 8 * quad;
+                        in[m][c][j] = load8<T>(in_src[m][j] + k, in_src[m][j] != nullptr ? K - k : 0);
+                    }
+        }
     };
 
-    f32x4 acc[MS][NT ? NT : 1], low[MS][RT];
+    f32x4 acc[MS][NT ? NT : 1], low[MU][RT];
 #pragma unroll
-    for (int m = 0; m < MS; ++m) {
+    for (int m = 0; m < MS; ++m)
 #pragma unroll
         for (int n = 0; n < NT; ++n) acc[m][n] = f32x4{0, 0, 0, 0};
 #pragma unroll
+    for (int m = 0; m < MU; ++m)
+#pragma unroll
         for (int j = 0; j < RT; ++j) low[m][j] = f32x4{0, 0, 0, 0};
-    }
 
-    unsigned char* const xs0 = smem;
-    unsigned char* const ws0 = smem + P * XB;
-    fetch_w(0, ws0);
-    fetch_x(0, xs0);
-    fetch_in(0);
-    keep_x(xs0);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    for (int kt = 0; kt < nk; ++kt) {
-        const int cur = kt & 1;
-        const unsigned char* const xb = smem + cur * BUF;
+    auto compute = [&](const unsigned char* xb, const Raw8<T> (&in)[MU][KC][RT]) {
         const unsigned char* const wb = xb + P * XB;
-        unsigned char* const xn = smem + (cur ^ 1) * BUF;
-        const bool more = kt + 1 < nk;
-        Planes8<T> in_pl[MS][KC][RT];
+        if constexpr (P == 1 && MS == 1 && NT > 0) {
+            // one product per operand that is read: all reads of the tile go ahead of the products
+            s16x8 xa[KC], wa[KC][NT];
 #pragma unroll
-        for (int m = 0; m < MS; ++m)
+            for (int c = 0; c < KC; ++c) {
+                const int xrow = wm * 16 + l15;
+                xa[c] = *reinterpret_cast<const s16x8*>(xb + (xrow * CH + ((4 * c + quad) ^ swz(xrow))) * 16);
 #pragma unroll
-            for (int c = 0; c < KC; ++c)
+                for (int n = 0; n < NT; ++n) {
+                    const int row = wn * NT * 16 + w_row(n);
+                    wa[c][n] = *reinterpret_cast<const s16x8*>(wb + (row * CH + ((4 * c + quad) ^ swz_w(row))) * 16);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int j = 0; j < RT; ++j) in_pl[m][c][j] = to_planes(in_raw[m][c][j]);
-        if (more) {
-            fetch_w((kt + 1) * BK, xn + P * XB);
-            fetch_x((kt + 1) * BK, xn);
-            fetch_in((kt + 1) * BK);
+            for (int c = 0; c < KC; ++c) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n) acc[0][n] = mfma32(wa[c][n], xa[c], acc[0][n]);
+#pragma unroll
+                for (int j = 0; j < RT; ++j) low[0][j] = mfma32(to_planes(in[0][c][j]).p[0], xa[c], low[0][j]);
+            }
+            return;
         }
 #pragma unroll
         for (int c = 0; c < KC; ++c) {
             s16x8 xf[MS][P];
 #pragma unroll
             for (int m = 0; m < MS; ++m) {
-                const int row = (wave * MS + m) * 16 + l15;
+                const int row = (wm * MS + m) * 16 + l15;
 #pragma unroll
                 for (int p = 0; p < P; ++p)
                     xf[m][p] = *reinterpret_cast<const s16x8*>(xb + p * XB + (row * CH + ((4 * c + quad) ^ swz(row))) * 16);
             }
 #pragma unroll
-            for (int m = 0; m < MS; ++m)
-#pragma unroll
-                for (int j = 0; j < RT; ++j) low[m][j] = mma(in_pl[m][c][j].p, xf[m], low[m][j]);
-#pragma unroll
             for (int n = 0; n < NT; ++n) {
                 s16x8 wf[P];
-                const int row = n * 16 + l15;
+                const int row = wn * NT * 16 + w_row(n);
 #pragma unroll
                 for (int p = 0; p < P; ++p)
-                    wf[p] = *reinterpret_cast<const s16x8*>(wb + p * WB + (row * CH + ((4 * c + quad) ^ swz(row))) * 16);
+                    wf[p] = *reinterpret_cast<const s16x8*>(wb + p * WB + (row * CH + ((4 * c + quad) ^ swz_w(row))) * 16);
 #pragma unroll
                 for (int m = 0; m < MS; ++m) acc[m][n] = mma(wf, xf[m], acc[m][n]);
             }
+#pragma unroll
+            for (int m = 0; m < MU; ++m)
+#pragma unroll
+                for (int j = 0; j < RT; ++j) {
+                    const Planes8<T> pl = to_planes(in[m][c][j]);
+                    if constexpr (WN == 1) low[m][j] = mma(pl.p, xf[m], low[m][j]);
+                    else if (wn == 0) low[m][j] = mma(pl.p, xf[m], low[m][j]);
+                    else low[m][j] = mma(pl.p, xf[MS - MU + m], low[m][j]);
+                }
         }
-        if (more) keep_x(xn);
+    };
+
+    using Yes = std::integral_constant<bool, true>;
+    using No = std::integral_constant<bool, false>;
+    Raw8<T> in0[MU][KC][RT], in1[MU][KC][RT];
+    // Tile kt is multiplied while tile kt + 1 is on its way.  (Three buffers with counted waits were measured no faster: what they hid of
+    // the latency, the workgroups that no longer fitted a CU had hidden before.)
+    auto fetch = [&](int k0, unsigned char* to, Raw8<T> (&in)[MU][KC][RT]) {
+        if (k0 + BK <= K) {
+            fetch_in(Yes(), k0, in);
+            fetch_x(Yes(), k0, to);
+        } else {
+            fetch_in(No(), k0, in);
+            fetch_x(No(), k0, to);
+        }
+        fetch_w(k0, to + P * XB);
+    };
+    fetch(0, smem, in0);
+    keep_x(smem);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    for (int kt = 0; kt < nk; ++kt) {
+        unsigned char* const to = smem + ((kt + 1) & 1) * BUF;
+        const bool more = kt + 1 < nk;
+        if (more) fetch((kt + 1) * BK, to, in1);
+        __builtin_amdgcn_sched_barrier(0);
+        compute(smem + (kt & 1) * BUF, in0);
+        __builtin_amdgcn_sched_barrier(0);
+        if (more) keep_x(to);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
+#pragma unroll
+        for (int m = 0; m < MU; ++m)
+#pragma unroll
+            for (int c = 0; c < KC; ++c)
+#pragma unroll
+                for (int j = 0; j < RT; ++j) in0[m][c][j] = in1[m][c][j];
     }
 
+    // ---- u of the wave's rows: the WN waves on the same rows computed a share each
+    constexpr int LS = 16 * RT + 4;   // floats between rows of the exchange (16-byte pieces of 16 rows in different banks)
+    float* const lows = reinterpret_cast<float*>(smem);   // [BM][LS]: the tiles are done with
+    static_assert(WN == 1 || BM * LS * 4 <= 2 * BUF, "the exchange fits the tile buffers");
+    if constexpr (WN > 1) {
+#pragma unroll
+        for (int m = 0; m < MU; ++m)
+#pragma unroll
+            for (int j = 0; j < RT; ++j)
+                *reinterpret_cast<f32x4*>(lows + ((wm * MS + wn * MU + m) * 16 + l15) * LS + 16 * j + 4 * quad) = low[m][j];
+        __syncthreads();
+    }
+    typename Raw4<T>::type of[RT][NT ? NT : 1];
+    int have = -1;   // the adapter that `of` holds: neighbouring subtiles mostly have the same
 #pragma unroll
     for (int m = 0; m < MS; ++m) {
-        const int slot = tile * BM + (wave * MS + m) * 16 + l15;
-        const int rid = slot < 16 * n_sub ? slot_row[slot] : -1;
-        if (a.low != nullptr && n0 == 0 && rid >= 0) {
+        if (tile * (MS * WM) + wm * MS + m >= n_sub) break;
+        const int g = out_grp[m], rid = out_row[m];
+        f32x4 lo[RT];
+#pragma unroll
+        for (int j = 0; j < RT; ++j) {
+            if constexpr (WN > 1) lo[j] = *reinterpret_cast<const f32x4*>(lows + ((wm * MS + m) * 16 + l15) * LS + 16 * j + 4 * quad);
+            else lo[j] = low[m][j];
+        }
+        if (a.low != nullptr && n0 == 0 && wn == 0 && rid >= 0) {
 #pragma unroll
             for (int j = 0; j < RT; ++j) {
                 const int rank = 16 * j + 4 * quad;
                 float* dst = a.low + (int64_t)rid * r + rank;
                 if ((r & 3) == 0 && rank + 4 <= r) {
-                    *reinterpret_cast<f32x4*>(dst) = low[m][j] * a.low_scale;
+                    *reinterpret_cast<f32x4*>(dst) = lo[j] * a.low_scale;
                 } else {
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        if (rank + i < r) dst[i] = low[m][j][i] * a.low_scale;
+                        if (rank + i < r) dst[i] = lo[j][i] * a.low_scale;
                 }
             }
         }
         if constexpr (NT > 0) {
-            if (grp[m] >= 0) {
+            const int nw = n0 + wn * NT * 16;
+            if (g >= 0) {
+                if (g != have) {
+                    have = g;
+#pragma unroll
+                    for (int jn = 0; jn < RT * NT; ++jn) {
+                        const int n = jn % NT, rank = 16 * (jn / NT) + 4 * quad;
+                        const int col = nw + w_row(n);
+                        const T* src = (const T*)a.outer + (TRANS ? ((int64_t)g * r + rank) * a.N + col : ((int64_t)g * a.N + col) * r + rank);
+                        load4(src, TRANS ? a.N : 1, col < a.N ? r - rank : 0, !TRANS && (r & 3) == 0, of[jn / NT][n]);
+                    }
+                }
 #pragma unroll
                 for (int j = 0; j < RT; ++j) {
                     s16x4 uf[PU];
-                    cut4<PU>(low[m][j] * a.scale, uf);
-                    const int rank = 16 * j + 4 * quad;
+                    cut4<PU>(lo[j] * a.scale, uf);
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
-                        const int col = n0 + 16 * n + l15;
-                        s16x4 of[P];
-                        const T* src = (const T*)a.outer + (TRANS ? ((int64_t)grp[m] * r + rank) * a.N + col : ((int64_t)grp[m] * a.N + col) * r + rank);
-                        load4_planes(src, TRANS ? a.N : 1, col < a.N ? r - rank : 0, of);
+                        s16x4 op[P];
+                        planes4(of[j][n], op);
 #pragma unroll
                         for (int s = 2; s >= 0; --s)
 #pragma unroll
                             for (int i = 0; i < P; ++i)
 #pragma unroll
                                 for (int k = 0; k < PU; ++k)
-                                    if (i + k == s) acc[m][n] = mfma16(of[i], uf[k], acc[m][n]);
+                                    if (i + k == s) acc[m][n] = mfma16(op[i], uf[k], acc[m][n]);
                     }
                 }
             }
             T* yrow = (T*)a.y + (int64_t)max(rid, 0) * a.ldy;
-            const bool wide = (a.ldy & 3) == 0 && ((uintptr_t)a.y & (4 * sizeof(T) - 1)) == 0;
-            T out[NT][4];
+            const bool wide = (a.ldy & 7) == 0 && ((uintptr_t)a.y & 15) == 0;
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                const int col = n0 + 16 * n + 4 * quad;
+            for (int b = 0; b < NT / 2; ++b) {   // a lane's eight columns of a block of 32
+                const int col = nw + 32 * b + 8 * quad;
+                float v[8];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float v = acc[m][n][i];
-                    if (a.bias != nullptr) v += a.bias[col + i];
-                    if (a.activation) v = v > 0.f ? v : v * a.slope;
-                    out[n][i] = from_f<T>(v);
+                for (int e = 0; e < 8; ++e) v[e] = acc[m][2 * b + (e >> 2)][e & 3];
+                if (!TRANS && a.bias != nullptr) {
+                    const f32x4 b0 = *(VH_GLOBAL(f32x4, a.bias + col)), b1 = *(VH_GLOBAL(f32x4, a.bias + col + 4));
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] += e < 4 ? b0[e & 3] : b1[e & 3];
                 }
+                if (!TRANS && a.activation) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] = fmaxf(v[e], v[e] * a.slope);   // 0 <= slope <= 1
+                }
+                struct __attribute__((aligned(16))) Row8 { T e[8]; } o;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) o.e[e] = from_f<T>(v[e]);
                 if (rid >= 0) {
-                    if (wide && col + 4 <= a.N) {
-                        struct __attribute__((aligned(4 * sizeof(T)))) Four { T e[4]; };
-                        Four f = {{out[n][0], out[n][1], out[n][2], out[n][3]}};
-                        *reinterpret_cast<Four*>(yrow + col) = f;
+                    if (wide && col + 8 <= a.N) {
+                        *reinterpret_cast<Row8*>(yrow + col) = o;
                     } else {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (col + i < a.N) yrow[col + i] = out[n][i];
+                        for (int e = 0; e < 8; ++e)
+                            if (col + e < a.N) yrow[col + e] = o.e[e];
                     }
                 }
-            }
-            if (!TRANS && a.codes != nullptr) {
-                // checkpoint of the rounded y: a block of 32 columns is two subtiles, 4 x 2 elements of four lanes
-#pragma unroll
-                for (int b = 0; b < NT / 2; ++b) {
-                    const int c0 = n0 + 32 * b;
-                    float v[8], amax = 0.f;
+                if (!TRANS && a.codes != nullptr) {
+                    // checkpoint of the rounded y: the block's other columns are in the lanes 16, 32 and 48 further on
+                    float amax = 0.f;
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        const int col = c0 + 16 * (e >> 2) + 4 * quad + (e & 3);
-                        v[e] = col < a.N ? to_f<T>(out[2 * b + (e >> 2)][e & 3]) : 0.f;
+                        v[e] = col + e < a.N ? to_f<T>(o.e[e]) : 0.f;
                         amax = fmaxf(amax, finite_size(v[e]));
                     }
                     amax = fmaxf(amax, __shfl_xor(amax, 16));
                     amax = fmaxf(amax, __shfl_xor(amax, 32));
                     const int k = block_exp(amax);
-                    if (rid >= 0 && c0 < a.N) {
-                        uint8_t* dst = a.codes + (int64_t)rid * a.ldc + c0 + 4 * quad;
-                        *reinterpret_cast<unsigned*>(dst) = encode4(v[0], v[1], v[2], v[3], k);
-                        *reinterpret_cast<unsigned*>(dst + 16) = encode4(v[4], v[5], v[6], v[7], k);
-                        if (quad == 0) a.exps[(int64_t)rid * (a.ldc / kBlockCols) + c0 / kBlockCols] = (uint8_t)(k + 127);
+                    if (rid >= 0 && nw + 32 * b < a.N) {
+                        *reinterpret_cast<u32x2*>(a.codes + (int64_t)rid * a.ldc + col) =
+                            u32x2{encode4(v[0], v[1], v[2], v[3], k), encode4(v[4], v[5], v[6], v[7], k)};
+                        if (quad == 0) a.exps[(int64_t)rid * (a.ldc / kBlockCols) + col / kBlockCols] = (uint8_t)(k + 127);
                     }
                 }
             }
@@ -355,31 +495,35 @@ __global__ __launch_bounds__(256) void linear_kernel(LinArgs a) {
     }
 }
 
-template <class T, int NT, int MS, int RT, bool TRANS, bool DMA>
+template <class T, class S, int RT, bool TRANS, bool DMA>
 void launch_one(const LinArgs& a, hipStream_t s) {
-    constexpr int P = Elem<T>::planes, BK = P == 1 ? 64 : 32;
-    constexpr int bytes = 2 * P * (64 * MS + 16 * NT) * BK * 2;
+    constexpr int P = Elem<T>::planes, BK = S::BK, BM = 16 * S::MS * S::WM, BN = 16 * S::NT * S::WN;
+    constexpr int bytes = 2 * P * (BM + BN) * BK * 2;
     if constexpr (bytes > 65536) {   // per device, cheap, and valid while a stream is captured
-        VH_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(linear_kernel<T, NT, MS, RT, TRANS, DMA>),
+        VH_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(linear_kernel<T, S, RT, TRANS, DMA>),
                                    hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
     }
-    const int64_t row_tiles = ceil_div(a.ps.subs, 4 * MS), col_tiles = NT ? ceil_div(a.N, 16 * NT) : 1;
-    const int64_t blocks = round_up(row_tiles * col_tiles, 8);
+    const int64_t row_tiles = ceil_div(a.ps.subs, S::MS * S::WM), col_tiles = S::NT ? ceil_div(a.N, BN ? BN : 1) : 1;
+    const int64_t blocks = round_up(row_tiles, 8) * col_tiles;
     VH_REQUIRE(blocks < (int64_t(1) << 31), "too many rows for one launch");
-    linear_kernel<T, NT, MS, RT, TRANS, DMA><<<dim3((unsigned)blocks), 256, bytes, s>>>(a);
+    linear_kernel<T, S, RT, TRANS, DMA><<<dim3((unsigned)blocks), 64 * S::WM * S::WN, bytes, s>>>(a);
     VH_HIP(hipGetLastError());
 }
 
 template <class T, int RT, bool TRANS, bool DMA>
 void launch_shape(const LinArgs& a, hipStream_t s) {
+    constexpr bool F = Elem<T>::planes == 3;
+    constexpr int BK = F ? 32 : 64;
     if (a.y == nullptr) {
-        if constexpr (TRANS) launch_one<T, 0, 1, RT, TRANS, DMA>(a, s);
+        if constexpr (TRANS) launch_one<T, Shape<4, 1, 1, 0, BK>, RT, TRANS, DMA>(a, s);
         return;
     }
-    if (a.N <= 32) return launch_one<T, 2, 1, RT, TRANS, DMA>(a, s);
-    const int64_t tiles128 = ceil_div(a.ps.subs, 8) * ceil_div(a.N, 128);
-    if (tiles128 < 1024) launch_one<T, 8, 1, RT, TRANS, DMA>(a, s);
-    else launch_one<T, 8, 2, RT, TRANS, DMA>(a, s);
+    if (a.N <= 32) return launch_one<T, Shape<4, 1, 1, 2, BK>, RT, TRANS, DMA>(a, s);
+    const int64_t big = ceil_div(a.ps.subs, F ? 8 : 16) * ceil_div(a.N, F ? 128 : 256);
+    if (big < 512) return launch_one<T, Shape<4, 1, 1, 8, BK>, RT, TRANS, DMA>(a, s);
+    if constexpr (F) launch_one<T, Shape<4, 2, 2, 4, BK>, RT, TRANS, DMA>(a, s);
+    else if constexpr (RT == 1 && !TRANS) launch_one<T, Shape<4, 2, 4, 8, BK>, RT, TRANS, DMA>(a, s);
+    else launch_one<T, Shape<4, 2, 2, 8, BK>, RT, TRANS, DMA>(a, s);
 }
 template <class T, bool TRANS, bool DMA>
 void launch_rank(const LinArgs& a, hipStream_t s) {
