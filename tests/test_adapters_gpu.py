@@ -358,6 +358,29 @@ def test_captured_and_replayed(ad, dtype):
             assert all(torch.equal(a, b) for a, b in zip(out, want))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,k", [(300, 96), (129, 130), (640, 200)])
+def test_large_batches_take_the_wide_tiles(ad, dtype, n, k):
+    """Enough rows for the widest tiles, and widths that end inside one, in both directions."""
+    rows, rank, groups = 70000, 20 if n == 300 else 9, 300
+    c = make(50, dtype, rows, k, n, rank, groups, order="sorted")
+    shared = ad.SharedProjection(c["w"], c["b"])
+    plan = ad.group_rows(c["groups"], groups)
+    y, low, y8 = ad.adapted_linear_train(c["x"], shared, c["down"], c["up"], plan, SCALE, SLOPE)
+    dx, _, _ = ad.adapted_linear_backward(c["dy"], c["x"], y, low, shared, c["down"], c["up"], plan, SCALE, SLOPE)
+    rng = np.random.default_rng(0)
+    at = np.concatenate([np.arange(40), rng.integers(0, rows, 200), np.arange(rows - 40, rows)])
+    t = torch.from_numpy(at).cuda()
+    part = dict(c, x=c["x"][t], dy=c["dy"][t], g=c["g"][at])
+    u, want, tu, ty = forward_bounds(part, dtype, SLOPE)
+    close(y[t], want, ty, "y")
+    close(low[t], u, tu, "u")
+    value, tol = backward_bounds(part, f64(part["x"]), f64(y[t]), f64(low[t]), dtype, SLOPE)["dx"]
+    close(dx[t], value, tol, "dx")
+    again = ad.checkpoint8(y)
+    assert torch.equal(y8.codes, again.codes) and torch.equal(y8.exponents, again.exponents)
+
+
 def test_two_streams_at_once(ad):
     c = [make(30 + i, torch.bfloat16, 4000, 128, 128, 16, 60) for i in range(2)]
     shared = [ad.SharedProjection(d["w"], d["b"]) for d in c]

@@ -113,6 +113,7 @@ __device__ __forceinline__ void place_rows(const int* groups, int64_t lo, int64_
         load_keys(groups, row0, hi, G, key);
 #pragma unroll
         for (int b = 0; b < PB; ++b) {
+            if (row0 + 64 * b >= hi) break;
             const unsigned long long same = same_key(key[b], bits);
             const int rank = __popcll(same & ((1ull << lane) - 1));
             if (key[b] <= G) {
@@ -209,7 +210,7 @@ static bool plan_is_small(int64_t rows, int64_t groups) { return rows <= kSmallR
 static int64_t plan_pieces(int64_t rows) { return rows < 512 ? 1 : (rows / 512 < 1024 ? rows / 512 : 1024); }
 
 // =====================================================================================================================
-// Shared weight: both orientations, zero-filled to multiples of 128 rows and 64 columns, cut into planes
+// Shared weight: both orientations, zero-filled to whole tiles, cut into planes
 // =====================================================================================================================
 struct WeightShape {
     int64_t np, kp, nq, kq, fwd, bwd, bias_off, bytes;   // fwd: [P][np][kq], bwd: [P][kp][nq]
@@ -219,10 +220,10 @@ struct WeightShape {
 static WeightShape weight_shape(int64_t n, int64_t k, int dtype) {
     WeightShape w{};
     w.planes = dtype == VH_BF16 ? 1 : 3;
-    w.np = round_up(n, 128);
-    w.kq = round_up(k, 64);
-    w.kp = round_up(k, 128);
-    w.nq = round_up(n, 64);
+    w.np = n <= 128 ? 128 : round_up(n, 256);   // whole result tiles (launch_shape: 256 columns only above 128)
+    w.kq = round_up(k, 128);   // the deepest tile
+    w.kp = k <= 128 ? 128 : round_up(k, 256);
+    w.nq = round_up(n, 128);
     w.fwd = w.np * w.kq;
     w.bwd = w.kp * w.nq;
     w.bias_off = 2 * w.planes * (w.fwd + w.bwd);

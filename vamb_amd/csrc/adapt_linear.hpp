@@ -79,16 +79,17 @@ template <class T> struct Raw4;
 template <> struct Raw4<bf16_t> { typedef u32x2 type; };
 template <> struct Raw4<float> { typedef f32x4 type; };
 
-// A tile shape: WM x WN waves, each MS x NT subtiles of 16 x 16; two tile buffers of depth BK in the LDS.
+// A tile shape: WM x WN waves, each MS x NT subtiles of 16 x 16; two tile buffers of depth BK in the LDS; KG such groups of waves that take
+// every KG-th tile of the depth each and add their sums at the end (small grids: more waves a CU to hide each other's latencies).
 // NT = 0: only `low` is computed (a backward pass without dx).
-template <int WM_, int WN_, int MS_, int NT_, int BK_>
+template <int WM_, int WN_, int MS_, int NT_, int BK_, int KG_ = 1>
 struct Shape {
-    static constexpr int WM = WM_, WN = WN_, MS = MS_, NT = NT_, BK = BK_;
+    static constexpr int WM = WM_, WN = WN_, MS = MS_, NT = NT_, BK = BK_, KG = KG_;
 };
 
 template <class T, class S, int RT, bool TRANS, bool DMA>
-__global__ __launch_bounds__(64 * S::WM * S::WN) void linear_kernel(LinArgs a) {
-    constexpr int WM = S::WM, WN = S::WN, MS = S::MS, NT = S::NT, NW = WM * WN, THREADS = 64 * NW;
+__global__ __launch_bounds__(64 * S::WM * S::WN * S::KG) void linear_kernel(LinArgs a) {
+    constexpr int WM = S::WM, WN = S::WN, MS = S::MS, NT = S::NT, NW = WM * WN, THREADS = 64 * NW, KG = S::KG;
     constexpr int P = Elem<T>::planes;
     constexpr int PU = P == 1 ? 2 : 3;
     constexpr int BK = S::BK;
@@ -104,8 +105,11 @@ __global__ __launch_bounds__(64 * S::WM * S::WN) void linear_kernel(LinArgs a) {
     static_assert(PX >= 1 && BM * CH % THREADS == 0 && MS % WN == 0 && (!DMA || P == 1), "tile shape");
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    static_assert(KG == 1 || (WN == 1 && MS == 1), "groups along the depth have narrow waves");
+    const int kg = __builtin_amdgcn_readfirstlane((int)threadIdx.x / THREADS), tid = (int)threadIdx.x % THREADS;   // (within the group of waves)
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l15 = lane & 15, quad = lane >> 4, wm = wave / WN, wn = wave % WN;
+    unsigned char* const tiles = smem + kg * 2 * BUF;
     // workgroup b runs on XCD b % 8: a row tile's column tiles are eight apart, so that XCD's L2 has its x rows after the first
     const int col_tiles = NT ? (a.N + BN - 1) / (BN ? BN : 1) : 1;
     const int bid = blockIdx.x, tile = bid / (8 * col_tiles) * 8 + (bid & 7), n0 = (bid / 8 % col_tiles) * BN;
@@ -117,8 +121,8 @@ __global__ __launch_bounds__(64 * S::WM * S::WN) void linear_kernel(LinArgs a) {
     // 16-byte pieces of a tile row are XOR-permuted by half the row's number within the operand: the 16 rows of an operand read then
     // take the LDS's full 256 B a clock (measured; permuted by a quarter of it, rows of four pieces took 128).  Rows of W are read in another order: a lane's four results of the subtiles 2 i and
     // 2 i + 1 are eight consecutive columns, 32 i + 8 (l15 / 4) + 4 (0 or 1) + l15 % 4 being the column of operand row l15.
-    auto swz = [](int row) { return (row >> 1) & (CH - 1); };
-    auto swz_w = [](int row) { return ((row >> 1) & 1) | ((row >> 2) & (CH - 2)); };
+    auto swz = [](int row) { return CH == 16 ? row & 15 : (row >> 1) & (CH - 1); };
+    auto swz_w = [](int row) { return CH == 16 ? (row & 3) | ((row >> 1) & 12) : ((row >> 1) & 1) | ((row >> 2) & (CH - 2)); };
     auto w_row = [&](int n) { return 32 * (n >> 1) + 8 * (l15 >> 2) + 4 * (n & 1) + (l15 & 3); };
 
     // ---- x pieces of this thread
@@ -225,7 +229,7 @@ __global__ __launch_bounds__(64 * S::WM * S::WN) void linear_kernel(LinArgs a) {
         }
     };
     // (the workgroup's rows of W begin at a uniform address; within them 32 bits are enough: BN * 2^20 * 2 bytes)
-    const Buffer w_buf = buffer_of(a.w + (int64_t)n0 * a.ldw, kBehind);
+    const Buffer w_buf = buffer_of(a.w + (int64_t)n0 * a.ldw, (unsigned)(2 * (P * a.w_plane - (int64_t)n0 * a.ldw)));
     unsigned w_off[QW];
 #pragma unroll
     for (int q = 0; q < QW; ++q) {
@@ -353,16 +357,19 @@ __global__ __launch_bounds__(64 * S::WM * S::WN) void linear_kernel(LinArgs a) {
         }
         fetch_w(k0, to + P * XB);
     };
-    fetch(0, smem, in0);
-    keep_x(smem);
+    if (kg < nk) {
+        fetch(kg * BK, tiles, in0);
+        keep_x(tiles);
+    }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    for (int kt = 0; kt < nk; ++kt) {
-        unsigned char* const to = smem + ((kt + 1) & 1) * BUF;
-        const bool more = kt + 1 < nk;
-        if (more) fetch((kt + 1) * BK, to, in1);
+    for (int i = 0; i < (nk + KG - 1) / KG; ++i) {
+        const int kt = kg + i * KG;
+        unsigned char* const to = tiles + ((i + 1) & 1) * BUF;
+        const bool more = kt + KG < nk;
+        if (more) fetch((kt + KG) * BK, to, in1);
         __builtin_amdgcn_sched_barrier(0);
-        compute(smem + (kt & 1) * BUF, in0);
+        if (KG == 1 || kt < nk) compute(tiles + (i & 1) * BUF, in0);
         __builtin_amdgcn_sched_barrier(0);
         if (more) keep_x(to);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -373,6 +380,26 @@ __global__ __launch_bounds__(64 * S::WM * S::WN) void linear_kernel(LinArgs a) {
             for (int c = 0; c < KC; ++c)
 #pragma unroll
                 for (int j = 0; j < RT; ++j) in0[m][c][j] = in1[m][c][j];
+    }
+    if constexpr (KG > 1) {   // the groups' sums, in their order (the tiles are done with)
+        f32x4* const part = reinterpret_cast<f32x4*>(smem);   // [KG - 1][NT + RT][THREADS]
+        static_assert((KG - 1) * (NT + RT) * THREADS * 16 <= KG * 2 * BUF, "the partial sums fit the tile buffers");
+        if (kg > 0) {
+            f32x4* const mine = part + (kg - 1) * (NT + RT) * THREADS + tid;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mine[n * THREADS] = acc[0][n];
+#pragma unroll
+            for (int j = 0; j < RT; ++j) mine[(NT + j) * THREADS] = low[0][j];
+        }
+        __syncthreads();
+        if (kg > 0) return;
+#pragma unroll
+        for (int q = 0; q < KG - 1; ++q) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) acc[0][n] += part[(q * (NT + RT) + n) * THREADS + tid];
+#pragma unroll
+            for (int j = 0; j < RT; ++j) low[0][j] += part[(q * (NT + RT) + NT + j) * THREADS + tid];
+        }
     }
 
     // ---- u of the wave's rows: the WN waves on the same rows computed a share each
@@ -498,7 +525,7 @@ __global__ __launch_bounds__(64 * S::WM * S::WN) void linear_kernel(LinArgs a) {
 template <class T, class S, int RT, bool TRANS, bool DMA>
 void launch_one(const LinArgs& a, hipStream_t s) {
     constexpr int P = Elem<T>::planes, BK = S::BK, BM = 16 * S::MS * S::WM, BN = 16 * S::NT * S::WN;
-    constexpr int bytes = 2 * P * (BM + BN) * BK * 2;
+    constexpr int bytes = S::KG * 2 * P * (BM + BN) * BK * 2;
     if constexpr (bytes > 65536) {   // per device, cheap, and valid while a stream is captured
         VH_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(linear_kernel<T, S, RT, TRANS, DMA>),
                                    hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
@@ -506,7 +533,7 @@ void launch_one(const LinArgs& a, hipStream_t s) {
     const int64_t row_tiles = ceil_div(a.ps.subs, S::MS * S::WM), col_tiles = S::NT ? ceil_div(a.N, BN ? BN : 1) : 1;
     const int64_t blocks = round_up(row_tiles, 8) * col_tiles;
     VH_REQUIRE(blocks < (int64_t(1) << 31), "too many rows for one launch");
-    linear_kernel<T, S, RT, TRANS, DMA><<<dim3((unsigned)blocks), 64 * S::WM * S::WN, bytes, s>>>(a);
+    linear_kernel<T, S, RT, TRANS, DMA><<<dim3((unsigned)blocks), 64 * S::WM * S::WN * S::KG, bytes, s>>>(a);
     VH_HIP(hipGetLastError());
 }
 
@@ -514,13 +541,15 @@ template <class T, int RT, bool TRANS, bool DMA>
 void launch_shape(const LinArgs& a, hipStream_t s) {
     constexpr bool F = Elem<T>::planes == 3;
     constexpr int BK = F ? 32 : 64;
+    constexpr int KG = RT == 4 ? 2 : 4;   // (rank 33-64: the registers of 16 waves a CU are too few)
     if (a.y == nullptr) {
-        if constexpr (TRANS) launch_one<T, Shape<4, 1, 1, 0, BK>, RT, TRANS, DMA>(a, s);
+        if constexpr (TRANS) launch_one<T, Shape<4, 1, 1, 0, BK, KG>, RT, TRANS, DMA>(a, s);
         return;
     }
-    if (a.N <= 32) return launch_one<T, Shape<4, 1, 1, 2, BK>, RT, TRANS, DMA>(a, s);
+    // small grids, and the narrow latent layers
+    if (a.N <= 32 || ceil_div(a.ps.subs, 4) * ceil_div(a.N, 32) <= 1024) return launch_one<T, Shape<4, 1, 1, 2, BK, KG>, RT, TRANS, DMA>(a, s);
     const int64_t big = ceil_div(a.ps.subs, F ? 8 : 16) * ceil_div(a.N, F ? 128 : 256);
-    if (big < 512) return launch_one<T, Shape<4, 1, 1, 8, BK>, RT, TRANS, DMA>(a, s);
+    if (big < 512 || a.N <= 128) return launch_one<T, Shape<4, 1, 1, 8, BK>, RT, TRANS, DMA>(a, s);
     if constexpr (F) launch_one<T, Shape<4, 2, 2, 4, BK>, RT, TRANS, DMA>(a, s);
     else if constexpr (RT == 1 && !TRANS) launch_one<T, Shape<4, 2, 4, 8, BK>, RT, TRANS, DMA>(a, s);
     else launch_one<T, Shape<4, 2, 2, 8, BK>, RT, TRANS, DMA>(a, s);
