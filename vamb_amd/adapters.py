@@ -399,3 +399,231 @@ def checkpoint_weight_grad(dy, x: Checkpoint8, y=None, negative_slope: Optional[
         _lib.check(lib.vh_checkpoint8_weight_grad(dy.data_ptr(), ld, held_x, held_y if negative_slope is not None else None,
                                                   negative_slope or 0.0, rows, n, k, code, dweight.data_ptr(), dbias.data_ptr(), scratch.data_ptr(), stream))
     return dweight, dbias
+
+
+# ---- adapters of a trained VAE --------------------------------------------------------------------------------------------------
+_SLOPE = 0.01       # torch.nn.LeakyReLU's default (encode.py:264)
+_BN_EPS = 1e-5
+
+
+class VAEAdapters:
+    """Low-rank adapters of a trained :class:`vamb_amd.encode.VAE`, one set per sample: trained on the VAE's own loss with the VAE's weights
+    and BatchNorm statistics as they are, and used to encode.  (The reference has no counterpart: its VAE treats all samples alike.)
+
+    Every Linear of the encoder (the hidden layers and ``mu``) has an adapter of ``rank`` per group; the decoder is as it was trained.  The
+    BatchNorm of a layer (eval mode, encode.py:264) is folded into the Linear behind it, so an adapter reads the layer's input in front of that BatchNorm.
+    A new adapter changes nothing (``up`` is zero).  Arithmetic in ``dtype`` (default: the VAE's compute type), ``mu`` always
+    in float32; parameters and their optimiser (torch's Adam) in float32.  Activations wait for the backward pass as 8-bit checkpoints.
+
+    ``groups``: the sample of each contig of the data set, integers; a value outside ``[0, n_groups)`` stands for a contig without an adapter."""
+
+    def __init__(self, vae, n_groups: int, rank: int = 8, scale: float = 1.0, seed: int = 0, dtype: Optional[_torch.dtype] = None,
+                 device: Union[str, _torch.device] = "cuda"):
+        from . import encode as _encode
+        if type(vae) is not _encode.VAE:
+            raise ValueError("adapters are made for a plain VAE")
+        if not 1 <= n_groups <= MAX_GROUPS:
+            raise ValueError(f"the number of groups must be in [1, {MAX_GROUPS}], not {n_groups}")
+        if not 1 <= rank <= MAX_RANK:
+            raise ValueError(f"the rank must be in [1, {MAX_RANK}], not {rank}")
+        if not math.isfinite(scale):
+            raise ValueError(f"scale must be finite, not {scale}")
+        if dtype is None:
+            dtype = _torch.bfloat16 if vae.compute_dtype == "bf16" else _torch.float32
+        if dtype not in _DTYPES:
+            raise ValueError(f"dtype must be float32 or bfloat16, not {dtype}")
+        self.nsamples, self.nlatent, self.alpha, self.beta = vae.nsamples, vae.nlatent, vae.alpha, vae.beta
+        self.ntnf = vae.ntnf
+        self.n_groups, self.rank, self.scale, self.dtype = n_groups, rank, float(scale), dtype
+        device = _torch.device(device)
+        self.device = _torch.device("cuda", _torch.cuda.current_device()) if device.type == "cuda" and device.index is None else device
+        state = {k: v.double() for k, v in vae.state_dict().items()}
+        self._mu_weight = self._mu_bias = None
+        n = len(vae.nhiddens)
+        self._encoder = self._folded(state, "encoder", n, "mu")
+        self._decoder = self._folded(state, "decoder", n, "outputlayer")
+        g = _torch.Generator(device="cpu").manual_seed(seed)
+        self.down, self.up = [], []
+        for s in self._encoder:
+            bound = s.k ** -0.5
+            d = (_torch.rand((n_groups, rank, s.k), generator=g) * 2 - 1) * bound
+            self.down.append(d.to(self.device))
+            self.up.append(_torch.zeros((n_groups, s.n, rank), device=self.device))
+        self._generator = _torch.Generator(device=self.device).manual_seed(seed)
+        # the decoder's layers have no adapters: no row asks for this one
+        self._none = [(_torch.zeros((1, 1, s.k), dtype=s.dtype, device=self.device), _torch.zeros((1, s.n, 1), dtype=s.dtype, device=self.device))
+                      for s in self._decoder]
+
+    def _folded(self, state, kind: str, n: int, last: str):
+        """The layers' weights with the BatchNorm in front of each folded in: W (a x + c) + b = (W a) x + (W c + b)."""
+        layers, a, c = [], None, None
+        for i, name in enumerate([f"{kind}layers.{i}" for i in range(n)] + [last]):
+            w, b = state[name + ".weight"], state[name + ".bias"]
+            if a is not None:
+                w, b = w * a, w @ c + b
+            dtype = _torch.float32 if name == "mu" else self.dtype
+            w, b = (t.float().to(self.device, dtype).contiguous() for t in (w, b))
+            if name == "mu":
+                self._mu_weight, self._mu_bias = w, b
+            layers.append(SharedProjection(w, b))
+            if i < n:
+                norm = f"{kind}norms.{i}"
+                a = state[norm + ".weight"] / (state[norm + ".running_var"] + _BN_EPS).sqrt()
+                c = state[norm + ".bias"] - state[norm + ".running_mean"] * a
+        return layers
+
+    def _pairs(self):
+        """The adapters in the types that the layers compute in."""
+        return [(d.to(s.dtype), u.to(s.dtype)) for d, u, s in zip(self.down, self.up, self._encoder)]
+
+    # ---- data -------------------------------------------------------------------------------------------------------------------
+    def _features(self, data_loader):
+        tensors = data_loader.dataset.tensors
+        if len(tensors) != 4:
+            raise ValueError("expected a DataLoader made by make_dataloader (4 tensors)")
+        parts = [_torch.as_tensor(t[:]) for t in tensors]
+        n = len(parts[0])
+        if parts[0].shape != (n, self.nsamples) or parts[1].shape != (n, self.ntnf) or parts[2].shape != (n, 1) or parts[3].shape != (n, 1):
+            raise ValueError("dataset tensors do not match this VAE (nsamples / 103 TNF / 1 / 1 columns)")
+        return _torch.cat(parts[:3], dim=1).to(self.device), parts[3].to(self.device)
+
+    def _groups(self, groups, n: int) -> _torch.Tensor:
+        g = _torch.as_tensor(groups)
+        if g.dim() != 1 or len(g) != n or g.dtype.is_floating_point or g.dtype in (_torch.bool, _torch.complex64, _torch.complex128):
+            raise ValueError(f"groups must be {n} integers, one per contig")
+        g = g.to(self.device, _torch.int64)
+        return _torch.where((g >= 0) & (g < self.n_groups), g, -1).to(_torch.int32)
+
+    # ---- encode -----------------------------------------------------------------------------------------------------------------
+    def encode(self, data_loader, groups, batchsize: int = 262144):
+        """Latents ``[n, nlatent]`` like ``VAE.encode`` (float32, the low 12 mantissa bits cleared, vambtools.py:324-330)."""
+        if batchsize < 1:
+            raise ValueError(f"batchsize must be at least 1, not {batchsize}")
+        x, _ = self._features(data_loader)
+        g = self._groups(groups, len(x))
+        pairs = self._pairs()
+        out = []
+        for at in range(0, len(x), batchsize):
+            plan = group_rows(g[at:at + batchsize], self.n_groups)
+            h = x[at:at + batchsize].to(self.dtype)
+            for i, (s, (d, u)) in enumerate(zip(self._encoder, pairs)):
+                last = i == len(pairs) - 1
+                h = adapted_linear(h.to(s.dtype), s, d, u, plan, self.scale, None if last else _SLOPE)
+            out.append((h.view(_torch.int32) & ~0xfff).view(_torch.float32))
+        if not out:
+            return _torch.empty((0, self.nlatent)).numpy()
+        return _torch.cat(out).cpu().numpy()
+
+    # ---- training ---------------------------------------------------------------------------------------------------------------
+    def gradients(self, x, weights, groups, noise, mu_too: bool = False):
+        """``(loss, gradients of down, gradients of up, gradients of mu's weight and bias or None)`` of one batch: ``x`` float32 ``[rows, columns]``,
+        ``weights`` ``[rows, 1]``, ``groups`` int32 ``[rows]``, ``noise`` the reparameterisation noise ``[rows, nlatent]``.  The loss is
+        ``VAE.calc_loss`` (encode.py:316-357), whose ``[rows] * [rows, 1]`` means the product of two means."""
+        rows = len(x)
+        plan, alone = group_rows(groups, self.n_groups), group_rows(_torch.full_like(groups, -1), 1)
+        pairs = self._pairs()
+        last = len(pairs) - 1
+        # forward: every layer leaves its input's checkpoint and its own (whose signs are the derivative)
+        h, held, low = x.to(self.dtype), [checkpoint8(x.to(self.dtype))], []
+        for i, (s, (d, u)) in enumerate(zip(self._encoder, pairs)):
+            h, l, c = adapted_linear_train(h.to(s.dtype), s, d, u, plan, self.scale, None if i == last else _SLOPE)
+            held.append(c)
+            low.append(l)
+        mu = h
+        h = (mu + noise).to(self.dtype)
+        kept = [checkpoint8(h)]
+        for i, (s, (d, u)) in enumerate(zip(self._decoder, self._none)):
+            h, zero, c = adapted_linear_train(h, s, d, u, alone, 0.0, None if i == len(self._decoder) - 1 else _SLOPE)
+            kept.append((c, zero))
+        out = h.float()
+        # loss and its gradient
+        ns, nt = self.nsamples, self.ntnf
+        mean_w = weights.mean()
+        per = mean_w / rows
+        do = _torch.empty_like(out)
+        ab_w, sse_w, kld_w = (1 - self.alpha) / ns, self.alpha / nt, 1 / (self.nlatent * self.beta)
+        diff = out[:, ns:] - x[:, ns:]
+        loss = (diff[:, :nt].square().sum(1) * sse_w + diff[:, nt:].square().sum(1) * ab_w + 0.5 * mu.square().sum(1) * kld_w)
+        do[:, ns:ns + nt] = diff[:, :nt] * (2 * sse_w * per)
+        do[:, ns + nt:] = diff[:, nt:] * (2 * ab_w * per)
+        if ns > 1:
+            ce_w = (1 - self.alpha) * (ns - 1) / (ns * math.log(ns))
+            p = _torch.softmax(out[:, :ns], dim=1)
+            loss = loss - ((p + 1e-9).log() * x[:, :ns]).sum(1) * ce_w
+            dp = x[:, :ns] / (p + 1e-9)
+            do[:, :ns] = p * ((dp * p).sum(1, keepdim=True) - dp) * (ce_w * per)
+        else:
+            do[:, :ns] = 0.0
+        loss = loss.mean() * mean_w
+        # backward
+        dh = do.to(self.dtype)
+        for i in range(len(self._decoder) - 1, -1, -1):
+            c, zero = kept[i + 1]
+            below = kept[i] if i == 0 else kept[i][0]
+            dh, _, _ = adapted_linear_backward(dh, below, c, zero, self._decoder[i], *self._none[i], alone, 0.0,
+                                               None if i == len(self._decoder) - 1 else _SLOPE)
+        dh = dh.float() + mu * (kld_w * per)
+        downs, ups, shared = [None] * (last + 1), [None] * (last + 1), None
+        for i in range(last, -1, -1):
+            s, (d, u) = self._encoder[i], pairs[i]
+            slope = None if i == last else _SLOPE
+            if i == last and mu_too:
+                shared = checkpoint_weight_grad(dh, held[i])
+            dh, dd, du = adapted_linear_backward(dh.to(s.dtype), held[i], held[i + 1], low[i], s, d, u, plan, self.scale, slope, need_dx=i > 0)
+            downs[i], ups[i] = dd.float(), du.float()
+        return loss, downs, ups, shared
+
+    def train(self, data_loader, groups, nepochs: int = 10, batchsize: int = 4096, lrate: float = 1e-3, mu_too: bool = False):
+        """Train the adapters (Adam) for ``nepochs`` epochs over shuffled batches; ``mu_too``: the shared ``mu`` layer with them.  Returns
+        the mean loss of every epoch."""
+        if nepochs < 1:
+            raise ValueError(f"Minimum 1 epoch, not {nepochs}")
+        if batchsize < 1:
+            raise ValueError(f"batchsize must be at least 1, not {batchsize}")
+        if not lrate > 0:
+            raise ValueError(f"lrate must be > 0, not {lrate}")
+        x, w = self._features(data_loader)
+        g = self._groups(groups, len(x))
+        n = len(x)
+        if n < 1:
+            raise ValueError("cannot train on a dataset without sequences")
+        batch = min(batchsize, n)
+        shared = [self._mu_weight, self._mu_bias] if mu_too else []
+        params = [*self.down, *self.up, *shared]
+        optimizer = _torch.optim.Adam(params, lr=lrate)
+        losses = []
+        for _ in range(nepochs):
+            order = _torch.randperm(n, generator=self._generator, device=self.device)
+            total = []
+            for at in range(0, n - batch + 1, batch):     # the ragged tail is dropped, as by make_dataloader's loader
+                rows = order[at:at + batch]
+                noise = _torch.randn((batch, self.nlatent), generator=self._generator, device=self.device)
+                loss, downs, ups, mu_grads = self.gradients(x[rows], w[rows], g[rows], noise, mu_too)
+                for p, grad in zip(params, [*downs, *ups, *(mu_grads or ())]):
+                    p.grad = grad
+                optimizer.step()
+                optimizer.zero_grad(set_to_none=True)
+                if mu_too:
+                    self._encoder[-1] = SharedProjection(self._mu_weight, self._mu_bias)
+                total.append(loss)
+            losses.append(float(_torch.stack(total).mean()))
+        return losses
+
+    # ---- files ------------------------------------------------------------------------------------------------------------------
+    def save(self, file) -> None:
+        _torch.save({"n_groups": self.n_groups, "rank": self.rank, "scale": self.scale, "down": [t.cpu() for t in self.down],
+                     "up": [t.cpu() for t in self.up], "mu": [self._mu_weight.cpu(), self._mu_bias.cpu()]}, file)
+
+    @classmethod
+    def load(cls, file, vae, dtype: Optional[_torch.dtype] = None, device: Union[str, _torch.device] = "cuda"):
+        """Adapters that :meth:`save` wrote, on the VAE that they were made for."""
+        d = _torch.load(file, map_location="cpu", weights_only=True)
+        self = cls(vae, d["n_groups"], d["rank"], d["scale"], dtype=dtype, device=device)
+        for mine, saved in ((self.down, d["down"]), (self.up, d["up"])):
+            if [tuple(t.shape) for t in mine] != [tuple(t.shape) for t in saved]:
+                raise ValueError("the saved adapters do not match this VAE")
+            for m, t in zip(mine, saved):
+                m.copy_(t)
+        self._mu_weight, self._mu_bias = (t.to(self.device) for t in d["mu"])
+        self._encoder[-1] = SharedProjection(self._mu_weight, self._mu_bias)
+        return self

@@ -843,6 +843,12 @@ class VAE:
         _lib.check(self._lib.vh_vae_encode(self._h, _lib.ptr(latent)))
         return latent
 
+    def adapters(self, n_groups: int, rank: int = 8, **kwargs):
+        """Low-rank adapters of this (trained) VAE's encoder, one set per sample: ``vamb_amd.adapters.VAEAdapters``, which trains
+        them and encodes with them.  No counterpart in the reference."""
+        from .adapters import VAEAdapters
+        return VAEAdapters(self, n_groups, rank, **kwargs)
+
     # ---- model.pt (encode.py:486-541) ---------------------------------------------------------------
     def save(self, filehandle):
         state = {"nsamples": self.nsamples, "alpha": self.alpha, "beta": self.beta, "dropout": self.dropout,
