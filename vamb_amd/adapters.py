@@ -36,6 +36,8 @@ BLOCK = 32   # columns of a checkpoint that share an exponent
 FEW_ROWS = 64
 
 _DTYPES = {_torch.float32: 0, _torch.bfloat16: 1}
+# the current stream's handle without a Stream object around it (a call here is a few microseconds in all)
+_raw_stream = getattr(_torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: _torch.cuda.current_stream(index).cuda_stream)
 
 
 def _dtype_of(t: _torch.Tensor, what: str) -> int:
@@ -49,15 +51,17 @@ def _matrix(t, what: str, rows: Optional[int] = None, cols: Optional[int] = None
     """Check a [rows, cols] tensor whose rows are contiguous; returns its row stride."""
     if not isinstance(t, _torch.Tensor) or t.dim() != 2:
         raise ValueError(f"{what} must be a two-dimensional tensor")
-    if (rows is not None and t.shape[0] != rows) or (cols is not None and t.shape[1] != cols):
-        raise ValueError(f"{what} must be [{'rows' if rows is None else rows}, {'columns' if cols is None else cols}], not {list(t.shape)}")
-    if t.shape[1] > 1 and t.stride(1) != 1:
+    n, m = t.shape
+    if (rows is not None and n != rows) or (cols is not None and m != cols):
+        raise ValueError(f"{what} must be [{'rows' if rows is None else rows}, {'columns' if cols is None else cols}], not {[n, m]}")
+    ld, step = t.stride()
+    if m > 1 and step != 1:
         raise ValueError(f"the rows of {what} must be contiguous")
-    if t.shape[0] <= 1:
-        return t.shape[1]
-    if t.stride(0) < t.shape[1]:
-        raise ValueError(f"the rows of {what} overlap (row stride {t.stride(0)}, {t.shape[1]} columns)")
-    return t.stride(0)
+    if n <= 1:
+        return m
+    if ld < m:
+        raise ValueError(f"the rows of {what} overlap (row stride {ld}, {m} columns)")
+    return ld
 
 
 def _dense(t, what: str, shape) -> None:
@@ -67,29 +71,24 @@ def _dense(t, what: str, shape) -> None:
         raise ValueError(f"{what} must be contiguous")
 
 
-class _On:
-    """The device of a call: checks that all tensors are there, makes it current for the library, gives its stream."""
+def _enter(first, *others):
+    """The library's side of a call: all tensors on one GPU, that GPU current; ``(its stream, the device to go back to or None)``."""
+    index = first.get_device()
+    if index < 0:
+        raise ValueError(f"the tensors must be on a GPU, not on {first.device}")
+    for t in others:
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"the tensors of a call must be on one device: {first.device} and {t.device}")
+    before = _torch.cuda.current_device()
+    if before == index:
+        return _raw_stream(index), None
+    _torch.cuda.set_device(index)
+    return _raw_stream(index), before
 
-    __slots__ = ("device", "_before")
 
-    def __init__(self, first, *others):
-        self.device = first.device
-        if self.device.type != "cuda":
-            raise ValueError(f"the tensors must be on a GPU, not on {self.device}")
-        for t in others:
-            if t is not None and t.device != self.device:
-                raise ValueError(f"the tensors of a call must be on one device: {self.device} and {t.device}")
-
-    def __enter__(self):
-        self._before = _torch.cuda.current_device()
-        if self._before != self.device.index:
-            _torch.cuda.set_device(self.device)
-        return _torch.cuda.current_stream(self.device).cuda_stream
-
-    def __exit__(self, *exc):
-        if self._before != self.device.index:
-            _torch.cuda.set_device(self._before)
-        return False
+def _leave(before) -> None:
+    if before is not None:
+        _torch.cuda.set_device(before)
 
 
 @lru_cache(maxsize=4096)
@@ -139,11 +138,14 @@ def group_rows(groups: _torch.Tensor, n_groups: int) -> RowGroups:
     if rows == 0:
         return RowGroups(0, n_groups, None)
     lib = _lib.load()
-    with _On(groups) as stream:
+    stream, before = _enter(groups)
+    try:
         words, scratch_words = _plan_words(rows, n_groups)
         plan = _torch.empty(words, dtype=_torch.int32, device=groups.device)
         scratch = _torch.empty(scratch_words, dtype=_torch.int32, device=groups.device) if scratch_words else None
         _lib.check(lib.vh_rows_plan(groups.data_ptr(), rows, n_groups, plan.data_ptr(), scratch.data_ptr() if scratch is not None else None, stream))
+    finally:
+        _leave(before)
     return RowGroups(rows, n_groups, plan)
 
 
@@ -165,12 +167,15 @@ class SharedProjection:
                 raise ValueError(f"bias must have the weight's type {weight.dtype}, not {bias.dtype}")
         self.device = weight.device
         lib = _lib.load()
-        with _On(weight, bias) as stream:
+        stream, before = _enter(weight, bias)
+        try:
             size = ctypes.c_int64()
             _lib.check(lib.vh_adapt_weight_size(self.n, self.k, code, ctypes.byref(size)))
             self.packed = _torch.empty(size.value, dtype=_torch.uint8, device=weight.device)
             _lib.check(lib.vh_adapt_weight_pack(weight.data_ptr(), ld, bias.data_ptr() if bias is not None else None, self.n, self.k, code,
                                                 self.packed.data_ptr(), stream))
+        finally:
+            _leave(before)
 
 
 def _layer(shared, down, up, n_groups, scale, negative_slope):
@@ -224,7 +229,8 @@ def adapted_linear(x, shared: SharedProjection, down, up, groups: Union[_torch.T
     if (groups.rows if planned else groups.shape[0]) != rows:
         raise ValueError(f"x has {rows} rows, groups {groups.rows if planned else groups.shape[0]}")
     lib = _lib.load()
-    with _On(x, shared.packed, down, up, groups.plan if planned else groups) as stream:
+    stream, before = _enter(x, shared.packed, down, up, groups.plan if planned else groups)
+    try:
         y = _torch.empty((rows, shared.n), dtype=x.dtype, device=x.device)
         if rows == 0:
             return y
@@ -234,6 +240,8 @@ def adapted_linear(x, shared: SharedProjection, down, up, groups: Union[_torch.T
         if not planned:
             groups = group_rows(groups, n_groups)
         _lib.check(lib.vh_adapt_forward(layer, x.data_ptr(), ld, rows, groups.plan.data_ptr(), y.data_ptr(), shared.n, None, None, None, stream))
+    finally:
+        _leave(before)
     return y
 
 
@@ -248,13 +256,16 @@ def adapted_linear_train(x, shared: SharedProjection, down, up, groups: RowGroup
     if groups.rows != rows:
         raise ValueError(f"x has {rows} rows, groups {groups.rows}")
     lib = _lib.load()
-    with _On(x, shared.packed, down, up, groups.plan) as stream:
+    stream, before = _enter(x, shared.packed, down, up, groups.plan)
+    try:
         y = _torch.empty((rows, shared.n), dtype=x.dtype, device=x.device)
         low = _torch.empty((rows, down.shape[1]), dtype=_torch.float32, device=x.device)
         held = Checkpoint8._empty(rows, shared.n, x.device)
         if rows:
             _lib.check(lib.vh_adapt_forward(layer, x.data_ptr(), ld, rows, groups.plan.data_ptr(), y.data_ptr(), shared.n, low.data_ptr(),
                                             held.codes.data_ptr(), held.exponents.data_ptr(), stream))
+    finally:
+        _leave(before)
     return y, low, held
 
 
@@ -279,7 +290,8 @@ def adapted_linear_backward(dy, x, y, low, shared: SharedProjection, down, up, g
     if low.dtype != _torch.float32:
         raise ValueError(f"low must be float32, not {low.dtype}")
     lib = _lib.load()
-    with _On(dy, shared.packed, down, up, groups.plan, tx, ty, low) as stream:
+    stream, before = _enter(dy, shared.packed, down, up, groups.plan, tx, ty, low)
+    try:
         dx = _torch.empty((rows, shared.k), dtype=dy.dtype, device=dy.device) if need_dx else None
         if rows == 0:
             return dx, _torch.zeros_like(down), _torch.zeros_like(up)
@@ -287,6 +299,8 @@ def adapted_linear_backward(dy, x, y, low, shared: SharedProjection, down, up, g
         scratch = _torch.empty(_backward_words(rows, groups.groups, shared.n, shared.k, rank, layer.dtype), dtype=_torch.float32, device=dy.device)
         _lib.check(lib.vh_adapt_backward(layer, dy.data_ptr(), ld, held_x, held_y, low.data_ptr(), rows, groups.plan.data_ptr(),
                                          dx.data_ptr() if need_dx else None, shared.k, ddown.data_ptr(), dup.data_ptr(), scratch.data_ptr(), stream))
+    finally:
+        _leave(before)
     return dx, ddown, dup
 
 
@@ -337,11 +351,14 @@ class Checkpoint8:
             raise ValueError(f"a checkpoint is restored to float32 or bfloat16, not {dtype}")
         rows = self.codes.shape[0]
         lib = _lib.load()
-        with _On(self.codes) as stream:
+        stream, before = _enter(self.codes)
+        try:
             out = _torch.empty((rows, self.columns), dtype=dtype, device=self.codes.device)
             if rows:
                 _lib.check(lib.vh_checkpoint8_restore(self.codes.data_ptr(), self.exponents.data_ptr(), rows, self.columns, _DTYPES[dtype],
                                                       out.data_ptr(), stream))
+        finally:
+            _leave(before)
         return out
 
 
@@ -353,10 +370,13 @@ def checkpoint8(x: _torch.Tensor) -> Checkpoint8:
     if columns < 1:
         raise ValueError("x must have at least one column")
     lib = _lib.load()
-    with _On(x) as stream:
+    stream, before = _enter(x)
+    try:
         held = Checkpoint8._empty(rows, columns, x.device)
         if rows:
             _lib.check(lib.vh_checkpoint8(x.data_ptr(), ld, rows, columns, code, held.codes.data_ptr(), held.exponents.data_ptr(), stream))
+    finally:
+        _leave(before)
     return held
 
 
@@ -390,7 +410,8 @@ def checkpoint_weight_grad(dy, x: Checkpoint8, y=None, negative_slope: Optional[
     # (without an activation y plays no part, as in adapted_linear_backward)
     held_y, ty = _held(y, "y", rows, n, dy.dtype) if y is not None else (None, None)
     lib = _lib.load()
-    with _On(dy, tx, ty) as stream:
+    stream, before = _enter(dy, tx, ty)
+    try:
         if rows == 0:
             return _torch.zeros((n, k), dtype=dy.dtype, device=dy.device), _torch.zeros(n, dtype=dy.dtype, device=dy.device)
         dweight = _torch.empty((n, k), dtype=dy.dtype, device=dy.device)
@@ -398,6 +419,8 @@ def checkpoint_weight_grad(dy, x: Checkpoint8, y=None, negative_slope: Optional[
         scratch = _torch.empty(_weight_grad_words(rows, n, k), dtype=_torch.float32, device=dy.device)
         _lib.check(lib.vh_checkpoint8_weight_grad(dy.data_ptr(), ld, held_x, held_y if negative_slope is not None else None,
                                                   negative_slope or 0.0, rows, n, k, code, dweight.data_ptr(), dbias.data_ptr(), scratch.data_ptr(), stream))
+    finally:
+        _leave(before)
     return dweight, dbias
 
 

@@ -106,47 +106,63 @@ __device__ __forceinline__ void load_keys(const int* groups, int64_t row0, int64
         key[b] = row < hi ? ((unsigned)key[b] < (unsigned)G ? key[b] : G) : G + 1;   // G + 1: no row
     }
 }
-__device__ __forceinline__ void place_rows(const int* groups, int64_t lo, int64_t hi, int G, int bits, int* counter, int* plan, const PlanShape& ps) {
+// (rows that are in the order of their groups already: 64 equal keys are one count and one run of slots)
+__device__ __forceinline__ bool all_equal(int key) { return __all(key == __builtin_amdgcn_readfirstlane(key)); }
+__device__ __forceinline__ void place_keys(const int (&key)[PB], int64_t row0, int64_t hi, int G, int bits, int* counter, int* plan, const PlanShape& ps) {
     const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int b = 0; b < PB; ++b) {
+        if (row0 + 64 * b >= hi) break;
+        const unsigned long long same = all_equal(key[b]) ? ~0ull : same_key(key[b], bits);
+        const int rank = __popcll(same & ((1ull << lane) - 1));
+        if (key[b] <= G) {
+            const int slot = counter[key[b]] + rank;
+            plan[ps.o_row + slot] = (int)(row0 + 64 * b + lane);
+            if ((slot & 15) == 0) plan[ps.o_sub + slot / 16] = key[b] < G ? key[b] : -1;
+        }
+        __builtin_amdgcn_wave_barrier();   // every lane has read its counter (LDS operations of a wave complete in order)
+        if (key[b] <= G && rank == 0) counter[key[b]] += __popcll(same);
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+__device__ __forceinline__ void count_keys(const int (&key)[PB], int G, int* counter) {
+#pragma unroll
+    for (int b = 0; b < PB; ++b) {
+        if (all_equal(key[b])) {
+            if ((threadIdx.x & 63) == 0 && key[b] <= G) counter[key[b]] += 64;   // (the wave's own counters)
+        } else if (key[b] <= G) {
+            atomicAdd(&counter[key[b]], 1);   // integers: any order
+        }
+    }
+}
+__device__ __forceinline__ void place_rows(const int* groups, int64_t lo, int64_t hi, int G, int bits, int* counter, int* plan, const PlanShape& ps) {
     for (int64_t row0 = lo; row0 < hi; row0 += 64 * PB) {
         int key[PB];
         load_keys(groups, row0, hi, G, key);
-#pragma unroll
-        for (int b = 0; b < PB; ++b) {
-            if (row0 + 64 * b >= hi) break;
-            const unsigned long long same = same_key(key[b], bits);
-            const int rank = __popcll(same & ((1ull << lane) - 1));
-            if (key[b] <= G) {
-                const int slot = counter[key[b]] + rank;
-                plan[ps.o_row + slot] = (int)(row0 + 64 * b + lane);
-                if ((slot & 15) == 0) plan[ps.o_sub + slot / 16] = key[b] < G ? key[b] : -1;
-            }
-            __builtin_amdgcn_wave_barrier();   // every lane has read its counter (LDS operations of a wave complete in order)
-            if (key[b] <= G && rank == 0) counter[key[b]] += __popcll(same);
-            __builtin_amdgcn_wave_barrier();
-        }
+        place_keys(key, row0, hi, G, bits, counter, plan, ps);
     }
 }
 __device__ __forceinline__ void count_rows(const int* groups, int64_t lo, int64_t hi, int G, int* counter) {
     for (int64_t row0 = lo; row0 < hi; row0 += 64 * PB) {
         int key[PB];
         load_keys(groups, row0, hi, G, key);
-#pragma unroll
-        for (int b = 0; b < PB; ++b)
-            if (key[b] <= G) atomicAdd(&counter[key[b]], 1);   // integers: any order
+        count_keys(key, G, counter);
     }
 }
 
-constexpr int kSmallRows = 16384, kSmallCounters = 16 * 1024;   // one workgroup: 16 waves' counters in 64 KB
+constexpr int kSmallRows = 1024 * PB, kSmallCounters = 16 * 1024;   // one workgroup: 16 waves' counters in 64 KB
 
 __global__ __launch_bounds__(1024) void plan_small_kernel(const int* groups, int* plan, PlanShape ps, int bits) {
     extern __shared__ int counters[];   // [16][G + 1]
     __shared__ int lds[48];
     const int G = (int)ps.groups, wave = threadIdx.x >> 6;
+    // at most PB keys a lane: they stay in registers
+    const int64_t seg = (ps.rows + 1023) / 1024 * 64, lo = min(wave * seg, ps.rows), hi = min(lo + seg, ps.rows);
+    int key[PB];
+    if (lo < hi) load_keys(groups, lo, hi, G, key);
     for (int i = threadIdx.x; i < 16 * (G + 1); i += 1024) counters[i] = 0;
     __syncthreads();
-    const int64_t seg = (ps.rows + 1023) / 1024 * 64, lo = min(wave * seg, ps.rows), hi = min(lo + seg, ps.rows);
-    count_rows(groups, lo, hi, G, counters + wave * (G + 1));
+    if (lo < hi) count_keys(key, G, counters + wave * (G + 1));
     __syncthreads();
     plan_offsets(plan, ps, lds,
                  [&](int g) {
@@ -162,7 +178,7 @@ __global__ __launch_bounds__(1024) void plan_small_kernel(const int* groups, int
                      }
                  });
     __syncthreads();
-    place_rows(groups, lo, hi, G, bits, counters + wave * (G + 1), plan, ps);
+    if (lo < hi) place_keys(key, lo, hi, G, bits, counters + wave * (G + 1), plan, ps);
 }
 
 // Larger: one wave per piece of rows; counts [G + 1][pieces], then run totals [G + 1] behind them
@@ -365,6 +381,19 @@ __device__ __forceinline__ void store8(T* p, const float (&v)[8], int n) {
             if (e < n) p[e] = from_f<T>(v[e]);
     }
 }
+template <class T>
+__device__ __forceinline__ void store4(T* p, f32x4 v, int n) {
+    if (n >= 4) {
+        if constexpr (sizeof(T) == 2)
+            *reinterpret_cast<u32x2_any*>(p) = u32x2{f_to_bf(v[0]) | (unsigned)f_to_bf(v[1]) << 16, f_to_bf(v[2]) | (unsigned)f_to_bf(v[3]) << 16};
+        else
+            *reinterpret_cast<f32x4_any*>(p) = v;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i < n) p[i] = from_f<T>(v[i]);
+    }
+}
 // f'(y) of eight columns applied to f
 template <class T>
 __device__ __forceinline__ void masked8(const Source& s, const Eight<T>& v, float slope, float (&f)[8]) {
@@ -377,7 +406,7 @@ __device__ __forceinline__ void masked8(const Source& s, const Eight<T>& v, floa
 
 // =====================================================================================================================
 // Gradients of the adapters:  down_g = sum v^T x  [rank][K],  up_g = s sum p^T u  [N][rank]
-// One workgroup = one item (at most item_rows rows of one group) and 128 columns of x or of p.  v_mfma_f32_16x16x4_f32: its operands
+// One wave = one item (at most item_rows rows of one group) and 128 columns of x or of p.  v_mfma_f32_16x16x4_f32: its operands
 // are one element per lane, so eight consecutive columns that a lane has read are the operands of eight instructions and nothing is
 // transposed; products and sums are fp32 whatever the tensors' type.
 // =====================================================================================================================
@@ -388,19 +417,21 @@ struct AdapterGradArgs {
     const float* low;          // u [rows][rank], from the forward pass
     const float* v;            // [rows][rank], s included
     void *ddown, *dup;
+    const void* up;            // [groups][N][rank], and ...
+    void* turned;              // ... [groups][rank][N]
     float* parts;
     int K, N, rank;
     float scale, slope;
     const int* plan;
     PlanShape ps;
-    int down_tiles;
 };
 
-// `whole`: the tile's 128 columns exist (the same for the workgroup), so that its loads need no branch
+// One wave: an item's rows and 128 columns.  WHOLE: all of them exist, so that the loads need no branch.
 template <class T, int RT, bool UP, bool WHOLE>
-__device__ __forceinline__ void adapter_grad_tile(const AdapterGradArgs& a, int g, int first, int count, int part, int tile0, f32x4 (*red)[8][64]) {
+__device__ __forceinline__ void adapter_grad_tile(const AdapterGradArgs& a, const int* it, int tile0) {
+    const int g = it[0], first = it[1], count = it[2], part = it[3];
     const int* slot_row = a.plan + a.ps.o_row;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l15 = lane & 15, quad = lane >> 4;
+    const int lane = threadIdx.x & 63, l15 = lane & 15, quad = lane >> 4;
     const int C = UP ? a.N : a.K, c0 = tile0 + 8 * l15, valid = WHOLE ? 8 : C - c0, r = a.rank;
     const float* small = UP ? a.low : a.v;
     const Source wide = UP ? Source{a.dy, nullptr, a.ldy} : a.x;
@@ -412,13 +443,13 @@ __device__ __forceinline__ void adapter_grad_tile(const AdapterGradArgs& a, int 
 #pragma unroll
         for (int e = 0; e < 8; ++e) acc[j][e] = f32x4{0, 0, 0, 0};
 
-    // a wave takes eight rows a step (two of each quad), the workgroup 32
-    Eight<T> w[2], m[2];
-    float s[2][RT];
+    constexpr int H = 2;   // rows of a quad a step: 4 H rows
+    Eight<T> w[H], m[H];
+    float s[H][RT];
     auto row_of = [&](int i) { return i < count ? slot_row[first + i] : -1; };
-    auto fetch = [&](const int (&rid)[2]) {
+    auto fetch = [&](const int (&rid)[H]) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < H; ++h) {
             const int row = max(rid[h], 0);   // (a row that is not there is read as row 0 and counts with a factor of zero ...)
             read8<T>(wide, row, c0, valid, w[h]);
             if (masked) read8<T>(a.mask, row, c0, valid, m[h]);
@@ -426,17 +457,16 @@ __device__ __forceinline__ void adapter_grad_tile(const AdapterGradArgs& a, int 
             for (int j = 0; j < RT; ++j) s[h][j] = small[(int64_t)row * r + min(16 * j + l15, r - 1)];
         }
     };
-    int rid[2], nxt[2];
-    const int i0 = 8 * wave + quad;
+    int rid[H], nxt[H];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) rid[h] = row_of(i0 + 4 * h);
+    for (int h = 0; h < H; ++h) rid[h] = row_of(quad + 4 * h);
+#pragma unroll
+    for (int h = 0; h < H; ++h) nxt[h] = row_of(quad + 4 * (H + h));
     fetch(rid);
+    for (int i = 0; i < count; i += 4 * H) {
+        float f[H][8], sc[H][RT];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) nxt[h] = row_of(i0 + 32 + 4 * h);
-    for (int i = 8 * wave; i < count; i += 32) {
-        float f[2][8], sc[2][RT];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < H; ++h) {
             values8<T>(wide, w[h], f[h]);
             if (masked) masked8<T>(a.mask, m[h], a.slope, f[h]);
 #pragma unroll
@@ -445,74 +475,95 @@ __device__ __forceinline__ void adapter_grad_tile(const AdapterGradArgs& a, int 
             for (int j = 0; j < RT; ++j) sc[h][j] = rid[h] >= 0 && 16 * j + l15 < r ? s[h][j] : 0.f;
             rid[h] = nxt[h];
         }
-        if (i + 32 < count) {
+        if (i + 4 * H < count) {
             fetch(rid);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) nxt[h] = row_of(i + quad + 64 + 4 * h);
+            for (int h = 0; h < H; ++h) nxt[h] = row_of(i + quad + 4 * (2 * H + h));
         }
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < H; ++h)
 #pragma unroll
             for (int j = 0; j < RT; ++j)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) acc[j][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(sc[h][j], f[h][e], acc[j][e], 0, 0, 0);
     }
-    // the four waves' sums, in their order; 16 ranks x 128 columns at a time, every thread eight neighbouring results
     const int64_t pair = (int64_t)r * (a.K + a.N);
     float* po = part >= 0 ? a.parts + part * pair + (UP ? (int64_t)r * a.K : 0) : nullptr;
     T* dst = UP ? (T*)a.dup + (int64_t)g * a.N * r : (T*)a.ddown + (int64_t)g * r * a.K;
 #pragma unroll
     for (int j = 0; j < RT; ++j) {
-        if (j) __syncthreads();
-#pragma unroll
-        for (int e = 0; e < 8; ++e) red[wave][e][lane] = acc[j][e];
-        __syncthreads();
-        float v[8];
-        int64_t at;
-        int n;
-        if constexpr (UP) {   // up [N][rank]: thread = column, eight ranks
-            const int col = tid >> 1, rank = 16 * j + 8 * (tid & 1), q = 2 * (tid & 1);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                f32x4 t = red[0][col & 7][16 * (q + h) + (col >> 3)];
-#pragma unroll
-                for (int wv = 1; wv < 4; ++wv) t += red[wv][col & 7][16 * (q + h) + (col >> 3)];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) v[4 * h + i] = t[i] * a.scale;
-            }
-            at = (int64_t)(tile0 + col) * r + rank;
-            n = tile0 + col < C ? r - rank : 0;
-        } else {              // down [rank][K]: thread = rank, eight columns
-            const int rk = tid >> 4, cc = tid & 15;
+        const int rank = 16 * j + 4 * quad;
+        if constexpr (UP) {   // up [N][rank]: four ranks of each of eight columns
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                float t = 0.f;
-#pragma unroll
-                for (int wv = 0; wv < 4; ++wv) t += red[wv][e][16 * (rk >> 2) + cc][rk & 3];
-                v[e] = t;   // (v has the scale)
+                const int n = e < valid ? r - rank : 0;
+                const int64_t at = (int64_t)(c0 + e) * r + rank;
+                const f32x4 v = acc[j][e] * a.scale;
+                if (po) store4<float>(po + at, v, n);
+                else store4<T>(dst + at, v, n);
             }
-            at = (int64_t)(16 * j + rk) * a.K + tile0 + 8 * cc;
-            n = 16 * j + rk < r ? C - tile0 - 8 * cc : 0;
+        } else {              // down [rank][K]: eight columns of each of four ranks
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float v[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = acc[j][e][i];   // (v has the scale)
+                const int n = rank + i < r ? valid : 0;
+                const int64_t at = (int64_t)(rank + i) * a.K + c0;
+                if (po) store8<float>(po + at, v, n);
+                else store8<T>(dst + at, v, n);
+            }
         }
-        if (po) store8<float>(po + at, v, n);
-        else store8<T>(dst + at, v, n);
     }
 }
-template <class T, int RT>
-__global__ __launch_bounds__(256) void adapter_grad_kernel(AdapterGradArgs a) {
-    __shared__ __attribute__((aligned(16))) f32x4 red[4][8][64];
-    if ((int)blockIdx.x >= a.plan[kPlanItems]) return;
-    const int* it = a.plan + a.ps.o_item + 4 * (int64_t)blockIdx.x;
-    const int g = it[0], first = it[1], count = it[2], part = it[3];
-    const bool up = (int)blockIdx.y >= a.down_tiles;
-    const int tile0 = 128 * ((int)blockIdx.y - (up ? a.down_tiles : 0));
-    if (up) {
-        if (tile0 + 128 <= a.N) adapter_grad_tile<T, RT, true, true>(a, g, first, count, part, tile0, red);
-        else adapter_grad_tile<T, RT, true, false>(a, g, first, count, part, tile0, red);
-    } else {
-        if (tile0 + 128 <= a.K) adapter_grad_tile<T, RT, false, true>(a, g, first, count, part, tile0, red);
-        else adapter_grad_tile<T, RT, false, false>(a, g, first, count, part, tile0, red);
+template <class T, int RT, bool UP>
+__device__ __forceinline__ void adapter_grad_wave(const AdapterGradArgs& a, int item, int tile) {
+    const int C = UP ? a.N : a.K;
+    if (item >= a.plan[kPlanItems] || 128 * tile >= C) return;
+    const int* it = a.plan + a.ps.o_item + 4 * (int64_t)item;
+    if (128 * tile + 128 <= C) adapter_grad_tile<T, RT, UP, true>(a, it, 128 * tile);
+    else adapter_grad_tile<T, RT, UP, false>(a, it, 128 * tile);
+}
+// up [N][rank] of an adapter that some row asks for -> [rank][N], the orientation that dy is contracted with: the projection reads
+// its inner operands 16 bytes at a time along the depth.  64 columns, all ranks.
+template <class T>
+__device__ __forceinline__ void turn_up(const AdapterGradArgs& a, int item, int n0, T* tile /* [64][rank | 1] */) {
+    if (item >= a.plan[kPlanItems]) return;
+    const int* it = a.plan + a.ps.o_item + 4 * (int64_t)item;
+    if (it[2] == 0 || (item > 0 && it[-4] == it[0])) return;   // no rows; a later piece of the same group
+    const int r = a.rank, pitch = r | 1, n = min(64, a.N - n0), tid = threadIdx.x;
+    const T* src = (const T*)a.up + (int64_t)it[0] * a.N * r + (int64_t)n0 * r;   // n * rank neighbouring elements
+    T* out = (T*)a.turned + (int64_t)it[0] * a.N * r + n0;
+    for (int i = 8 * tid; i < n * r; i += 8 * 256) {
+        const Raw8<T> v = load8<T>(src + i, n * r - i);
+        int c = i / r, j = i - c * r;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if (i + e < n * r) tile[c * pitch + j] = from_f<T>(v.get(e));
+            if (++j == r) { j = 0; ++c; }
+        }
     }
+    __syncthreads();
+    for (int i = tid; i < 8 * r; i += 256) {
+        const int j = i >> 3, c = 8 * (i & 7);
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = to_f<T>(tile[min(c + e, 63) * pitch + j]);
+        store8<T>(out + (int64_t)j * a.N + c, v, n - c);
+    }
+}
+// before the projection's pass: the gradients of up (four tiles a workgroup), and up turned around (64 columns a workgroup)
+template <class T, int RT>
+__global__ __launch_bounds__(256) void adapter_first_kernel(AdapterGradArgs a) {
+    __shared__ T tile[64 * (kMaxRank + 1)];
+    const int quads = (a.N + 511) / 512;
+    if ((int)blockIdx.y < quads) adapter_grad_wave<T, RT, true>(a, blockIdx.x, 4 * (int)blockIdx.y + ((int)threadIdx.x >> 6));
+    else turn_up<T>(a, blockIdx.x, 64 * ((int)blockIdx.y - quads), tile);
+}
+// behind it: the gradients of down, which need v
+template <class T, int RT>
+__global__ __launch_bounds__(256) void adapter_last_kernel(AdapterGradArgs a) {
+    adapter_grad_wave<T, RT, false>(a, blockIdx.x, 4 * (int)blockIdx.y + ((int)threadIdx.x >> 6));
 }
 template <class T>
 __global__ __launch_bounds__(256) void adapter_join_kernel(AdapterGradArgs a) {
@@ -526,24 +577,6 @@ __global__ __launch_bounds__(256) void adapter_join_kernel(AdapterGradArgs a) {
     for (int p = 0; p < n; ++p) s += a.parts[(part + p) * pair + i];
     if (i < half) ((T*)a.ddown)[(int64_t)g * half + i] = from_f<T>(s);
     else ((T*)a.dup)[(int64_t)g * a.N * a.rank + i - half] = from_f<T>(s);
-}
-
-// up [N][rank] of the adapters that some row asks for -> [rank][N], the orientation that dy is contracted with: the projection
-// reads its inner operands 16 bytes at a time along the depth
-template <class T>
-__global__ __launch_bounds__(256) void turn_up_kernel(const T* up, T* out, int N, int r, const int* plan, PlanShape ps) {
-    __shared__ T tile[64][kMaxRank + 1];
-    if ((int)blockIdx.x >= plan[kPlanItems]) return;
-    const int* it = plan + ps.o_item + 4 * (int64_t)blockIdx.x;
-    if (it[2] == 0 || (blockIdx.x > 0 && it[-4] == it[0])) return;   // no rows; a later piece of the same group
-    const int64_t base = (int64_t)it[0] * N * r;
-    const int n0 = blockIdx.y * 64, n = min(64, N - n0);
-    for (int i = threadIdx.x; i < n * r; i += 256) tile[i / r][i % r] = up[base + (int64_t)n0 * r + i];
-    __syncthreads();
-    for (int i = threadIdx.x; i < 64 * r; i += 256) {
-        const int j = i >> 6, c = i & 63;
-        if (c < n) out[base + (int64_t)j * N + n0 + c] = tile[c][j];
-    }
 }
 
 // =====================================================================================================================
@@ -673,27 +706,27 @@ __device__ __forceinline__ void weight_grad_tile(const WeightGradArgs& a, int n0
 
     // pieces of eight columns: thread t has column piece t % 16 of rows t / 16 and t / 16 + 32
     const int pc = tid & 15, pr = tid >> 4;
-    Eight<T> pw[2], mw[2], xw[2];
-    auto fetch = [&](int64_t row0) {
+    struct Ahead { Eight<T> pw[2], mw[2], xw[2]; } ahead[2];   // two tiles on their way
+    auto fetch = [&](int64_t row0, Ahead& t) {
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
             const int64_t at = min(row0 + pr + 32 * q, hi - 1);   // (behind the last row: read again, and set to zero in keep)
-            read8<T>(dy, at, n0 + 8 * pc, WHOLE ? 8 : a.N - n0 - 8 * pc, pw[q]);
-            if (masked) read8<T>(a.mask, at, n0 + 8 * pc, WHOLE ? 8 : a.N - n0 - 8 * pc, mw[q]);
-            read8<T>(a.x, at, k0 + 8 * pc, WHOLE ? 8 : a.K - k0 - 8 * pc, xw[q]);
+            read8<T>(dy, at, n0 + 8 * pc, WHOLE ? 8 : a.N - n0 - 8 * pc, t.pw[q]);
+            if (masked) read8<T>(a.mask, at, n0 + 8 * pc, WHOLE ? 8 : a.N - n0 - 8 * pc, t.mw[q]);
+            read8<T>(a.x, at, k0 + 8 * pc, WHOLE ? 8 : a.K - k0 - 8 * pc, t.xw[q]);
         }
     };
     float bsum[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) bsum[e] = 0.f;
-    auto keep = [&](unsigned char* buf, int64_t row0) {
+    auto keep = [&](unsigned char* buf, int64_t row0, const Ahead& t) {
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
             const int row = pr + 32 * q, at = row * 256 + (((pc >> 1) ^ tr_swz(row)) * 32 + (pc & 1) * 16);
             const bool in = row0 + row < hi;
             float f[8];
-            values8<T>(dy, pw[q], f);
-            if (masked) masked8<T>(a.mask, mw[q], a.slope, f);
+            values8<T>(dy, t.pw[q], f);
+            if (masked) masked8<T>(a.mask, t.mw[q], a.slope, f);
             Raw8<T> o;
             o.zero();
 #pragma unroll
@@ -705,7 +738,7 @@ __device__ __forceinline__ void weight_grad_tile(const WeightGradArgs& a, int n0
             const Planes8<T> pl = to_planes(o);
 #pragma unroll
             for (int p = 0; p < P; ++p) *reinterpret_cast<s16x8*>(buf + p * TB + at) = pl.p[p];
-            values8<T>(a.x, xw[q], f);
+            values8<T>(a.x, t.xw[q], f);
             u32x4 xv;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -729,16 +762,7 @@ __device__ __forceinline__ void weight_grad_tile(const WeightGradArgs& a, int n0
         const s16x4 a1 = read_tr(buf + (fr + 4) * 256 + ((piece ^ tr_swz(fr + 4)) * 32) + off);
         return __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
     };
-    fetch(lo);
-    keep(smem, lo);
-    __syncthreads();
-    int cur = 0;
-    for (int64_t row0 = lo; row0 < hi; row0 += BR) {
-        const unsigned char* buf = smem + cur * (P + 1) * TB;
-        unsigned char* nxt = smem + (cur ^ 1) * (P + 1) * TB;
-        const bool more = row0 + BR < hi;
-        if (more) fetch(row0 + BR);
-        __builtin_amdgcn_sched_barrier(0);
+    auto multiply = [&](const unsigned char* buf) {
         s16x8 xf[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) xf[j] = frag(buf + P * TB, wk * 64 + 16 * j);
@@ -752,10 +776,45 @@ __device__ __forceinline__ void weight_grad_tile(const WeightGradArgs& a, int n0
 #pragma unroll
                 for (int p = P - 1; p >= 0; --p) acc[i][j] = mfma32(xf[j], pf[p], acc[i][j]);   // D[k column][n column]
         }
-        __builtin_amdgcn_sched_barrier(0);
-        if (more) keep(nxt, row0 + BR);
+    };
+    unsigned char* const buf0 = smem;
+    unsigned char* const buf1 = smem + (P + 1) * TB;
+    // (rows behind the last one are read as the last and set to zero: every request is in bounds, and no branch is needed)
+    if constexpr (P == 1) {
+        fetch(lo, ahead[0]);
+        fetch(lo + BR, ahead[1]);
+        keep(buf0, lo, ahead[0]);
         __syncthreads();
-        cur ^= 1;
+        for (int64_t row0 = lo; row0 < hi; row0 += 2 * BR) {
+            fetch(row0 + 2 * BR, ahead[0]);
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(buf0);
+            __builtin_amdgcn_sched_barrier(0);
+            keep(buf1, row0 + BR, ahead[1]);
+            __syncthreads();
+            fetch(row0 + 3 * BR, ahead[1]);
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(buf1);
+            __builtin_amdgcn_sched_barrier(0);
+            keep(buf0, row0 + 2 * BR, ahead[0]);
+            __syncthreads();
+        }
+    } else {   // (three planes: the registers of one tile ahead)
+        fetch(lo, ahead[0]);
+        keep(buf0, lo, ahead[0]);
+        __syncthreads();
+        unsigned char *now = buf0, *next = buf1;
+        for (int64_t row0 = lo; row0 < hi; row0 += BR) {
+            fetch(row0 + BR, ahead[0]);
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(now);
+            __builtin_amdgcn_sched_barrier(0);
+            keep(next, row0 + BR, ahead[0]);
+            __syncthreads();
+            unsigned char* const t = now;
+            now = next;
+            next = t;
+        }
     }
     // the two halves' sums
     f32x4* red = reinterpret_cast<f32x4*>(smem);   // [4 waves][16][64]: the tiles are done with (barrier above)
@@ -815,7 +874,7 @@ __global__ __launch_bounds__(256) void weight_join_kernel(const float* parts, in
 // about 256 workgroups, at least 128 rows each
 static int64_t weight_splits(int64_t rows, int64_t n, int64_t k, int64_t* split_rows) {
     const int64_t tiles = ceil_div(n, 128) * ceil_div(k, 128);
-    int64_t want = ceil_div(256, tiles);
+    int64_t want = tiles < 256 ? 256 / tiles : 1;   // one workgroup a CU
     const int64_t most = ceil_div(rows, 128);
     want = want < most ? want : most;
     *split_rows = round_up(ceil_div(rows, want), 64);
@@ -862,10 +921,6 @@ static void check_layer(const vh_adapt_layer* l) {
     check_slope(l->activation, l->negative_slope);
     VH_REQUIRE(l->scale == l->scale && fabsf(l->scale) < __builtin_inff(), "scale must be finite");
 }
-static void run_linear(const LinArgs& a, int dtype, bool backward, hipStream_t s) {
-    if (dtype == VH_BF16) launch_linear_bf16(a, backward, s);
-    else launch_linear_f32(a, backward, s);
-}
 template <class T, int RT>
 static void launch_few(const FewArgs& a, hipStream_t s) {
     few_kernel<T, RT><<<dim3((unsigned)ceil_div(a.N, 16), (unsigned)ceil_div(a.rows, 16)), 512, 0, s>>>(a);
@@ -877,12 +932,14 @@ static void few_rank(const FewArgs& a, hipStream_t s) {
     else if (a.rank <= 32) launch_few<T, 2>(a, s);
     else launch_few<T, 4>(a, s);
 }
-template <class T>
-static void adapter_grads(const AdapterGradArgs& a, hipStream_t s) {
-    const dim3 grid((unsigned)a.ps.items, (unsigned)(a.down_tiles + ceil_div(a.N, 128)));
-    if (a.rank <= 16) adapter_grad_kernel<T, 1><<<grid, 256, 0, s>>>(a);
-    else if (a.rank <= 32) adapter_grad_kernel<T, 2><<<grid, 256, 0, s>>>(a);
-    else adapter_grad_kernel<T, 4><<<grid, 256, 0, s>>>(a);
+template <class T, int RT>
+static void adapter_first(const AdapterGradArgs& a, hipStream_t s) {
+    adapter_first_kernel<T, RT><<<dim3((unsigned)a.ps.items, (unsigned)(ceil_div(a.N, 512) + ceil_div(a.N, 64))), 256, 0, s>>>(a);
+    VH_HIP(hipGetLastError());
+}
+template <class T, int RT>
+static void adapter_last(const AdapterGradArgs& a, hipStream_t s) {
+    adapter_last_kernel<T, RT><<<dim3((unsigned)a.ps.items, (unsigned)ceil_div(a.K, 512)), 256, 0, s>>>(a);
     VH_HIP(hipGetLastError());
     if (a.ps.rows > a.ps.item_rows) {
         const int64_t multis = a.ps.rows / a.ps.item_rows < a.ps.groups ? a.ps.rows / a.ps.item_rows : a.ps.groups;
@@ -890,13 +947,14 @@ static void adapter_grads(const AdapterGradArgs& a, hipStream_t s) {
         VH_HIP(hipGetLastError());
     }
 }
+template <class T>
+static void adapter_grads(const AdapterGradArgs& a, bool last, hipStream_t s) {
+    if (a.rank <= 16) last ? adapter_last<T, 1>(a, s) : adapter_first<T, 1>(a, s);
+    else if (a.rank <= 32) last ? adapter_last<T, 2>(a, s) : adapter_first<T, 2>(a, s);
+    else last ? adapter_last<T, 4>(a, s) : adapter_first<T, 4>(a, s);
+}
 static int64_t turned_words(int64_t groups, int64_t n, int64_t rank, int dtype) {
     return round_up(dtype == VH_BF16 ? ceil_div(groups * n * rank, 2) : groups * n * rank, 4);
-}
-template <class T>
-static void turn_up(const void* up, void* out, int64_t n, int64_t r, const int* plan, const PlanShape& ps, hipStream_t s) {
-    turn_up_kernel<T><<<dim3((unsigned)ps.items, (unsigned)ceil_div(n, 64)), 256, 0, s>>>((const T*)up, (T*)out, (int)n, (int)r, plan, ps);
-    VH_HIP(hipGetLastError());
 }
 static int64_t grad_parts(const PlanShape& ps) { return ps.rows > ps.item_rows ? 2 * (ps.rows / ps.item_rows) : 0; }
 
@@ -1026,7 +1084,8 @@ int vh_adapt_forward(const vh_adapt_layer* l, const void* x, int64_t ldx, int64_
         const int64_t x_bytes = ((rows - 1) * ldx + l->k) * es;
         a.dma = es == 2 && l->k % 8 == 0 && ldx % 8 == 0 && (uintptr_t)x % 16 == 0 && x_bytes < 0xfffffff0ll;   // (down is read at any alignment)
         a.x_bytes = a.dma ? (unsigned)x_bytes : 0;
-        run_linear(a, l->dtype, false, (hipStream_t)stream);
+        if (l->dtype == VH_BF16) launch_linear_bf16(a, false, (hipStream_t)stream);
+        else launch_linear_f32(a, false, (hipStream_t)stream);
     });
 }
 
@@ -1097,7 +1156,28 @@ int vh_adapt_backward(const vh_adapt_layer* l, const void* dy, int64_t lddy, con
         Source mask = {nullptr, nullptr, 0};
         if (l->activation) mask = source_of(y, l->n, "y");
         const PlanShape ps = plan_shape(rows, l->groups);
-        float* v = scratch;
+        VH_REQUIRE((uintptr_t)scratch % 16 == 0, "scratch must be 16-byte aligned");
+        hipStream_t s = (hipStream_t)stream;
+        AdapterGradArgs g{};
+        g.x = xs;
+        g.mask = mask;
+        g.dy = dy;
+        g.ldy = lddy;
+        g.low = low;
+        g.v = scratch;
+        g.ddown = ddown;
+        g.dup = dup;
+        g.up = l->up;
+        float* turned = scratch + round_up(rows * l->rank, 4);
+        g.turned = turned;
+        g.parts = turned + turned_words(l->groups, l->n, l->rank, l->dtype);
+        g.K = (int)l->k;
+        g.N = (int)l->n;
+        g.rank = (int)l->rank;
+        g.scale = l->scale;
+        g.slope = l->negative_slope;
+        g.plan = plan;
+        g.ps = ps;
         const WeightShape ws = weight_shape(l->n, l->k, l->dtype);
         LinArgs a{};
         a.x = dy;
@@ -1109,42 +1189,26 @@ int vh_adapt_backward(const vh_adapt_layer* l, const void* dy, int64_t lddy, con
         a.w = (const bf16_t*)l->packed + ws.planes * ws.fwd;
         a.w_plane = ws.bwd;
         a.ldw = (int)ws.nq;
-        float* turned = scratch + round_up(rows * l->rank, 4);
-        VH_REQUIRE((uintptr_t)scratch % 16 == 0, "scratch must be 16-byte aligned");
-        if (l->dtype == VH_BF16) turn_up<bf16_t>(l->up, turned, l->n, l->rank, plan, ps, (hipStream_t)stream);
-        else turn_up<float>(l->up, turned, l->n, l->rank, plan, ps, (hipStream_t)stream);
         a.inner = turned;
         a.outer = l->down;
         a.K = (int)l->n;
         a.N = (int)l->k;
         a.rank = (int)l->rank;
         a.scale = a.low_scale = l->scale;
-        a.low = v;
+        a.low = scratch;   // v
         a.y = dx;
         a.ldy = lddx;
         a.plan = plan;
         a.ps = ps;
-        run_linear(a, l->dtype, true, (hipStream_t)stream);
-        AdapterGradArgs g{};
-        g.x = xs;
-        g.mask = mask;
-        g.dy = dy;
-        g.ldy = lddy;
-        g.low = low;
-        g.v = v;
-        g.ddown = ddown;
-        g.dup = dup;
-        g.parts = turned + turned_words(l->groups, l->n, l->rank, l->dtype);
-        g.K = (int)l->k;
-        g.N = (int)l->n;
-        g.rank = (int)l->rank;
-        g.scale = l->scale;
-        g.slope = l->negative_slope;
-        g.plan = plan;
-        g.ps = ps;
-        g.down_tiles = (int)ceil_div(l->k, 128);
-        if (l->dtype == VH_BF16) adapter_grads<bf16_t>(g, (hipStream_t)stream);
-        else adapter_grads<float>(g, (hipStream_t)stream);
+        if (l->dtype == VH_BF16) {
+            adapter_grads<bf16_t>(g, false, s);
+            launch_linear_bf16(a, true, s);
+            adapter_grads<bf16_t>(g, true, s);
+        } else {
+            adapter_grads<float>(g, false, s);
+            launch_linear_f32(a, true, s);
+            adapter_grads<float>(g, true, s);
+        }
     });
 }
 

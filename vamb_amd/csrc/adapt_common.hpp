@@ -182,7 +182,7 @@ __device__ __forceinline__ void decode4(unsigned codes, float scale, float (&o)[
 // ---- the row plan -----------------------------------------------------------------------------------------------------------
 // Rows sorted by group (stably: sums over a group's rows have one order), every group's run filled up to a multiple of 16 slots, so that
 // a 16-row MFMA operand has ONE adapter.  Rows whose group is not in [0, groups) stand last, without an adapter.  An "item" is
-// a piece of at most item_rows rows of one group: a workgroup of the gradient kernel; a group of several items ("multi") writes parts
+// a piece of at most item_rows rows of one group: what a wave of the gradient kernels takes; a group of several items ("multi") writes parts
 // that the join kernel adds in their order.  A group without rows has one empty item, which writes its zeros.
 struct PlanShape {
     int64_t rows, groups;
@@ -197,7 +197,7 @@ inline PlanShape plan_shape(int64_t rows, int64_t groups) {
     s.subs = rows / 16 + runs;
     s.slots = 16 * s.subs;
     int64_t ir = (rows / 512 + 15) / 16 * 16;
-    s.item_rows = ir < 256 ? 256 : ir;
+    s.item_rows = ir < 128 ? 128 : ir;
     s.items = groups + rows / s.item_rows;
     s.multis = rows / s.item_rows + 1;
     s.o_row = 16;

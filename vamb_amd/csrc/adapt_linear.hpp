@@ -75,6 +75,7 @@ __device__ __forceinline__ void load4(const float* p, int64_t stride, int valid,
 }
 __device__ __forceinline__ void planes4(const u32x2& r, s16x4 (&o)[1]) { o[0] = __builtin_bit_cast(s16x4, r); }
 __device__ __forceinline__ void planes4(const f32x4& r, s16x4 (&o)[3]) { cut4<3>(r, o); }
+typedef short tr_s16x4 __attribute__((ext_vector_type(4)));
 template <class T> struct Raw4;
 template <> struct Raw4<bf16_t> { typedef u32x2 type; };
 template <> struct Raw4<float> { typedef f32x4 type; };
@@ -415,6 +416,10 @@ __global__ __launch_bounds__(64 * S::WM * S::WN * S::KG) void linear_kernel(LinA
         __syncthreads();
     }
     typename Raw4<T>::type of[RT][NT ? NT : 1];
+    // (behind what other waves may still read: the exchange above, or the groups' sums)
+    constexpr int kLows = WN > 1 ? BM * LS * 4 : (KG - 1) * (NT + RT) * THREADS * 16;
+    unsigned char* const corner = smem + kLows + wave * 512 * (NT ? NT : 1);   // [16 ranks][16 NT columns]
+    static_assert(!(TRANS && P == 1) || kLows + NW * 512 * NT <= KG * 2 * BUF, "the corners fit the tile buffers");
     int have = -1;   // the adapter that `of` holds: neighbouring subtiles mostly have the same
 #pragma unroll
     for (int m = 0; m < MS; ++m) {
@@ -443,7 +448,34 @@ __global__ __launch_bounds__(64 * S::WM * S::WN * S::KG) void linear_kernel(LinA
         if constexpr (NT > 0) {
             const int nw = n0 + wn * NT * 16;
             if (g >= 0) {
-                if (g != have) {
+                if constexpr (TRANS && P == 1) {
+                    // down [rank][N]: 16 ranks x the wave's columns, 16 bytes at a time, to the wave's own corner of the LDS; the
+                    // transposing read gives a lane four ranks of its column
+                    if (g != have) {
+                        have = g;
+                        const T* const base = (const T*)a.outer + (int64_t)g * r * a.N + nw;
+#pragma unroll
+                        for (int j = 0; j < RT; ++j) {
+                            Raw8<T> in[NT / 2];
+#pragma unroll
+                            for (int q = 0; q < NT / 2; ++q) {
+                                const int at = lane + 64 * q, rank = 16 * j + at / (2 * NT), c = 8 * (at % (2 * NT)), left = rank < r ? a.N - nw - c : 0;
+                                in[q] = load8<T>(base + (int64_t)min(rank, r - 1) * a.N + c, left);
+                            }
+#pragma unroll
+                            for (int q = 0; q < NT / 2; ++q) *reinterpret_cast<u32x4*>(corner + (lane + 64 * q) * 16) = in[q].v;
+                            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) {
+                                const int c = 32 * (n >> 1) + 8 * (l15 & 3) + 4 * (n & 1);
+                                const tr_s16x4 t = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                    (__attribute__((address_space(3))) tr_s16x4*)(corner + (4 * quad + (l15 >> 2)) * NT * 32 + 2 * c));
+                                of[j][n] = __builtin_bit_cast(u32x2, t);
+                            }
+                            __builtin_amdgcn_wave_barrier();
+                        }
+                    }
+                } else if (g != have) {
                     have = g;
 #pragma unroll
                     for (int jn = 0; jn < RT * NT; ++jn) {
