@@ -15,12 +15,14 @@ namespace adapt {
 // themselves by ballots over the key's bits, the LDS counter of the wave gives the base.
 // =====================================================================================================================
 __device__ __forceinline__ unsigned long long same_key(int key, int bits) {
-    unsigned long long m = ~0ull;
+    unsigned lo = ~0u, hi = ~0u;
     for (int b = 0; b < bits; ++b) {
-        const unsigned long long v = __ballot((key >> b) & 1);
-        m &= ((key >> b) & 1) ? v : ~v;
+        const unsigned s = (unsigned)__builtin_amdgcn_sbfe(key, b, 1);   // all ones where the bit is set
+        const unsigned long long v = __ballot(s != 0);
+        lo &= ~((unsigned)v ^ s);
+        hi &= ~((unsigned)(v >> 32) ^ s);
     }
-    return m;
+    return (unsigned long long)hi << 32 | lo;
 }
 // exclusive scan over a workgroup of 1024; *total = the sum
 __device__ __forceinline__ int3 block_scan3(int3 v, int3* total, int* lds /* 3 * 16 */) {
@@ -338,18 +340,19 @@ struct Eight {             // eight columns of a row as read
     u32x2 code;
     unsigned exp;
 };
+template <class E>
+__device__ __forceinline__ void read_codes8(const Source& s, int64_t row, int col, int valid, E& o) {
+    o.code = u32x2{0, 0};
+    o.exp = 0;
+    if (valid > 0) {   // rows are filled up to a multiple of 32 codes (of value zero)
+        o.code = *(VH_GLOBAL(u32x2, (const uint8_t*)s.p + row * s.ld + col));
+        o.exp = *(VH_GLOBAL(uint8_t, s.exps + row * (s.ld / kBlockCols) + col / kBlockCols));
+    }
+}
 template <class T>
 __device__ __forceinline__ void read8(const Source& s, int64_t row, int col, int valid, Eight<T>& o) {
-    if (s.exps == nullptr) {
-        o.raw = load8<T>((const T*)s.p + row * s.ld + col, valid);
-    } else {
-        o.code = u32x2{0, 0};
-        o.exp = 0;
-        if (valid > 0) {   // rows are filled up to a multiple of 32 codes (of value zero)
-            o.code = *reinterpret_cast<const u32x2*>((const uint8_t*)s.p + row * s.ld + col);
-            o.exp = s.exps[row * (s.ld / kBlockCols) + col / kBlockCols];
-        }
-    }
+    if (s.exps == nullptr) o.raw = load8<T>((const T*)s.p + row * s.ld + col, valid);
+    else read_codes8(s, row, col, valid, o);
 }
 template <class T>
 __device__ __forceinline__ void values8(const Source& s, const Eight<T>& v, float (&f)[8]) {
@@ -397,10 +400,12 @@ __device__ __forceinline__ void store4(T* p, f32x4 v, int n) {
 // f'(y) of eight columns applied to f
 template <class T>
 __device__ __forceinline__ void masked8(const Source& s, const Eight<T>& v, float slope, float (&f)[8]) {
+    if (s.exps != nullptr) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const bool pos = s.exps == nullptr ? v.raw.get(e) > 0.f : !((v.code[e >> 2] >> (8 * (e & 3) + 7)) & 1);
-        f[e] = pos ? f[e] : f[e] * slope;
+        for (int e = 0; e < 8; ++e) f[e] *= slope_of(v.code[e >> 2], e & 3, slope);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = v.raw.get(e) > 0.f ? f[e] : f[e] * slope;
     }
 }
 
@@ -418,7 +423,9 @@ struct AdapterGradArgs {
     const float* v;            // [rows][rank], s included
     void *ddown, *dup;
     const void* up;            // [groups][N][rank], and ...
-    void* turned;              // ... [groups][rank][N]
+    void* turned;              // ... [groups][rank][ldp], zeros behind N
+    bf16_t* p;                 // dy f' as operand planes [planes][slots][ldp] in the plan's order, zeros behind N and in filling slots
+    int64_t ldp;
     float* parts;
     int K, N, rank;
     float scale, slope;
@@ -426,16 +433,19 @@ struct AdapterGradArgs {
     PlanShape ps;
 };
 
-// One wave: an item's rows and 128 columns.  WHOLE: all of them exist, so that the loads need no branch.
-template <class T, int RT, bool UP, bool WHOLE>
-__device__ __forceinline__ void adapter_grad_tile(const AdapterGradArgs& a, const int* it, int tile0) {
+// An item's rows, 4 H a step, and 128 columns: one wave (SPLIT = 1), or the workgroup's four, each with every fourth step (SPLIT = 4; their
+// sums are added in order).  WHOLE: all columns exist, so that the loads need no branch.
+template <class T, int RT, int H, int SPLIT, bool UP, bool WHOLE>
+__device__ __forceinline__ void adapter_grad_tile(const AdapterGradArgs& a, const int* it, int tile0, f32x4 (*red)[8][64]) {
     const int g = it[0], first = it[1], count = it[2], part = it[3];
     const int* slot_row = a.plan + a.ps.o_row;
-    const int lane = threadIdx.x & 63, l15 = lane & 15, quad = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, quad = lane >> 4;
     const int C = UP ? a.N : a.K, c0 = tile0 + 8 * l15, valid = WHOLE ? 8 : C - c0, r = a.rank;
     const float* small = UP ? a.low : a.v;
     const Source wide = UP ? Source{a.dy, nullptr, a.ldy} : a.x;
     const bool masked = UP && a.mask.p != nullptr;
+    const int begin = SPLIT > 1 ? 4 * H * wave : 0;
+    constexpr int STEP = 4 * H * SPLIT;
 
     f32x4 acc[RT][8];
 #pragma unroll
@@ -443,7 +453,6 @@ __device__ __forceinline__ void adapter_grad_tile(const AdapterGradArgs& a, cons
 #pragma unroll
         for (int e = 0; e < 8; ++e) acc[j][e] = f32x4{0, 0, 0, 0};
 
-    constexpr int H = 2;   // rows of a quad a step: 4 H rows
     Eight<T> w[H], m[H];
     float s[H][RT];
     auto row_of = [&](int i) { return i < count ? slot_row[first + i] : -1; };
@@ -459,11 +468,11 @@ __device__ __forceinline__ void adapter_grad_tile(const AdapterGradArgs& a, cons
     };
     int rid[H], nxt[H];
 #pragma unroll
-    for (int h = 0; h < H; ++h) rid[h] = row_of(quad + 4 * h);
+    for (int h = 0; h < H; ++h) rid[h] = row_of(begin + quad + 4 * h);
 #pragma unroll
-    for (int h = 0; h < H; ++h) nxt[h] = row_of(quad + 4 * (H + h));
+    for (int h = 0; h < H; ++h) nxt[h] = row_of(begin + STEP + quad + 4 * h);
     fetch(rid);
-    for (int i = 0; i < count; i += 4 * H) {
+    for (int i = begin; i < count; i += STEP) {
         float f[H][8], sc[H][RT];
 #pragma unroll
         for (int h = 0; h < H; ++h) {
@@ -475,10 +484,10 @@ __device__ __forceinline__ void adapter_grad_tile(const AdapterGradArgs& a, cons
             for (int j = 0; j < RT; ++j) sc[h][j] = rid[h] >= 0 && 16 * j + l15 < r ? s[h][j] : 0.f;
             rid[h] = nxt[h];
         }
-        if (i + 4 * H < count) {
+        if (i + STEP < count) {
             fetch(rid);
 #pragma unroll
-            for (int h = 0; h < H; ++h) nxt[h] = row_of(i + quad + 4 * (2 * H + h));
+            for (int h = 0; h < H; ++h) nxt[h] = row_of(i + 2 * STEP + quad + 4 * h);
         }
 #pragma unroll
         for (int h = 0; h < H; ++h)
@@ -486,6 +495,22 @@ __device__ __forceinline__ void adapter_grad_tile(const AdapterGradArgs& a, cons
             for (int j = 0; j < RT; ++j)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) acc[j][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(sc[h][j], f[h][e], acc[j][e], 0, 0, 0);
+    }
+    if constexpr (SPLIT > 1) {
+#pragma unroll
+        for (int j = 0; j < RT; ++j) {
+            if (j) __syncthreads();
+            if (wave > 0) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) red[wave - 1][e][lane] = acc[j][e];
+            }
+            __syncthreads();
+            if (wave == 0) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) acc[j][e] += red[0][e][lane] + red[1][e][lane] + red[2][e][lane];
+            }
+        }
+        if (wave > 0) return;
     }
     const int64_t pair = (int64_t)r * (a.K + a.N);
     float* po = part >= 0 ? a.parts + part * pair + (UP ? (int64_t)r * a.K : 0) : nullptr;
@@ -516,14 +541,6 @@ __device__ __forceinline__ void adapter_grad_tile(const AdapterGradArgs& a, cons
         }
     }
 }
-template <class T, int RT, bool UP>
-__device__ __forceinline__ void adapter_grad_wave(const AdapterGradArgs& a, int item, int tile) {
-    const int C = UP ? a.N : a.K;
-    if (item >= a.plan[kPlanItems] || 128 * tile >= C) return;
-    const int* it = a.plan + a.ps.o_item + 4 * (int64_t)item;
-    if (128 * tile + 128 <= C) adapter_grad_tile<T, RT, UP, true>(a, it, 128 * tile);
-    else adapter_grad_tile<T, RT, UP, false>(a, it, 128 * tile);
-}
 // up [N][rank] of an adapter that some row asks for -> [rank][N], the orientation that dy is contracted with: the projection reads
 // its inner operands 16 bytes at a time along the depth.  64 columns, all ranks.
 template <class T>
@@ -533,7 +550,7 @@ __device__ __forceinline__ void turn_up(const AdapterGradArgs& a, int item, int 
     if (it[2] == 0 || (item > 0 && it[-4] == it[0])) return;   // no rows; a later piece of the same group
     const int r = a.rank, pitch = r | 1, n = min(64, a.N - n0), tid = threadIdx.x;
     const T* src = (const T*)a.up + (int64_t)it[0] * a.N * r + (int64_t)n0 * r;   // n * rank neighbouring elements
-    T* out = (T*)a.turned + (int64_t)it[0] * a.N * r + n0;
+    T* out = (T*)a.turned + (int64_t)it[0] * a.ldp * r + n0;
     for (int i = 8 * tid; i < n * r; i += 8 * 256) {
         const Raw8<T> v = load8<T>(src + i, n * r - i);
         int c = i / r, j = i - c * r;
@@ -548,22 +565,74 @@ __device__ __forceinline__ void turn_up(const AdapterGradArgs& a, int item, int 
         const int j = i >> 3, c = 8 * (i & 7);
         float v[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = to_f<T>(tile[min(c + e, 63) * pitch + j]);
-        store8<T>(out + (int64_t)j * a.N + c, v, n - c);
+        for (int e = 0; e < 8; ++e) v[e] = c + e < n ? to_f<T>(tile[(c + e) * pitch + j]) : 0.f;
+        if (n0 + c < a.ldp) store8<T>(out + (int64_t)j * a.ldp + c, v, 8);   // (ldp is a multiple of 8)
     }
 }
-// before the projection's pass: the gradients of up (four tiles a workgroup), and up turned around (64 columns a workgroup)
-template <class T, int RT>
+// p = dy f'(y), cut into operand planes, in the plan's order.  (bf16: where the slope applies p is rounded once more, to 8 bits: 2^-8 of
+// terms that the slope made small; dup is computed from the unrounded ones.)
+template <class T>
+__device__ __forceinline__ void mask_and_order(const AdapterGradArgs& a, int64_t chunk0) {
+    const int per = (int)(a.ldp / 8);
+    const int slots = 16 * a.plan[kPlanSubs];
+    const Source dy = {a.dy, nullptr, a.ldy};
+    constexpr int Q = 4;   // pieces of eight columns a thread, requested together
+    int64_t slot[Q];
+    int col[Q], rid[Q];
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+        const int64_t i = chunk0 + threadIdx.x + 256 * q;
+        slot[q] = i / per;
+        col[q] = 8 * (int)(i - slot[q] * per);
+        rid[q] = a.plan[a.ps.o_row + min(slot[q], (int64_t)slots - 1)];
+    }
+    Eight<T> w[Q], m[Q];
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+        read8<T>(dy, max(rid[q], 0), col[q], a.N - col[q], w[q]);
+        if (a.mask.p != nullptr) read8<T>(a.mask, max(rid[q], 0), col[q], a.N - col[q], m[q]);
+    }
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+        if (slot[q] >= slots) continue;
+        float f[8];
+        values8<T>(dy, w[q], f);
+        if (a.mask.p != nullptr) masked8<T>(a.mask, m[q], a.slope, f);
+        Raw8<T> o;
+        o.zero();
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o.set(e, from_f<T>(rid[q] >= 0 ? f[e] : 0.f));
+        const Planes8<T> pl = to_planes(o);
+#pragma unroll
+        for (int p = 0; p < Elem<T>::planes; ++p)
+            *reinterpret_cast<s16x8*>(a.p + ((int64_t)p * a.ps.slots + slot[q]) * a.ldp + col[q]) = pl.p[p];
+    }
+}
+// before the projection's pass, two kinds of workgroups: up turned around (64 columns each), and p
+template <class T>
 __global__ __launch_bounds__(256) void adapter_first_kernel(AdapterGradArgs a) {
     __shared__ T tile[64 * (kMaxRank + 1)];
-    const int quads = (a.N + 511) / 512;
-    if ((int)blockIdx.y < quads) adapter_grad_wave<T, RT, true>(a, blockIdx.x, 4 * (int)blockIdx.y + ((int)threadIdx.x >> 6));
-    else turn_up<T>(a, blockIdx.x, 64 * ((int)blockIdx.y - quads), tile);
+    const int turns = (a.N + 63) / 64;
+    const int64_t b = blockIdx.x, turning = a.ps.items * turns;
+    if (b < turning) turn_up<T>(a, (int)(b / turns), 64 * (int)(b % turns), tile);
+    else mask_and_order<T>(a, (b - turning) * 1024);
 }
-// behind it: the gradients of down, which need v
-template <class T, int RT>
-__global__ __launch_bounds__(256) void adapter_last_kernel(AdapterGradArgs a) {
-    adapter_grad_wave<T, RT, false>(a, blockIdx.x, 4 * (int)blockIdx.y + ((int)threadIdx.x >> 6));
+// behind it (v): tiles of down, then tiles of up
+template <class T, int RT, int H, int SPLIT>
+__global__ __launch_bounds__(256) void adapter_grad_kernel(AdapterGradArgs a) {
+    __shared__ f32x4 red[SPLIT > 1 ? 3 : 1][SPLIT > 1 ? 8 : 1][64];
+    auto* const r = reinterpret_cast<f32x4(*)[8][64]>(red);
+    if ((int)blockIdx.x >= a.plan[kPlanItems]) return;
+    const int* it = a.plan + a.ps.o_item + 4 * (int64_t)blockIdx.x;
+    const int downs = (a.K + 127) / 128, ups = (a.N + 127) / 128;
+    int tile = SPLIT > 1 ? (int)blockIdx.y : 4 * (int)blockIdx.y + ((int)threadIdx.x >> 6);
+    if (tile < downs) {
+        if (128 * tile + 128 <= a.K) adapter_grad_tile<T, RT, H, SPLIT, false, true>(a, it, 128 * tile, r);
+        else adapter_grad_tile<T, RT, H, SPLIT, false, false>(a, it, 128 * tile, r);
+    } else if ((tile -= downs) < ups) {
+        if (128 * tile + 128 <= a.N) adapter_grad_tile<T, RT, H, SPLIT, true, true>(a, it, 128 * tile, r);
+        else adapter_grad_tile<T, RT, H, SPLIT, true, false>(a, it, 128 * tile, r);
+    }
 }
 template <class T>
 __global__ __launch_bounds__(256) void adapter_join_kernel(AdapterGradArgs a) {
@@ -706,46 +775,50 @@ __device__ __forceinline__ void weight_grad_tile(const WeightGradArgs& a, int n0
 
     // pieces of eight columns: thread t has column piece t % 16 of rows t / 16 and t / 16 + 32
     const int pc = tid & 15, pr = tid >> 4;
-    struct Ahead { Eight<T> pw[2], mw[2], xw[2]; } ahead[2];   // two tiles on their way
+    struct Codes { u32x2 code; unsigned exp; };
+    struct Ahead { Eight<T> pw[2], mw[2]; Codes xw[2]; } ahead[2];   // two tiles on their way
     auto fetch = [&](int64_t row0, Ahead& t) {
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
             const int64_t at = min(row0 + pr + 32 * q, hi - 1);   // (behind the last row: read again, and set to zero in keep)
             read8<T>(dy, at, n0 + 8 * pc, WHOLE ? 8 : a.N - n0 - 8 * pc, t.pw[q]);
             if (masked) read8<T>(a.mask, at, n0 + 8 * pc, WHOLE ? 8 : a.N - n0 - 8 * pc, t.mw[q]);
-            read8<T>(a.x, at, k0 + 8 * pc, WHOLE ? 8 : a.K - k0 - 8 * pc, t.xw[q]);
+            read_codes8(a.x, at, k0 + 8 * pc, WHOLE ? 8 : a.K - k0 - 8 * pc, t.xw[q]);
         }
     };
+    const bool sums = k0 == 0;   // these workgroups add up p as well
     float bsum[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) bsum[e] = 0.f;
-    auto keep = [&](unsigned char* buf, int64_t row0, const Ahead& t) {
+    auto keep = [&](unsigned char* buf, int64_t row0, Ahead& t) {
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
             const int row = pr + 32 * q, at = row * 256 + (((pc >> 1) ^ tr_swz(row)) * 32 + (pc & 1) * 16);
-            const bool in = row0 + row < hi;
-            float f[8];
-            values8<T>(dy, t.pw[q], f);
-            if (masked) masked8<T>(a.mask, t.mw[q], a.slope, f);
-            Raw8<T> o;
-            o.zero();
+            if (row0 + row >= hi) {
+                t.pw[q].raw.zero();
+                t.xw[q].code = u32x2{0, 0};
+            }
+            Raw8<T> o = t.pw[q].raw;
+            if (masked || sums) {
+                float f[8];
+                values8<T>(dy, t.pw[q], f);
+                if (masked) {
+                    masked8<T>(a.mask, t.mw[q], a.slope, f);
+                    o.zero();
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                f[e] = in ? f[e] : 0.f;
-                bsum[e] += f[e];
-                o.set(e, from_f<T>(f[e]));
+                    for (int e = 0; e < 8; ++e) o.set(e, from_f<T>(f[e]));
+                }
+                if (sums) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) bsum[e] += f[e];
+                }
             }
             const Planes8<T> pl = to_planes(o);
 #pragma unroll
             for (int p = 0; p < P; ++p) *reinterpret_cast<s16x8*>(buf + p * TB + at) = pl.p[p];
-            values8<T>(a.x, t.xw[q], f);
-            u32x4 xv;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const unsigned both = (__float_as_uint(f[2 * e]) >> 16) | (__float_as_uint(f[2 * e + 1]) & 0xffff0000u);   // exact
-                xv[e] = in ? both : 0u;
-            }
-            *reinterpret_cast<u32x4*>(buf + P * TB + at) = xv;
+            const float scale = __uint_as_float(t.xw[q].exp << 23);
+            const u32x2 x0 = decode4_bf16(t.xw[q].code[0], scale), x1 = decode4_bf16(t.xw[q].code[1], scale);
+            *reinterpret_cast<u32x4*>(buf + P * TB + at) = u32x4{x0[0], x0[1], x1[0], x1[1]};
         }
     };
     f32x4 acc[4][4];
@@ -842,7 +915,7 @@ __device__ __forceinline__ void weight_grad_tile(const WeightGradArgs& a, int n0
             }
         }
     }
-    if (k0 == 0) {
+    if (sums) {
         __syncthreads();
         float* s = reinterpret_cast<float*>(smem);   // [32 rows][128]
 #pragma unroll
@@ -932,31 +1005,47 @@ static void few_rank(const FewArgs& a, hipStream_t s) {
     else if (a.rank <= 32) launch_few<T, 2>(a, s);
     else launch_few<T, 4>(a, s);
 }
-template <class T, int RT>
+template <class T>
 static void adapter_first(const AdapterGradArgs& a, hipStream_t s) {
-    adapter_first_kernel<T, RT><<<dim3((unsigned)a.ps.items, (unsigned)(ceil_div(a.N, 512) + ceil_div(a.N, 64))), 256, 0, s>>>(a);
+    const int64_t blocks = a.ps.items * ceil_div(a.N, 64) + ceil_div(a.ps.slots * (a.ldp / 8), 1024);
+    VH_REQUIRE(blocks < (int64_t(1) << 31), "too many rows for one launch");
+    adapter_first_kernel<T><<<(unsigned)blocks, 256, 0, s>>>(a);
     VH_HIP(hipGetLastError());
 }
 template <class T, int RT>
-static void adapter_last(const AdapterGradArgs& a, hipStream_t s) {
-    adapter_last_kernel<T, RT><<<dim3((unsigned)a.ps.items, (unsigned)ceil_div(a.K, 512)), 256, 0, s>>>(a);
+static void adapter_grads_rank(const AdapterGradArgs& a, hipStream_t s) {
+    // Few waves (up to 4096: a quarter of what the chip holds): the workgroup's four share a tile's rows, so that a group's rows are four
+    // round trips fewer.  Many: a wave a tile, nothing to add up.  (200 groups, 8192 rows, K = N = 512: 20 us against 28)
+    const int64_t tiles = ceil_div(a.K, 128) + ceil_div(a.N, 128);
+    if (a.ps.items * tiles < 4096) adapter_grad_kernel<T, RT, 2, 4><<<dim3((unsigned)a.ps.items, (unsigned)tiles), 256, 0, s>>>(a);
+    else adapter_grad_kernel<T, RT, 2, 1><<<dim3((unsigned)a.ps.items, (unsigned)ceil_div(tiles, 4)), 256, 0, s>>>(a);
     VH_HIP(hipGetLastError());
+}
+template <class T>
+static void adapter_grads(const AdapterGradArgs& a, hipStream_t s) {
+    if (a.rank <= 16) adapter_grads_rank<T, 1>(a, s);
+    else if (a.rank <= 32) adapter_grads_rank<T, 2>(a, s);
+    else adapter_grads_rank<T, 4>(a, s);
     if (a.ps.rows > a.ps.item_rows) {
         const int64_t multis = a.ps.rows / a.ps.item_rows < a.ps.groups ? a.ps.rows / a.ps.item_rows : a.ps.groups;
         adapter_join_kernel<T><<<dim3((unsigned)multis, (unsigned)ceil_div((int64_t)a.rank * (a.K + a.N), 256)), 256, 0, s>>>(a);
         VH_HIP(hipGetLastError());
     }
 }
-template <class T>
-static void adapter_grads(const AdapterGradArgs& a, bool last, hipStream_t s) {
-    if (a.rank <= 16) last ? adapter_last<T, 1>(a, s) : adapter_first<T, 1>(a, s);
-    else if (a.rank <= 32) last ? adapter_last<T, 2>(a, s) : adapter_first<T, 2>(a, s);
-    else last ? adapter_last<T, 4>(a, s) : adapter_first<T, 4>(a, s);
+// the backward pass's scratch, in words: v, up turned around, p, the parts of groups of several items
+struct BackwardScratch {
+    int64_t ldp, turned, p, parts, words;
+};
+static BackwardScratch backward_scratch(const PlanShape& ps, int64_t n, int64_t k, int64_t rank, int dtype) {
+    BackwardScratch b{};
+    const int64_t es = dtype == VH_BF16 ? 2 : 4, planes = dtype == VH_BF16 ? 1 : 3;
+    b.ldp = round_up(n, 8);
+    b.turned = round_up(ps.rows * rank, 4);
+    b.p = b.turned + round_up(ps.groups * rank * b.ldp * es / 4, 4);
+    b.parts = b.p + round_up(planes * ps.slots * b.ldp / 2, 4);
+    b.words = b.parts + (ps.rows > ps.item_rows ? 2 * (ps.rows / ps.item_rows) * rank * (n + k) : 0);
+    return b;
 }
-static int64_t turned_words(int64_t groups, int64_t n, int64_t rank, int dtype) {
-    return round_up(dtype == VH_BF16 ? ceil_div(groups * n * rank, 2) : groups * n * rank, 4);
-}
-static int64_t grad_parts(const PlanShape& ps) { return ps.rows > ps.item_rows ? 2 * (ps.rows / ps.item_rows) : 0; }
 
 }  // namespace adapt
 }  // namespace vh
@@ -1067,6 +1156,7 @@ int vh_adapt_forward(const vh_adapt_layer* l, const void* x, int64_t ldx, int64_
         a.ldw = (int)ws.kq;
         a.bias = reinterpret_cast<const float*>((const char*)l->packed + ws.bias_off);
         a.inner = l->down;
+        a.ld_inner = l->k;
         a.outer = l->up;
         a.K = (int)l->k;
         a.N = (int)l->n;
@@ -1132,9 +1222,8 @@ int vh_adapt_backward_size(int64_t rows, int64_t groups, int64_t n, int64_t k, i
         check_width(k, "k");
         check_rank(rank);
         check_ptr(scratch_words, "scratch_words");
-        const PlanShape ps = plan_shape(rows, groups);
         check_dtype(dtype);
-        *scratch_words = round_up(rows * rank, 4) + turned_words(groups, n, rank, dtype) + grad_parts(ps) * rank * (n + k);
+        *scratch_words = backward_scratch(plan_shape(rows, groups), n, k, rank, dtype).words;
     });
 }
 
@@ -1168,9 +1257,11 @@ int vh_adapt_backward(const vh_adapt_layer* l, const void* dy, int64_t lddy, con
         g.ddown = ddown;
         g.dup = dup;
         g.up = l->up;
-        float* turned = scratch + round_up(rows * l->rank, 4);
-        g.turned = turned;
-        g.parts = turned + turned_words(l->groups, l->n, l->rank, l->dtype);
+        const BackwardScratch bs = backward_scratch(ps, l->n, l->k, l->rank, l->dtype);
+        g.turned = scratch + bs.turned;
+        g.p = reinterpret_cast<bf16_t*>(scratch + bs.p);
+        g.ldp = bs.ldp;
+        g.parts = scratch + bs.parts;
         g.K = (int)l->k;
         g.N = (int)l->n;
         g.rank = (int)l->rank;
@@ -1180,16 +1271,13 @@ int vh_adapt_backward(const vh_adapt_layer* l, const void* dy, int64_t lddy, con
         g.ps = ps;
         const WeightShape ws = weight_shape(l->n, l->k, l->dtype);
         LinArgs a{};
-        a.x = dy;
-        a.ldx = lddy;
-        a.mask = mask.p;
-        a.ldm = mask.ld;
-        a.mask_codes = mask.exps != nullptr;
-        a.slope = l->negative_slope;
+        a.x = g.p;
+        a.ldx = bs.ldp;
         a.w = (const bf16_t*)l->packed + ws.planes * ws.fwd;
         a.w_plane = ws.bwd;
         a.ldw = (int)ws.nq;
-        a.inner = turned;
+        a.inner = g.turned;
+        a.ld_inner = bs.ldp;
         a.outer = l->down;
         a.K = (int)l->n;
         a.N = (int)l->k;
@@ -1201,13 +1289,13 @@ int vh_adapt_backward(const vh_adapt_layer* l, const void* dy, int64_t lddy, con
         a.plan = plan;
         a.ps = ps;
         if (l->dtype == VH_BF16) {
-            adapter_grads<bf16_t>(g, false, s);
+            adapter_first<bf16_t>(g, s);
             launch_linear_bf16(a, true, s);
-            adapter_grads<bf16_t>(g, true, s);
+            adapter_grads<bf16_t>(g, s);
         } else {
-            adapter_grads<float>(g, false, s);
+            adapter_first<float>(g, s);
             launch_linear_f32(a, true, s);
-            adapter_grads<float>(g, true, s);
+            adapter_grads<float>(g, s);
         }
     });
 }

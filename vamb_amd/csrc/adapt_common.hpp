@@ -171,12 +171,21 @@ __device__ __forceinline__ unsigned encode4(float x0, float x1, float x2, float 
     }
     return ((unsigned)w & 0x7f7f7f7fu) | s | n;
 }
-__device__ __forceinline__ void decode4(unsigned codes, float scale, float (&o)[4]) {
-    const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, true);
-    o[0] = a[0] * scale;
-    o[1] = a[1] * scale;
-    o[2] = b[0] * scale;
-    o[3] = b[1] * scale;
+__device__ __forceinline__ void decode4(unsigned codes, float scale, float (&o)[4]) {   // (the conversion takes the power of two)
+    const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(codes, scale, false), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(codes, scale, true);
+    o[0] = a[0];
+    o[1] = a[1];
+    o[2] = b[0];
+    o[3] = b[1];
+}
+__device__ __forceinline__ u32x2 decode4_bf16(unsigned codes, float scale) {   // exact
+    return u32x2{__builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, false)),
+                 __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, true))};
+}
+// f' of element e from its code: 1, or the slope where the sign bit is set
+__device__ __forceinline__ float slope_of(unsigned codes, int e, float slope) {
+    const unsigned s = (unsigned)__builtin_amdgcn_sbfe((int)codes, 8 * e + 7, 1);
+    return __uint_as_float((s & __float_as_uint(slope)) | (~s & 0x3f800000u));
 }
 
 // ---- the row plan -----------------------------------------------------------------------------------------------------------
@@ -197,7 +206,8 @@ inline PlanShape plan_shape(int64_t rows, int64_t groups) {
     s.subs = rows / 16 + runs;
     s.slots = 16 * s.subs;
     int64_t ir = (rows / 512 + 15) / 16 * 16;
-    s.item_rows = ir < 128 ? 128 : ir;
+    const int64_t least = groups < 128 ? 128 : 512;   // (few groups: more pieces, many: fewer parts to join)
+    s.item_rows = ir < least ? least : ir;
     s.items = groups + rows / s.item_rows;
     s.multis = rows / s.item_rows + 1;
     s.o_row = 16;
@@ -211,19 +221,17 @@ enum { kPlanSubs = 0, kPlanItems = 1, kPlanMultis = 2, kPlanParts = 3 };
 
 // ---- arguments of the shared-projection kernel (adapt_linear.hpp) -----------------------------------------------------------------
 struct LinArgs {
-    const void* x;            // [rows][ldx]: the layer's input, or dy
+    const void* x;            // forward: the layer's input [rows][ldx]; backward: p = dy f' as operand planes [planes][slots][ldx], in the plan's order
     int64_t ldx;
-    const void* mask;         // backward: the layer's output whose sign selects f' (nullptr: f' = 1) ...
-    int64_t ldm;              // ... its row stride in elements / bytes
-    int mask_codes;           // ... as checkpoint codes
     float slope;
     int activation;           // forward: LeakyReLU(slope) on the result
     const bf16_t* w;          // packed operand [planes][.][ldw]
     int64_t w_plane;          // elements of a plane
     int ldw;
-    const float* bias;        // padded, or nullptr
-    const void* inner;        // adapters contracted with x (forward: down, backward: up)
-    const void* outer;        // adapters of the result (forward: up, backward: down)
+    const float* bias;        // padded (forward)
+    const void* inner;        // adapters contracted with x: [groups][rank][ld_inner] (forward: down, backward: up turned around)
+    int64_t ld_inner;
+    const void* outer;        // adapters of the result (forward: up [groups][N][rank], backward: down [groups][rank][N])
     int K, N, rank;
     float scale, low_scale;   // on the expanded part; on `low` as it is written
     float* low;               // [rows][rank] or nullptr
@@ -234,7 +242,7 @@ struct LinArgs {
     uint8_t* exps;            // row stride ldc / 32
     const int* plan;
     PlanShape ps;
-    int dma;                  // x rows are 16-byte aligned, K is a multiple of 8 and x ends below 2^32 - 16 bytes: ...
+    int dma;                  // forward: x rows are 16-byte aligned, K is a multiple of 8 and x ends below 2^32 - 16 bytes: ...
     unsigned x_bytes;         // ... its size, as a buffer
 };
 void launch_linear_bf16(const LinArgs& a, bool backward, hipStream_t s);

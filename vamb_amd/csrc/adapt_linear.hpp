@@ -10,8 +10,8 @@
 // lane ends with four consecutive columns of one row, and u's accumulator layout (lane: row l & 15, ranks 4 (l >> 4) + i) IS the
 // operand layout of the 16-deep product with B_g, which therefore follows without leaving the registers.
 //   u is cut into planes there (two for bf16 tensors: 16 bits, three for float32), never rounded to 8 bits.
-// x reaches the LDS by DMA where its rows are 16-byte aligned, else through registers (any alignment, any row stride; the backward's mask
-// is applied there).  LDS rows are 128 B (64 B with three planes); 16-byte pieces are XOR-permuted by the row so that
+// x reaches the LDS by DMA where its rows are 16-byte aligned bf16, else through registers (any alignment, any row stride; float32 is cut
+// into planes there).  The backward pass's p has been cut, masked and brought into the plan's order before (adapt.hip): DMA always.  LDS rows are 128 B (64 B with three planes); 16-byte pieces are XOR-permuted by the row so that
 // the 16 rows of an operand read fall into 16 different bank groups.
 #pragma once
 
@@ -103,7 +103,7 @@ __global__ __launch_bounds__(64 * S::WM * S::WN * S::KG) void linear_kernel(LinA
     constexpr int QW = NWI ? (NWI + NW - 1) / NW : 1;
     constexpr int KC = BK / 32;                         // 32-deep products per tile
     constexpr int MU = MS / WN;                         // subtiles whose u this wave computes (its share of the WN waves on the same rows)
-    static_assert(PX >= 1 && BM * CH % THREADS == 0 && MS % WN == 0 && (!DMA || P == 1), "tile shape");
+    static_assert(PX >= 1 && BM * CH % THREADS == 0 && MS % WN == 0 && (!DMA || TRANS || P == 1) && (!TRANS || DMA), "tile shape");
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
 
     static_assert(KG == 1 || (WN == 1 && MS == 1), "groups along the depth have narrow waves");
@@ -128,12 +128,21 @@ __global__ __launch_bounds__(64 * S::WM * S::WN * S::KG) void linear_kernel(LinA
 
     // ---- x pieces of this thread
     const T* x_src[PX];
-    const char* m_src[PX];
     int x_k[PX], rids[PX];
     unsigned x_off[PX];
-    const Buffer x_buf = buffer_of(a.x, a.x_bytes);
+    Buffer x_buf[P];
 #pragma unroll
-    for (int q = 0; q < PX; ++q) {
+    for (int p = 0; p < P; ++p) {
+        if constexpr (TRANS) {
+            // the tile's slots follow each other: its own buffer per plane (BM * 2^20 * 2 bytes at most), which ends with the slots
+            const int64_t at = (int64_t)tile * BM, left = (a.ps.slots - at) * a.ldx * 2;
+            x_buf[p] = buffer_of((const bf16_t*)a.x + ((int64_t)p * a.ps.slots + at) * a.ldx, left > 0 ? (unsigned)min(left, (int64_t)kBehind) : 0u);
+        } else {
+            x_buf[p] = buffer_of(a.x, a.x_bytes);
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < PX && !TRANS; ++q) {
         const int slot = tile * BM + (tid + THREADS * q) / CH;
         rids[q] = slot < (int)a.ps.slots ? slot_row[slot] : -1;   // (slots behind the last run hold anything: n_sub decides below)
     }
@@ -156,11 +165,14 @@ __global__ __launch_bounds__(64 * S::WM * S::WN * S::KG) void linear_kernel(LinA
 #pragma unroll
     for (int q = 0; q < PX; ++q) {
         const int idx = tid + THREADS * q, row = idx / CH, slot = tile * BM + row;
-        const int rid = max(slot < 16 * n_sub ? rids[q] : -1, 0);   // a filling slot takes row 0's values; its results are dropped
         x_k[q] = 8 * ((idx % CH) ^ swz(row));
-        x_src[q] = (const T*)a.x + (int64_t)rid * a.ldx;
-        x_off[q] = (unsigned)(rid * a.ldx * (int64_t)sizeof(T));   // (DMA: all of x lies below kBehind)
-        m_src[q] = a.mask ? (const char*)a.mask + (int64_t)rid * a.ldm * (a.mask_codes ? 1 : (int)sizeof(T)) : nullptr;
+        if constexpr (TRANS) {
+            x_off[q] = (unsigned)(row * (int)a.ldx * 2);
+        } else {
+            const int rid = max(slot < 16 * n_sub ? rids[q] : -1, 0);   // a filling slot takes row 0's values; its results are dropped
+            x_src[q] = (const T*)a.x + (int64_t)rid * a.ldx;
+            x_off[q] = (unsigned)(rid * a.ldx * (int64_t)sizeof(T));   // (DMA: all of x lies below kBehind)
+        }
     }
 #pragma unroll
     for (int m = 0; m < MU; ++m) {
@@ -168,62 +180,30 @@ __global__ __launch_bounds__(64 * S::WM * S::WN * S::KG) void linear_kernel(LinA
         grp[m] = __builtin_amdgcn_readfirstlane(sub < n_sub ? grp[m] : -1);
     }
 
-    Raw8<T> x_raw[PX], y_raw[PX];
-    u32x2 c_raw[PX];
+    Raw8<T> x_raw[PX];
     // WHOLE: the tile lies within K (no branch: a wait behind one would drain every load in flight)
     auto fetch_x = [&](auto whole, int k0, unsigned char* buf) {
         if constexpr (DMA) {
 #pragma unroll
-            for (int q = 0; q < PX; ++q) {
-                const int k = k0 + x_k[q];
-                dma16(x_buf, k < K ? x_off[q] + 2 * k : kBehind, buf + (wave + NW * q) * 1024);
-            }
+            for (int p = 0; p < P; ++p)
+#pragma unroll
+                for (int q = 0; q < PX; ++q) {
+                    const int k = k0 + x_k[q];
+                    dma16(x_buf[p], k < K ? x_off[q] + 2 * k : kBehind, buf + p * XB + (wave + NW * q) * 1024);
+                }
         } else if constexpr (decltype(whole)::value) {
 #pragma unroll
             for (int q = 0; q < PX; ++q) x_raw[q].load(x_src[q] + k0 + x_k[q]);
-            if (TRANS && a.mask) {
-                if (a.mask_codes) {
-#pragma unroll
-                    for (int q = 0; q < PX; ++q) c_raw[q] = *(VH_GLOBAL(u32x2, m_src[q] + k0 + x_k[q]));
-                } else {
-#pragma unroll
-                    for (int q = 0; q < PX; ++q) y_raw[q].load((const T*)m_src[q] + k0 + x_k[q]);
-                }
-            }
         } else {
 #pragma unroll
-            for (int q = 0; q < PX; ++q) {
-                const int k = k0 + x_k[q];
-                x_raw[q] = load8<T>(x_src[q] + k, K - k);
-                if (TRANS && a.mask) {
-                    if (a.mask_codes) {
-                        c_raw[q] = u32x2{0, 0};
-                        if (k < K) c_raw[q] = *(VH_GLOBAL(u32x2, m_src[q] + k));
-                    } else {
-                        y_raw[q] = load8<T>((const T*)m_src[q] + k, K - k);
-                    }
-                }
-            }
+            for (int q = 0; q < PX; ++q) x_raw[q] = load8<T>(x_src[q] + k0 + x_k[q], K - k0 - x_k[q]);
         }
     };
     auto keep_x = [&](unsigned char* buf) {
         if constexpr (!DMA) {
 #pragma unroll
             for (int q = 0; q < PX; ++q) {
-                Raw8<T> v = x_raw[q];
-                if (TRANS && a.mask) {
-                    Raw8<T> o;
-                    o.zero();
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const bool pos = a.mask_codes ? !((c_raw[q][e >> 2] >> (8 * (e & 3) + 7)) & 1) : y_raw[q].get(e) > 0.f;
-                        const float d = v.get(e);
-                        // (bf16: the masked elements are rounded once more, to 8 bits: 2^-8 of terms that the slope made small)
-                        o.set(e, from_f<T>(pos ? d : d * a.slope));
-                    }
-                    v = o;
-                }
-                const Planes8<T> pl = to_planes(v);
+                const Planes8<T> pl = to_planes(x_raw[q]);
 #pragma unroll
                 for (int p = 0; p < P; ++p) *reinterpret_cast<s16x8*>(buf + p * XB + (tid + THREADS * q) * 16) = pl.p[p];
             }
@@ -251,7 +231,7 @@ __global__ __launch_bounds__(64 * S::WM * S::WN * S::KG) void linear_kernel(LinA
     for (int m = 0; m < MU; ++m)
 #pragma unroll
         for (int j = 0; j < RT; ++j)
-            in_src[m][j] = grp[m] >= 0 && 16 * j + l15 < r ? (const T*)a.inner + ((int64_t)grp[m] * r + 16 * j + l15) * K : nullptr;
+            in_src[m][j] = grp[m] >= 0 && 16 * j + l15 < r ? (const T*)a.inner + ((int64_t)grp[m] * r + 16 * j + l15) * a.ld_inner : nullptr;
     auto fetch_in = [&](auto whole, int k0, Raw8<T> (&in)[MU][KC][RT]) {
         if constexpr (DMA || decltype(whole)::value) {
 #pragma unroll

@@ -4,7 +4,7 @@
 namespace vh {
 namespace adapt {
 void launch_linear_bf16(const LinArgs& a, bool backward, hipStream_t s) {
-    if (backward) launch_rank<bf16_t, true, false>(a, s);
+    if (backward) launch_rank<bf16_t, true, true>(a, s);
     else if (a.dma) launch_rank<bf16_t, false, true>(a, s);
     else launch_rank<bf16_t, false, false>(a, s);
 }

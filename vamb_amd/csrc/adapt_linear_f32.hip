@@ -4,7 +4,7 @@
 namespace vh {
 namespace adapt {
 void launch_linear_f32(const LinArgs& a, bool backward, hipStream_t s) {
-    if (backward) launch_rank<float, true, false>(a, s);
+    if (backward) launch_rank<float, true, true>(a, s);
     else launch_rank<float, false, false>(a, s);
 }
 }  // namespace adapt
