@@ -130,7 +130,7 @@ def backward_bounds(c, x, y, u, dtype, slope):
     # p rounded to bf16 where the slope was applied: at most 2^-8 of its magnitude in every product that has it
     p = 2.0 ** -8 if dtype == torch.bfloat16 and slope is not None else 0.0
     cut = 2.0 ** -15 if dtype == torch.bfloat16 else 0.0
-    rel = {"dx": (2 * n + rank + 16) * F32 + 2.0 ** -21 + cut + p, "ddown": (n + rows + 16) * F32 + 2.0 ** -21 + p, "dup": (rows + 16) * F32,
+    rel = {"dx": (2 * n + rank + 16) * F32 + 2.0 ** -21 + cut + p, "ddown": (n + rows + 16) * F32 + 2.0 ** -21 + p, "dup": (rows + 16) * F32 + p,
            "dw": (rows + 16) * F32 + 2.0 ** -21 + p, "db": (rows + 16) * F32}
     out = {}
     for name, v, m in zip(("dx", "ddown", "dup", "dw", "db"), want, mag):

@@ -47,9 +47,10 @@ __device__ __forceinline__ int3 block_scan3(int3 v, int3* total, int* lds /* 3 *
     return int3{base.x + s.x - v.x, base.y + s.y - v.y, base.z + s.z - v.z};
 }
 
-// One workgroup of 1024: rows per group `count(g)` -> run starts (handed to `start(g, first slot)`), filling slots, items, multis, header.
+// One workgroup of 1024: rows per group `count(g)` -> run starts (handed to `start(g, first slot)`); `write`: filling slots, items, multis,
+// header.
 template <class Count, class Start>
-__device__ __forceinline__ void plan_offsets(int* plan, const PlanShape& ps, int* lds, Count count, Start start) {
+__device__ __forceinline__ void plan_offsets(int* plan, const PlanShape& ps, int* lds, bool write, Count count, Start start) {
     const int G = (int)ps.groups, ir = (int)ps.item_rows;
     int slot0 = 0, item0 = 0, multi0 = 0, part0 = 0;
     for (int base = 0; base <= G; base += 1024) {
@@ -64,6 +65,9 @@ __device__ __forceinline__ void plan_offsets(int* plan, const PlanShape& ps, int
         if (g <= G) {
             const int first = slot0 + at.x;
             start(g, first);
+        }
+        if (g <= G && write) {
+            const int first = slot0 + at.x;
             for (int i = m; i < filled; ++i) plan[ps.o_row + first + i] = -1;
             const int part = part0 + (at.z >> 16);
             for (int i = 0; i < pieces; ++i) {
@@ -85,7 +89,7 @@ __device__ __forceinline__ void plan_offsets(int* plan, const PlanShape& ps, int
         multi0 += total.z & 0xffff;
         part0 += total.z >> 16;
     }
-    if (threadIdx.x == 0) {
+    if (threadIdx.x == 0 && write) {
         plan[kPlanSubs] = slot0 / 16;
         plan[kPlanItems] = item0;
         plan[kPlanMultis] = multi0;
@@ -152,27 +156,45 @@ __device__ __forceinline__ void count_rows(const int* groups, int64_t lo, int64_
     }
 }
 
-constexpr int kSmallRows = 1024 * PB, kSmallCounters = 16 * 1024;   // one workgroup: 16 waves' counters in 64 KB
+constexpr int kSmallRows = 16384, kSmallCounters = 12 * 1024;   // 48 KB of counters
 
+// Up to 16384 rows, one launch: every workgroup counts ALL rows (their keys come from the L2) and finds the runs' starts for itself, and then
+// places its own 1024 rows, 64 a wave.  (One workgroup for all of 8192 rows took 10 us: eight batches of ballots a wave.)
 __global__ __launch_bounds__(1024) void plan_small_kernel(const int* groups, int* plan, PlanShape ps, int bits) {
-    extern __shared__ int counters[];   // [16][G + 1]
+    extern __shared__ int counters[];   // [16][G + 1] of this workgroup's waves, [G + 1] of the rows before it, [G + 1] of all
     __shared__ int lds[48];
-    const int G = (int)ps.groups, wave = threadIdx.x >> 6;
-    // at most PB keys a lane: they stay in registers
-    const int64_t seg = (ps.rows + 1023) / 1024 * 64, lo = min(wave * seg, ps.rows), hi = min(lo + seg, ps.rows);
-    int key[PB];
-    if (lo < hi) load_keys(groups, lo, hi, G, key);
-    for (int i = threadIdx.x; i < 16 * (G + 1); i += 1024) counters[i] = 0;
+    const int G = (int)ps.groups, wave = threadIdx.x >> 6, rows = (int)ps.rows, mine = 1024 * (int)blockIdx.x;
+    int* const before = counters + 16 * (G + 1);
+    int* const all = before + G + 1;
+    for (int i = threadIdx.x; i < 18 * (G + 1); i += 1024) counters[i] = 0;
     __syncthreads();
-    if (lo < hi) count_keys(key, G, counters + wave * (G + 1));
+    int own = G + 1;   // this thread's row of this workgroup
+    for (int row0 = 0; row0 < rows; row0 += 1024 * PB) {
+        int key[PB];
+#pragma unroll
+        for (int b = 0; b < PB; ++b) key[b] = groups[min(row0 + 1024 * b + (int)threadIdx.x, rows - 1)];
+#pragma unroll
+        for (int b = 0; b < PB; ++b) {
+            const int first = row0 + 1024 * b, row = first + (int)threadIdx.x;
+            if (first >= rows) break;
+            const int k = row < rows ? ((unsigned)key[b] < (unsigned)G ? key[b] : G) : G + 1;   // G + 1: no row
+            int* const also = first < mine ? before : counters + wave * (G + 1);
+            if (all_equal(k)) {   // (sorted rows: 64 additions to one address would be done one by one)
+                if ((threadIdx.x & 63) == 0 && k <= G) {
+                    atomicAdd(&all[k], 64);
+                    if (first <= mine) atomicAdd(&also[k], 64);
+                }
+            } else if (k <= G) {
+                atomicAdd(&all[k], 1);
+                if (first <= mine) atomicAdd(&also[k], 1);
+            }
+            if (first == mine) own = k;
+        }
+    }
     __syncthreads();
-    plan_offsets(plan, ps, lds,
-                 [&](int g) {
-                     int m = 0;
-                     for (int w = 0; w < 16; ++w) m += counters[w * (G + 1) + g];
-                     return m;
-                 },
+    plan_offsets(plan, ps, lds, blockIdx.x == 0, [&](int g) { return all[g]; },
                  [&](int g, int first) {
+                     first += before[g];
                      for (int w = 0; w < 16; ++w) {
                          const int c = counters[w * (G + 1) + g];
                          counters[w * (G + 1) + g] = first;
@@ -180,7 +202,12 @@ __global__ __launch_bounds__(1024) void plan_small_kernel(const int* groups, int
                      }
                  });
     __syncthreads();
-    if (lo < hi) place_keys(key, lo, hi, G, bits, counters + wave * (G + 1), plan, ps);
+    const unsigned long long same = all_equal(own) ? ~0ull : same_key(own, bits);
+    if (own <= G) {
+        const int slot = counters[wave * (G + 1) + own] + __popcll(same & ((1ull << (threadIdx.x & 63)) - 1));
+        plan[ps.o_row + slot] = mine + (int)threadIdx.x;
+        if ((slot & 15) == 0) plan[ps.o_sub + slot / 16] = own < G ? own : -1;
+    }
 }
 
 // Larger: one wave per piece of rows; counts [G + 1][pieces], then run totals [G + 1] behind them
@@ -213,7 +240,7 @@ __global__ __launch_bounds__(64) void plan_scan_kernel(int* scratch, int G, int 
 }
 __global__ __launch_bounds__(1024) void plan_offsets_kernel(int* plan, int* totals, PlanShape ps) {
     __shared__ int lds[48];
-    plan_offsets(plan, ps, lds, [&](int g) { return totals[g]; }, [&](int g, int first) { totals[g] = first; });
+    plan_offsets(plan, ps, lds, true, [&](int g) { return totals[g]; }, [&](int g, int first) { totals[g] = first; });
 }
 __global__ __launch_bounds__(64) void plan_place_kernel(const int* groups, const int* scratch, int* plan, PlanShape ps, int64_t seg, int pieces, int bits) {
     extern __shared__ int counters[];
@@ -224,7 +251,7 @@ __global__ __launch_bounds__(64) void plan_place_kernel(const int* groups, const
     place_rows(groups, lo, hi, G, bits, counters, plan, ps);
 }
 
-static bool plan_is_small(int64_t rows, int64_t groups) { return rows <= kSmallRows && 16 * (groups + 1) <= kSmallCounters; }
+static bool plan_is_small(int64_t rows, int64_t groups) { return rows <= kSmallRows && 18 * (groups + 1) <= kSmallCounters; }
 static int64_t plan_pieces(int64_t rows) { return rows < 512 ? 1 : (rows / 512 < 1024 ? rows / 512 : 1024); }
 
 // =====================================================================================================================
@@ -442,8 +469,7 @@ __device__ __forceinline__ void adapter_grad_tile(const AdapterGradArgs& a, cons
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, quad = lane >> 4;
     const int C = UP ? a.N : a.K, c0 = tile0 + 8 * l15, valid = WHOLE ? 8 : C - c0, r = a.rank;
     const float* small = UP ? a.low : a.v;
-    const Source wide = UP ? Source{a.dy, nullptr, a.ldy} : a.x;
-    const bool masked = UP && a.mask.p != nullptr;
+    constexpr int PW = UP ? Elem<T>::planes : 1;
     const int begin = SPLIT > 1 ? 4 * H * wave : 0;
     constexpr int STEP = 4 * H * SPLIT;
 
@@ -453,15 +479,22 @@ __device__ __forceinline__ void adapter_grad_tile(const AdapterGradArgs& a, cons
 #pragma unroll
         for (int e = 0; e < 8; ++e) acc[j][e] = f32x4{0, 0, 0, 0};
 
-    Eight<T> w[H], m[H];
+    Eight<T> w[H];           // of x ...
+    s16x8 wp[H][PW];         // ... or of p's planes, which stand in the plan's order
     float s[H][RT];
     auto row_of = [&](int i) { return i < count ? slot_row[first + i] : -1; };
-    auto fetch = [&](const int (&rid)[H]) {
+    auto fetch = [&](const int (&rid)[H], int i) {
 #pragma unroll
         for (int h = 0; h < H; ++h) {
             const int row = max(rid[h], 0);   // (a row that is not there is read as row 0 and counts with a factor of zero ...)
-            read8<T>(wide, row, c0, valid, w[h]);
-            if (masked) read8<T>(a.mask, row, c0, valid, m[h]);
+            if constexpr (UP) {
+                const int64_t slot = first + max(min(i + quad + 4 * h, count - 1), 0), at = min((int64_t)c0, a.ldp - 8);   // (in bounds; not used behind N)
+#pragma unroll
+                for (int p = 0; p < PW; ++p)
+                    wp[h][p] = __builtin_bit_cast(s16x8, *(VH_GLOBAL(u32x4, a.p + ((int64_t)p * a.ps.slots + slot) * a.ldp + at)));
+            } else {
+                read8<T>(a.x, row, c0, valid, w[h]);
+            }
 #pragma unroll
             for (int j = 0; j < RT; ++j) s[h][j] = small[(int64_t)row * r + min(16 * j + l15, r - 1)];
         }
@@ -471,13 +504,21 @@ __device__ __forceinline__ void adapter_grad_tile(const AdapterGradArgs& a, cons
     for (int h = 0; h < H; ++h) rid[h] = row_of(begin + quad + 4 * h);
 #pragma unroll
     for (int h = 0; h < H; ++h) nxt[h] = row_of(begin + STEP + quad + 4 * h);
-    fetch(rid);
+    fetch(rid, begin);
     for (int i = begin; i < count; i += STEP) {
         float f[H][8], sc[H][RT];
 #pragma unroll
         for (int h = 0; h < H; ++h) {
-            values8<T>(wide, w[h], f[h]);
-            if (masked) masked8<T>(a.mask, m[h], a.slope, f[h]);
+            if constexpr (UP) {   // (float32: the three cuts add up to what they were cut from)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    f[h][e] = bf_to_f((bf16_t)wp[h][PW - 1][e]);
+#pragma unroll
+                    for (int p = PW - 2; p >= 0; --p) f[h][e] += bf_to_f((bf16_t)wp[h][p][e]);
+                }
+            } else {
+                values8<T>(a.x, w[h], f[h]);
+            }
 #pragma unroll
             for (int e = 0; e < 8; ++e) f[h][e] = rid[h] >= 0 ? f[h][e] : 0.f;   // (... on zeros: row 0 may hold anything)
 #pragma unroll
@@ -485,7 +526,7 @@ __device__ __forceinline__ void adapter_grad_tile(const AdapterGradArgs& a, cons
             rid[h] = nxt[h];
         }
         if (i + STEP < count) {
-            fetch(rid);
+            fetch(rid, i + STEP);
 #pragma unroll
             for (int h = 0; h < H; ++h) nxt[h] = row_of(i + 2 * STEP + quad + 4 * h);
         }
@@ -570,7 +611,7 @@ __device__ __forceinline__ void turn_up(const AdapterGradArgs& a, int item, int 
     }
 }
 // p = dy f'(y), cut into operand planes, in the plan's order.  (bf16: where the slope applies p is rounded once more, to 8 bits: 2^-8 of
-// terms that the slope made small; dup is computed from the unrounded ones.)
+// terms that the slope made small.)
 template <class T>
 __device__ __forceinline__ void mask_and_order(const AdapterGradArgs& a, int64_t chunk0) {
     const int per = (int)(a.ldp / 8);
@@ -1078,7 +1119,7 @@ int vh_rows_plan(const int32_t* row_groups, int64_t rows, int64_t groups, int32_
         int bits = 1;
         while ((1 << bits) < groups + 2) ++bits;   // keys 0 .. groups + 1
         if (plan_is_small(rows, groups)) {
-            plan_small_kernel<<<1, 1024, 16 * (groups + 1) * sizeof(int), s>>>(row_groups, plan, ps, bits);
+            plan_small_kernel<<<(unsigned)ceil_div(rows, 1024), 1024, 18 * (groups + 1) * sizeof(int), s>>>(row_groups, plan, ps, bits);
             VH_HIP(hipGetLastError());
             return;
         }
