@@ -500,7 +500,8 @@ int vh_vae_train_epoch_dp(vh_vae* h, const int64_t* perm, int64_t n_batches, int
 enum { VH_F32 = 0, VH_BF16 = 1 };
 
 /* Rows sorted by group: which rows each adapter serves.  row_groups [rows]: a value outside [0, groups) is a row without an adapter.  The
- * plan serves every call on the same rows (all layers of a pass, forward and backward), concurrent ones too. */
+ * plan serves every call on the same rows (all layers of a pass, forward and backward), concurrent ones too; the calls' rows and groups have to be
+ * the plan's. */
 int vh_rows_plan_size(int64_t rows, int64_t groups, int64_t* plan_words, int64_t* scratch_words);
 int vh_rows_plan(const int32_t* row_groups, int64_t rows, int64_t groups, int32_t* plan /* 16-byte aligned */, int32_t* scratch, void* stream);
 
@@ -530,7 +531,7 @@ typedef struct {
     const uint8_t* exponents;
 } vh_held;
 
-/* y [rows][ldy]; optional: low = u [rows][rank] and the checkpoint of y, for the backward pass */
+/* y [rows][ldy]; optional: low = u [rows][rank] (16-byte aligned) and the checkpoint of y, for the backward pass */
 int vh_adapt_forward(const vh_adapt_layer* layer, const void* x, int64_t ldx, int64_t rows, const int32_t* plan, void* y, int64_t ldy, float* low,
                      uint8_t* codes, uint8_t* exponents, void* stream);
 /* the same y for a few rows, in one launch without a plan (any number of rows is right; from about a hundred on the plan is faster) */

@@ -93,6 +93,20 @@ def test_forward(ad, shape, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(1, 512, 40, 64, 3), (2, 1104, 33, 16, 9), (3, 100, 512, 30, 2), (16, 65, 17, 8, 200), (33, 32, 16, 1, 1000), (60, 304, 512, 8, 4)])
+def test_few_rows(ad, shape, dtype, monkeypatch):
+    """The launch without a plan, whatever the number of rows; and that both ways give the same layer."""
+    monkeypatch.setattr(ad, "_FEW", {t: 10 ** 12 for t in TYPES})
+    c = make(80, dtype, *shape)
+    u, y, tu, ty = forward_bounds(c, dtype, SLOPE)
+    shared = ad.SharedProjection(c["w"], c["b"])
+    got = ad.adapted_linear(c["x"], shared, c["down"], c["up"], c["groups"], SCALE, SLOPE)
+    close(got, y, ty, "y")
+    monkeypatch.setattr(ad, "_FEW", {t: 0 for t in TYPES})
+    close(ad.adapted_linear(c["x"], shared, c["down"], c["up"], c["groups"], SCALE, SLOPE), y, ty, "y with a plan")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_plan_sorts_stably_and_covers_every_row(ad, dtype):
     if dtype != torch.float32:
         pytest.skip("the plan has no type")

@@ -32,8 +32,11 @@ from . import _lib
 MAX_RANK = 64
 MAX_GROUPS = 16384
 BLOCK = 32   # columns of a checkpoint that share an exponent
-# up to so many rows adapted_linear goes without a plan: one launch, W read once per 16 rows
-FEW_ROWS = 64
+# Up to so many elements of adapters that the rows of a call ask for (rows x rank x k), adapted_linear goes without a plan: one launch, in
+# which every 16 columns read them anew.  Measured, that launch against plan and projection: bf16 304 -> 512, rank 8, 64 rows (156 k) 9.3 us
+# against 10.7; 1104 -> 512, rank 16, 8 rows (141 k) 11.8 / 13.5, 16 rows (283 k) 23 / 14; float32 (six products for one) 304 -> 512,
+# rank 8, 8 rows (19 k) 10.4 / 13.3, 16 rows (39 k) 17 / 13.5.  One or two rows always (512 -> 512, rank 64, one row: bf16 8 / 13, float32 12 / 26).
+_FEW = {_torch.bfloat16: 160_000, _torch.float32: 36_000}
 
 _DTYPES = {_torch.float32: 0, _torch.bfloat16: 1}
 # the current stream's handle without a Stream object around it (a call here is a few microseconds in all)
@@ -201,8 +204,8 @@ def _layer(shared, down, up, n_groups, scale, negative_slope):
 
 
 def _check_slope(negative_slope) -> None:
-    if negative_slope is not None and not 0.0 <= negative_slope <= 1.0:
-        raise ValueError(f"negative_slope must be in [0, 1] (the derivative is read from the sign of the result), not {negative_slope}")
+    if negative_slope is not None and not 0.0 <= negative_slope < math.inf:
+        raise ValueError(f"negative_slope must be finite and >= 0 (the derivative is read from the sign of the result), not {negative_slope}")
 
 
 def _input(x, shared) -> int:
@@ -234,7 +237,7 @@ def adapted_linear(x, shared: SharedProjection, down, up, groups: Union[_torch.T
         y = _torch.empty((rows, shared.n), dtype=x.dtype, device=x.device)
         if rows == 0:
             return y
-        if not planned and rows <= FEW_ROWS:
+        if not planned and (rows <= 2 or rows * down.shape[1] * shared.k <= _FEW[x.dtype]):
             _lib.check(lib.vh_adapt_forward_few(layer, x.data_ptr(), ld, rows, groups.data_ptr(), y.data_ptr(), shared.n, stream))
             return y
         if not planned:

@@ -303,7 +303,8 @@ __global__ __launch_bounds__(256) void pack_weight_kernel(const T* w, int64_t ld
 // =====================================================================================================================
 // Checkpoints
 // =====================================================================================================================
-// four lanes share a block of 32 columns, eight each
+// Four lanes share a block of 32 columns, eight each.  Bound by memory: 1000003 x 512 bf16 in 376 us, 4.1 TB/s of the 4.9 that a large copy
+// reaches; the way back (codes to bf16) in 297 us, 5.2 TB/s.
 template <class T>
 __global__ __launch_bounds__(256) void checkpoint_kernel(const T* x, int64_t ldx, int64_t rows, int cols, uint8_t* codes, uint8_t* exps) {
     const int chunks = (cols + kBlockCols - 1) / kBlockCols * 4;
@@ -440,7 +441,8 @@ __device__ __forceinline__ void masked8(const Source& s, const Eight<T>& v, floa
 // Gradients of the adapters:  down_g = sum v^T x  [rank][K],  up_g = s sum p^T u  [N][rank]
 // One wave = one item (at most item_rows rows of one group) and 128 columns of x or of p.  v_mfma_f32_16x16x4_f32: its operands
 // are one element per lane, so eight consecutive columns that a lane has read are the operands of eight instructions and nothing is
-// transposed; products and sums are fp32 whatever the tensors' type.
+// transposed; products and sums are fp32 whatever the tensors' type.  65537 rows of 1000 groups, rank 32, 1104 + 512 columns, bf16: 140 us for
+// 6.8 GF (50 TF of the 157 that the instruction has; the rows of a group are few steps, whose latency is what counts) and 100 MB of gradients.
 // =====================================================================================================================
 struct AdapterGradArgs {
     Source x, mask;            // mask.p == nullptr: f' = 1
@@ -677,11 +679,11 @@ __global__ __launch_bounds__(256) void adapter_grad_kernel(AdapterGradArgs a) {
 }
 template <class T>
 __global__ __launch_bounds__(256) void adapter_join_kernel(AdapterGradArgs a) {
-    if ((int)blockIdx.x >= a.plan[kPlanMultis]) return;
-    const int* mu = a.plan + a.ps.o_multi + 4 * (int64_t)blockIdx.x;
+    if ((int)blockIdx.y >= a.plan[kPlanMultis]) return;
+    const int* mu = a.plan + a.ps.o_multi + 4 * (int64_t)blockIdx.y;
     const int g = mu[0], part = mu[1], n = mu[2];
     const int64_t half = (int64_t)a.rank * a.K, pair = (int64_t)a.rank * (a.K + a.N);
-    const int64_t i = blockIdx.y * (int64_t)256 + threadIdx.x;
+    const int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x;
     if (i >= pair) return;
     float s = 0.f;
     for (int p = 0; p < n; ++p) s += a.parts[(part + p) * pair + i];
@@ -691,7 +693,9 @@ __global__ __launch_bounds__(256) void adapter_join_kernel(AdapterGradArgs a) {
 
 // =====================================================================================================================
 // Few rows: no plan.  A workgroup = 16 rows x 16 columns; eight waves share the depth of the projection and, one distinct adapter at a
-// time, the u of the rows; the last 256 products with B_g are plain fused multiply-adds in float32.
+// time, the u of the rows; the last 256 products with B_g are plain fused multiply-adds in float32.  One row, 304 -> 512, rank 8, bf16: 5 us,
+// of which a launch is 4.  Every workgroup reads the rows' adapters: rows x rank x K decides when the plan and the projection behind it are
+// faster (vamb_amd/adapters.py).
 // =====================================================================================================================
 struct FewArgs {
     const void* x;
@@ -712,7 +716,7 @@ template <class T, int RT>
 __global__ __launch_bounds__(512) void few_kernel(FewArgs a) {
     constexpr int P = Elem<T>::planes;
     __shared__ float part[8][16][17];
-    __shared__ float low[16][16 * RT + 1];
+    __shared__ float low[8][16][16 * RT + 1];   // [slice of the depth][row][rank]
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l15 = lane & 15, quad = lane >> 4;
     const int n0 = blockIdx.x * 16, r = a.rank, K = a.K;
     const int64_t row0 = blockIdx.y * (int64_t)16;
@@ -734,33 +738,61 @@ __global__ __launch_bounds__(512) void few_kernel(FewArgs a) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) part[wave][l15][4 * quad + i] = acc[i];
 
+    // u: the waves share the distinct adapters, and with fewer than eight of them the depth too (SL slices of it)
     unsigned pending = (unsigned)__ballot(g >= 0) & 0xffffu;
+    int distinct = 0;
+    for (unsigned p = pending; p; ++distinct) p &= ~(unsigned)__ballot(g == __builtin_amdgcn_readfirstlane(__shfl(g, __builtin_ctz(p))));
+    const int SL = distinct <= 1 ? 8 : distinct <= 2 ? 4 : distinct <= 4 ? 2 : 1, slice = wave % SL;
     for (int at = 0; pending; ++at) {
         const int one = __builtin_amdgcn_readfirstlane(__shfl(g, __builtin_ctz(pending)));
         const unsigned same = (unsigned)__ballot(g == one) & 0xffffu;
         pending &= ~same;
-        if ((at & 7) != wave) continue;
+        if (at % (8 / SL) != wave / SL) continue;
+        const T* const base = (const T*)a.down + (int64_t)one * r * K;
         f32x4 u[RT];
 #pragma unroll
         for (int j = 0; j < RT; ++j) u[j] = f32x4{0, 0, 0, 0};
-        for (int k0 = 0; k0 < K; k0 += 32) {
+        constexpr int B = RT == 4 ? 2 : 4;   // pieces of the depth whose loads are requested together
+        int k0 = 32 * slice;
+        for (; k0 + 32 * SL * (B - 1) + 32 <= K; k0 += 32 * SL * B) {
+            Raw8<T> xr8[B], ar8[B][RT];
+#pragma unroll
+            for (int b = 0; b < B; ++b) {
+                const int k = k0 + 32 * SL * b + 8 * quad;
+                xr8[b].load(xr + k);
+#pragma unroll
+                for (int j = 0; j < RT; ++j) ar8[b][j].load(base + (int64_t)min(16 * j + l15, r - 1) * K + k);   // (ranks behind r are not used)
+            }
+#pragma unroll
+            for (int b = 0; b < B; ++b) {
+                const Planes8<T> xp = to_planes(xr8[b]);
+#pragma unroll
+                for (int j = 0; j < RT; ++j) u[j] = mma(to_planes(ar8[b][j]).p, xp.p, u[j]);
+            }
+        }
+        for (; k0 < K; k0 += 32 * SL) {
             const int k = k0 + 8 * quad;
             const Planes8<T> xp = to_planes(load8<T>(xr + k, K - k));
 #pragma unroll
-            for (int j = 0; j < RT; ++j) {
-                const int rank = 16 * j + l15;
-                const Planes8<T> ap = to_planes(load8<T>((const T*)a.down + ((int64_t)one * r + rank) * K + k, rank < r ? K - k : 0));
-                u[j] = mma(ap.p, xp.p, u[j]);
-            }
+            for (int j = 0; j < RT; ++j) u[j] = mma(to_planes(load8<T>(base + (int64_t)min(16 * j + l15, r - 1) * K + k, K - k)).p, xp.p, u[j]);
         }
         if (g == one) {
 #pragma unroll
             for (int j = 0; j < RT; ++j)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) low[l15][16 * j + 4 * quad + i] = u[j][i];
+                for (int i = 0; i < 4; ++i) low[slice][l15][16 * j + 4 * quad + i] = u[j][i];
         }
     }
     __syncthreads();
+    if (SL > 1) {   // the slices' sums, in their order
+        for (int i = tid; i < 16 * r; i += 512) {
+            const int row = i / r, j = i - row * r;
+            float v = low[0][row][j];
+            for (int q = 1; q < SL; ++q) v += low[q][row][j];
+            low[0][row][j] = v;
+        }
+        __syncthreads();
+    }
     if (tid >= 256) return;
     // thread = (row, column)
     const int row = tid >> 4, col = n0 + (tid & 15);
@@ -775,7 +807,10 @@ __global__ __launch_bounds__(512) void few_kernel(FewArgs a) {
         for (int j0 = 0; j0 < r; j0 += 8) {
             const Raw8<T> w = load8<T>(b + j0, r - j0);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) s = fmaf(j0 + e < r ? low[row][min(j0 + e, 16 * RT - 1)] : 0.f, w.get(e), s);
+            for (int e = 0; e < 8; ++e) {
+                if (j0 + e >= r) break;
+                s = fmaf(low[0][row][j0 + e], w.get(e), s);
+            }
         }
         v = fmaf(s, a.scale, v);
     }
@@ -788,7 +823,8 @@ __global__ __launch_bounds__(512) void few_kernel(FewArgs a) {
 // Gradient of the shared projection from checkpoints:  dW = p^T x  [N][K],  db = sum p  [N]
 // Tile 128 x 128, split over the rows; both operands are contracted along their slow dimension: row-major LDS tiles [64 rows][128
 // columns] read by the transposing LDS instruction.  x's values are exact in bf16 (one plane), so float32 dy costs three products, not
-// six.  256-byte tile rows: the 32-byte pieces are XOR-permuted by the row so that the eight rows of half a read differ in their banks.
+// six.  8192 x 512 x 512 bf16: 24 us and 6 us for the join of 16 parts (a quarter of it vector instructions that mask, decode and convert; the
+// rest the steps' latency, eight waves a CU in step); 4096 x 1104 x 512 float32: 42 us and 6 us.  256-byte tile rows: the 32-byte pieces are XOR-permuted by the row so that the eight rows of half a read differ in their banks.
 // =====================================================================================================================
 struct WeightGradArgs {
     Source x, mask;
@@ -1005,8 +1041,8 @@ static void check_groups(int64_t g) { VH_REQUIRE(g >= 1 && g <= kMaxGroups, "the
 static void check_rank(int64_t r) { VH_REQUIRE(r >= 1 && r <= kMaxRank, "the rank must be in [1, %d], not %lld", kMaxRank, (long long)r); }
 static void check_ptr(const void* p, const char* what) { VH_REQUIRE(p != nullptr, "%s is NULL", what); }
 static void check_slope(int activation, float slope) {
-    // below 0 the sign of the value would not tell the derivative; up to 1 the activation is max(v, slope v)
-    VH_REQUIRE(!activation || (slope >= 0.f && slope <= 1.f), "the negative slope must be in [0, 1]");
+    // (below 0 the sign of the value would not tell the derivative)
+    VH_REQUIRE(!activation || (slope >= 0.f && slope < __builtin_inff()), "the negative slope must be finite and >= 0");
 }
 static void check_held(const uint8_t* codes, const uint8_t* exps, const char* what) {
     VH_REQUIRE((codes == nullptr) == (exps == nullptr), "%s: codes and exponents come together", what);
@@ -1069,7 +1105,7 @@ static void adapter_grads(const AdapterGradArgs& a, hipStream_t s) {
     else adapter_grads_rank<T, 4>(a, s);
     if (a.ps.rows > a.ps.item_rows) {
         const int64_t multis = a.ps.rows / a.ps.item_rows < a.ps.groups ? a.ps.rows / a.ps.item_rows : a.ps.groups;
-        adapter_join_kernel<T><<<dim3((unsigned)multis, (unsigned)ceil_div((int64_t)a.rank * (a.K + a.N), 256)), 256, 0, s>>>(a);
+        adapter_join_kernel<T><<<dim3((unsigned)ceil_div((int64_t)a.rank * (a.K + a.N), 256), (unsigned)multis), 256, 0, s>>>(a);
         VH_HIP(hipGetLastError());
     }
 }
@@ -1185,6 +1221,7 @@ int vh_adapt_forward(const vh_adapt_layer* l, const void* x, int64_t ldx, int64_
         check_ptr(plan, "plan");
         VH_REQUIRE(ldx >= l->k && ldy >= l->n, "row strides below the number of columns");
         check_held(codes, exponents, "checkpoint of y");
+        VH_REQUIRE((uintptr_t)low % 16 == 0, "low must be 16-byte aligned");
         const WeightShape ws = weight_shape(l->n, l->k, l->dtype);
         const int es = l->dtype == VH_BF16 ? 2 : 4;
         LinArgs a{};
