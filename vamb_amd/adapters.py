@@ -234,7 +234,7 @@ def adapted_linear(x, shared: SharedProjection, down, up, groups: Union[_torch.T
     lib = _lib.load()
     stream, before = _enter(x, shared.packed, down, up, groups.plan if planned else groups)
     try:
-        y = _torch.empty((rows, shared.n), dtype=x.dtype, device=x.device)
+        y = x.new_empty((rows, shared.n))
         if rows == 0:
             return y
         if not planned and (rows <= 2 or rows * down.shape[1] * shared.k <= _FEW[x.dtype]):
@@ -261,12 +261,12 @@ def adapted_linear_train(x, shared: SharedProjection, down, up, groups: RowGroup
     lib = _lib.load()
     stream, before = _enter(x, shared.packed, down, up, groups.plan)
     try:
-        y = _torch.empty((rows, shared.n), dtype=x.dtype, device=x.device)
+        y = x.new_empty((rows, shared.n))
         low = _torch.empty((rows, down.shape[1]), dtype=_torch.float32, device=x.device)
         held = Checkpoint8._empty(rows, shared.n, x.device)
         if rows:
             _lib.check(lib.vh_adapt_forward(layer, x.data_ptr(), ld, rows, groups.plan.data_ptr(), y.data_ptr(), shared.n, low.data_ptr(),
-                                            held.codes.data_ptr(), held.exponents.data_ptr(), stream))
+                                            *held._at, stream))
     finally:
         _leave(before)
     return y, low, held
@@ -295,7 +295,7 @@ def adapted_linear_backward(dy, x, y, low, shared: SharedProjection, down, up, g
     lib = _lib.load()
     stream, before = _enter(dy, shared.packed, down, up, groups.plan, tx, ty, low)
     try:
-        dx = _torch.empty((rows, shared.k), dtype=dy.dtype, device=dy.device) if need_dx else None
+        dx = dy.new_empty((rows, shared.k)) if need_dx else None
         if rows == 0:
             return dx, _torch.zeros_like(down), _torch.zeros_like(up)
         ddown, dup = _torch.empty_like(down), _torch.empty_like(up)
@@ -317,7 +317,7 @@ class Checkpoint8:
     of LeakyReLU can be read from it), a non-finite element is NaN, and magnitudes that would round to
     2^128 become 240 * 2^120.  Every value is exact in bfloat16."""
 
-    __slots__ = ("codes", "exponents", "columns")
+    __slots__ = ("columns", "_rows", "_memory", "_codes", "_exponents", "_at")
 
     def __init__(self, codes: _torch.Tensor, exponents: _torch.Tensor, columns: int):
         if columns < 1:
@@ -333,32 +333,52 @@ class Checkpoint8:
             raise ValueError("codes and exponents must be on one device")
         if codes.numel() and codes.data_ptr() % 8:
             raise ValueError("codes must be 8-byte aligned")
-        self.codes, self.exponents, self.columns = codes, exponents, columns
+        self.columns, self._rows = columns, codes.shape[0]
+        self._memory = self._codes = codes
+        self._exponents = exponents
+        self._at = codes.data_ptr(), exponents.data_ptr()   # what the library is given
 
     @classmethod
     def _empty(cls, rows: int, columns: int, device):
+        """Memory for a checkpoint: one allocation, codes before exponents (the tensors of both are made when somebody asks)."""
         blocks = -(-columns // BLOCK)
         self = cls.__new__(cls)
-        self.codes = _torch.empty((rows, BLOCK * blocks), dtype=_torch.uint8, device=device)
-        self.exponents = _torch.empty((rows, blocks), dtype=_torch.uint8, device=device)
-        self.columns = columns
+        self.columns, self._rows = columns, rows
+        self._memory = _torch.empty(rows * blocks * (BLOCK + 1), dtype=_torch.uint8, device=device)
+        self._codes = self._exponents = None
+        at = self._memory.data_ptr()
+        self._at = at, at + rows * blocks * BLOCK
         return self
 
     @property
+    def codes(self) -> _torch.Tensor:
+        if self._codes is None:
+            width = BLOCK * -(-self.columns // BLOCK)
+            self._codes = self._memory[:self._rows * width].view(self._rows, width)
+        return self._codes
+
+    @property
+    def exponents(self) -> _torch.Tensor:
+        if self._exponents is None:
+            blocks = -(-self.columns // BLOCK)
+            self._exponents = self._memory[self._rows * blocks * BLOCK:].view(self._rows, blocks)
+        return self._exponents
+
+    @property
     def shape(self):
-        return _torch.Size((self.codes.shape[0], self.columns))
+        return _torch.Size((self._rows, self.columns))
 
     def restore(self, dtype: _torch.dtype = _torch.float32) -> _torch.Tensor:
         """The values that the codes stand for, ``[rows, columns]`` (exact in either type)."""
         if dtype not in _DTYPES:
             raise ValueError(f"a checkpoint is restored to float32 or bfloat16, not {dtype}")
-        rows = self.codes.shape[0]
+        rows = self._rows
         lib = _lib.load()
-        stream, before = _enter(self.codes)
+        stream, before = _enter(self._memory)
         try:
-            out = _torch.empty((rows, self.columns), dtype=dtype, device=self.codes.device)
+            out = self._memory.new_empty((rows, self.columns), dtype=dtype)
             if rows:
-                _lib.check(lib.vh_checkpoint8_restore(self.codes.data_ptr(), self.exponents.data_ptr(), rows, self.columns, _DTYPES[dtype],
+                _lib.check(lib.vh_checkpoint8_restore(*self._at, rows, self.columns, _DTYPES[dtype],
                                                       out.data_ptr(), stream))
         finally:
             _leave(before)
@@ -377,7 +397,7 @@ def checkpoint8(x: _torch.Tensor) -> Checkpoint8:
     try:
         held = Checkpoint8._empty(rows, columns, x.device)
         if rows:
-            _lib.check(lib.vh_checkpoint8(x.data_ptr(), ld, rows, columns, code, held.codes.data_ptr(), held.exponents.data_ptr(), stream))
+            _lib.check(lib.vh_checkpoint8(x.data_ptr(), ld, rows, columns, code, *held._at, stream))
     finally:
         _leave(before)
     return held
@@ -385,9 +405,9 @@ def checkpoint8(x: _torch.Tensor) -> Checkpoint8:
 
 def _held(t, what: str, rows: int, cols: int, dtype):
     if isinstance(t, Checkpoint8):
-        if tuple(t.shape) != (rows, cols):
+        if t._rows != rows or t.columns != cols:
             raise ValueError(f"the checkpoint {what} must be [{rows}, {cols}], not {list(t.shape)}")
-        return _lib.Held(None, 0, t.codes.data_ptr(), t.exponents.data_ptr()), t.codes
+        return _lib.Held(None, 0, *t._at), t._memory
     ld = _matrix(t, what, rows, cols)
     if t.dtype != dtype:
         raise ValueError(f"{what} must be {dtype}, not {t.dtype}")
@@ -417,8 +437,8 @@ def checkpoint_weight_grad(dy, x: Checkpoint8, y=None, negative_slope: Optional[
     try:
         if rows == 0:
             return _torch.zeros((n, k), dtype=dy.dtype, device=dy.device), _torch.zeros(n, dtype=dy.dtype, device=dy.device)
-        dweight = _torch.empty((n, k), dtype=dy.dtype, device=dy.device)
-        dbias = _torch.empty(n, dtype=dy.dtype, device=dy.device)
+        dweight = dy.new_empty((n, k))
+        dbias = dy.new_empty(n)
         scratch = _torch.empty(_weight_grad_words(rows, n, k), dtype=_torch.float32, device=dy.device)
         _lib.check(lib.vh_checkpoint8_weight_grad(dy.data_ptr(), ld, held_x, held_y if negative_slope is not None else None,
                                                   negative_slope or 0.0, rows, n, k, code, dweight.data_ptr(), dbias.data_ptr(), scratch.data_ptr(), stream))
