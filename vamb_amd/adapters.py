@@ -310,7 +310,8 @@ def adapted_linear_backward(dy, x, y, low, shared: SharedProjection, down, up, g
 # ---- checkpoints ----------------------------------------------------------------------------------------------------------------
 class Checkpoint8:
     """A matrix ``[rows, columns]`` held in one byte per element: ``codes`` uint8 ``[rows, columns rounded up to 32]``, e4m3 bits of
-    ``x 2^-e``, and ``exponents`` uint8 ``[rows, columns / 32 rounded up]``, ``e + 127`` of every 32 columns.
+    ``x 2^-e``, and ``exponents`` uint8 ``[rows, columns / 32 rounded up]``, ``e + 127`` of every 32 columns.  Those made by hand keep to
+    what is written here: exponent bytes in [10, 247], and codes of value zero behind the last column.
 
     ``e`` is the least with ``amax <= 448 * 2^e`` over the block's finite magnitudes, kept in [-117, 120]; codes are rounded to nearest even
     (2^-4 relative to the value, 2^-10 of the block's scale near zero), their sign bit is set where ``x > 0`` does not hold (the derivative

@@ -823,8 +823,9 @@ __global__ __launch_bounds__(512) void few_kernel(FewArgs a) {
 // Gradient of the shared projection from checkpoints:  dW = p^T x  [N][K],  db = sum p  [N]
 // Tile 128 x 128, split over the rows; both operands are contracted along their slow dimension: row-major LDS tiles [64 rows][128
 // columns] read by the transposing LDS instruction.  x's values are exact in bf16 (one plane), so float32 dy costs three products, not
-// six.  8192 x 512 x 512 bf16: 24 us and 6 us for the join of 16 parts (a quarter of it vector instructions that mask, decode and convert; the
-// rest the steps' latency, eight waves a CU in step); 4096 x 1104 x 512 float32: 42 us and 6 us.  256-byte tile rows: the 32-byte pieces are XOR-permuted by the row so that the eight rows of half a read differ in their banks.
+// six.  8192 x 512 x 512 bf16: 24 us and 6 us for the join of 16 parts (a quarter of it vector instructions that mask, decode and
+// convert; the rest the steps' latency, eight waves a CU in step); 4096 x 1104 x 512 float32: 42 us and 6 us.  256-byte tile rows: the
+// 32-byte pieces are XOR-permuted by the row so that the eight rows of half a read differ in their banks.
 // =====================================================================================================================
 struct WeightGradArgs {
     Source x, mask;

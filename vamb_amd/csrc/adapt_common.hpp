@@ -2,8 +2,8 @@
 //
 // Operands of the matrix products.  v_mfma_f32_16x16x32_bf16 is the only matrix instruction of the wide products: bf16 tensors are
 // one operand plane, float32 tensors three (x = x0 + x1 + x2, each the next 8 significant bits cut off: exact, 3 x 8 = 24 bits), and of
-// the nine products of two such splits the six with i + j <= 2 are taken; the three dropped ones are below 2^-23 of the
-// product.  Six bf16 products run at 2.5 PF / 6 = 420 TF, the fp32 instruction at 157 TF.
+// the nine products of two such splits the six with i + j <= 2 are taken; the dropped ones (of the product's own sign, as cuts are) are
+// below 2^-21 of it together, 2^-24 in the mean.  Six bf16 products run at 2.5 PF / 6 = 420 TF, the fp32 instruction at 157 TF.
 //
 // 8-bit checkpoints.  One byte per element (e4m3: 1 + 4 + 3 bits) and one exponent byte per 32 columns of a row.  The
 // exponent k is the least with amax <= 448 * 2^k, kept in [-117, 120], so that (a) no code saturates, (b) every value code * 2^k has 4

@@ -11,8 +11,9 @@
 // operand layout of the 16-deep product with B_g, which therefore follows without leaving the registers.
 //   u is cut into planes there (two for bf16 tensors: 16 bits, three for float32), never rounded to 8 bits.
 // x reaches the LDS by DMA where its rows are 16-byte aligned bf16, else through registers (any alignment, any row stride; float32 is cut
-// into planes there).  The backward pass's p has been cut, masked and brought into the plan's order before (adapt.hip): DMA always.  LDS rows are 128 B (64 B with three planes); 16-byte pieces are XOR-permuted by the row so that
-// the 16 rows of an operand read fall into 16 different bank groups.
+// into planes there).  The backward pass's p has been cut, masked and brought into the plan's order before (adapt.hip): DMA always.
+// LDS rows are 128 B (64 B with three planes); 16-byte pieces are XOR-permuted by the row so that the 16 rows of an operand read fall
+// into different bank groups.
 #pragma once
 
 #include "adapt_common.hpp"
@@ -104,6 +105,7 @@ __global__ __launch_bounds__(64 * S::WM * S::WN * S::KG) void linear_kernel(LinA
     constexpr int KC = BK / 32;                         // 32-deep products per tile
     constexpr int MU = MS / WN;                         // subtiles whose u this wave computes (its share of the WN waves on the same rows)
     static_assert(PX >= 1 && BM * CH % THREADS == 0 && MS % WN == 0 && (!DMA || TRANS || P == 1) && (!TRANS || DMA), "tile shape");
+    static_assert(CH == 4 || CH == 8, "the piece permutations are for these");
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
 
     static_assert(KG == 1 || (WN == 1 && MS == 1), "groups along the depth have narrow waves");
@@ -120,10 +122,11 @@ __global__ __launch_bounds__(64 * S::WM * S::WN * S::KG) void linear_kernel(LinA
     const int n_sub = a.plan[kPlanSubs];
 
     // 16-byte pieces of a tile row are XOR-permuted by half the row's number within the operand: the 16 rows of an operand read then
-    // take the LDS's full 256 B a clock (measured; permuted by a quarter of it, rows of four pieces took 128).  Rows of W are read in another order: a lane's four results of the subtiles 2 i and
-    // 2 i + 1 are eight consecutive columns, 32 i + 8 (l15 / 4) + 4 (0 or 1) + l15 % 4 being the column of operand row l15.
-    auto swz = [](int row) { return CH == 16 ? row & 15 : (row >> 1) & (CH - 1); };
-    auto swz_w = [](int row) { return CH == 16 ? (row & 3) | ((row >> 1) & 12) : ((row >> 1) & 1) | ((row >> 2) & (CH - 2)); };
+    // take the LDS's full 256 B a clock (measured; permuted by a quarter of it, rows of four pieces took 128).  Rows of W are read in
+    // another order: a lane's four results of the subtiles 2 i and 2 i + 1 are eight consecutive columns, 32 i + 8 (l15 / 4) + 4 (0 or
+    // 1) + l15 % 4 being the column of operand row l15.
+    auto swz = [](int row) { return (row >> 1) & (CH - 1); };
+    auto swz_w = [](int row) { return ((row >> 1) & 1) | ((row >> 2) & (CH - 2)); };
     auto w_row = [&](int n) { return 32 * (n >> 1) + 8 * (l15 >> 2) + 4 * (n & 1) + (l15 & 3); };
 
     // ---- x pieces of this thread
