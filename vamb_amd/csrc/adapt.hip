@@ -425,6 +425,19 @@ __device__ __forceinline__ void store4(T* p, f32x4 v, int n) {
             if (i < n) p[i] = from_f<T>(v[i]);
     }
 }
+// eight values rounded to T
+template <class T>
+__device__ __forceinline__ Raw8<T> rounded8(const float (&f)[8]) {
+    Raw8<T> o;
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o.v[e] = __builtin_bit_cast(unsigned, __builtin_convertvector(f32x2{f[2 * e], f[2 * e + 1]}, bfx2));
+    } else {
+        o.a = f32x4{f[0], f[1], f[2], f[3]};
+        o.b = f32x4{f[4], f[5], f[6], f[7]};
+    }
+    return o;
+}
 // f'(y) of eight columns applied to f
 template <class T>
 __device__ __forceinline__ void masked8(const Source& s, const Eight<T>& v, float slope, float (&f)[8]) {
@@ -823,15 +836,15 @@ __global__ __launch_bounds__(512) void few_kernel(FewArgs a) {
 // Gradient of the shared projection from checkpoints:  dW = p^T x  [N][K],  db = sum p  [N]
 // Tile 128 x 128, split over the rows; both operands are contracted along their slow dimension: row-major LDS tiles [64 rows][128
 // columns] read by the transposing LDS instruction.  x's values are exact in bf16 (one plane), so float32 dy costs three products, not
-// six.  8192 x 512 x 512 bf16: 24 us and 6 us for the join of 16 parts (a quarter of it vector instructions that mask, decode and
-// convert; the rest the steps' latency, eight waves a CU in step); 4096 x 1104 x 512 float32: 42 us and 6 us.  256-byte tile rows: the
+// six.  8192 x 512 x 512 bf16: 19 us and 5 us for the join of 16 parts (eight steps of 0.6; the rest is the first
+// loads, 64 KB of partial sums a workgroup and the launch); 4096 x 1104 x 512 float32: 31 us and 6 us.  256-byte tile rows: the
 // 32-byte pieces are XOR-permuted by the row so that the eight rows of half a read differ in their banks.
 // =====================================================================================================================
 struct WeightGradArgs {
     Source x, mask;
     const void* dy;
     int64_t ldy, rows;
-    int N, K, k_tiles;
+    int N, K, k_tiles, tiles;
     int64_t split_rows;
     float slope;
     float* parts;      // [splits][N * K + N]
@@ -842,26 +855,35 @@ __device__ __forceinline__ s16x4 read_tr(const unsigned char* p) {
 }
 __device__ __forceinline__ int tr_swz(int row) { return (row & 3) | ((row >> 1) & 4); }
 
-template <class T, bool WHOLE>
-__device__ __forceinline__ void weight_grad_tile(const WeightGradArgs& a, int n0, int k0, unsigned char* smem) {
+enum { kNoMask, kMaskElements, kMaskCodes };   // where f' comes from
+
+// EVEN: N is a multiple of 8.  Which kind of tensor is read is part of the kernel's type: a load behind a branch, even a uniform one,
+// made every load in flight be waited for (8192 x 512 x 512, mask of codes: 1.5 us a step of 64 rows instead of 0.6)
+template <class T, int MASK, bool EVEN>
+__global__ __launch_bounds__(512) void weight_grad_kernel(WeightGradArgs a) {
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    // (in an order that gives the tiles of a split to one XCD, whose L2 they would share: 32768 rows 45 us against 46, 8192 rows 26 against 24)
+    const int split = (int)blockIdx.x / a.tiles, tile = (int)blockIdx.x % a.tiles, n0 = (tile / a.k_tiles) * 128, k0 = (tile % a.k_tiles) * 128;
     constexpr int P = Elem<T>::planes, BR = 64, TB = BR * 256;   // smem: [2][P + 1][TB]: planes of p, then x
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l15 = lane & 15, quad = lane >> 4;
-    const int64_t lo = blockIdx.y * a.split_rows, hi = min(lo + a.split_rows, a.rows);
+    const int64_t lo = split * a.split_rows, hi = min(lo + a.split_rows, a.rows);
     const int half = wave >> 2, wn = (wave >> 1) & 1, wk = wave & 1;   // waves 0-3 take rows 0-31 of a tile, waves 4-7 rows 32-63
-    const bool masked = a.mask.p != nullptr;
-    const Source dy = {a.dy, nullptr, a.ldy};
 
     // pieces of eight columns: thread t has column piece t % 16 of rows t / 16 and t / 16 + 32
     const int pc = tid & 15, pr = tid >> 4;
+    // (columns behind the last are read as the last piece: what they add to is not stored)
+    const int nc = EVEN ? min(n0 + 8 * pc, a.N - 8) : n0 + 8 * pc, nv = EVEN ? 8 : a.N - nc;
+    const int xc = min(k0 + 8 * pc, (int)a.x.ld - 8), mc = MASK == kMaskCodes ? min(n0 + 8 * pc, (int)a.mask.ld - 8) : 0;
     struct Codes { u32x2 code; unsigned exp; };
-    struct Ahead { Eight<T> pw[2], mw[2]; Codes xw[2]; } ahead[2];   // two tiles on their way
+    struct Ahead { Raw8<T> pw[2], me[2]; Codes mw[2], xw[2]; } ahead[2];   // two tiles on their way
     auto fetch = [&](int64_t row0, Ahead& t) {
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
             const int64_t at = min(row0 + pr + 32 * q, hi - 1);   // (behind the last row: read again, and set to zero in keep)
-            read8<T>(dy, at, n0 + 8 * pc, WHOLE ? 8 : a.N - n0 - 8 * pc, t.pw[q]);
-            if (masked) read8<T>(a.mask, at, n0 + 8 * pc, WHOLE ? 8 : a.N - n0 - 8 * pc, t.mw[q]);
-            read_codes8(a.x, at, k0 + 8 * pc, WHOLE ? 8 : a.K - k0 - 8 * pc, t.xw[q]);
+            t.pw[q] = load8<T>((const T*)a.dy + at * a.ldy + nc, nv);
+            if constexpr (MASK == kMaskElements) t.me[q] = load8<T>((const T*)a.mask.p + at * a.mask.ld + nc, nv);
+            if constexpr (MASK == kMaskCodes) read_codes8(a.mask, at, mc, 8, t.mw[q]);
+            read_codes8(a.x, at, xc, 8, t.xw[q]);
         }
     };
     const bool sums = k0 == 0;   // these workgroups add up p as well
@@ -873,18 +895,21 @@ __device__ __forceinline__ void weight_grad_tile(const WeightGradArgs& a, int n0
         for (int q = 0; q < 2; ++q) {
             const int row = pr + 32 * q, at = row * 256 + (((pc >> 1) ^ tr_swz(row)) * 32 + (pc & 1) * 16);
             if (row0 + row >= hi) {
-                t.pw[q].raw.zero();
+                t.pw[q].zero();
                 t.xw[q].code = u32x2{0, 0};
             }
-            Raw8<T> o = t.pw[q].raw;
-            if (masked || sums) {
+            Raw8<T> o = t.pw[q];
+            if (MASK != kNoMask || sums) {
                 float f[8];
-                values8<T>(dy, t.pw[q], f);
-                if (masked) {
-                    masked8<T>(a.mask, t.mw[q], a.slope, f);
-                    o.zero();
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) o.set(e, from_f<T>(f[e]));
+                for (int e = 0; e < 8; ++e) f[e] = t.pw[q].get(e);
+                if constexpr (MASK != kNoMask) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        if constexpr (MASK == kMaskCodes) f[e] *= slope_of(t.mw[q].code[e >> 2], e & 3, a.slope);
+                        else f[e] = t.me[q].get(e) > 0.f ? f[e] : f[e] * a.slope;
+                    }
+                    o = rounded8<T>(f);
                 }
                 if (sums) {
 #pragma unroll
@@ -974,7 +999,7 @@ __device__ __forceinline__ void weight_grad_tile(const WeightGradArgs& a, int n0
         for (int q = 0; q < 16; ++q) red[((wave & 3) * 16 + q) * 64 + lane] = acc[q / 4][q % 4];
     }
     __syncthreads();
-    float* out = a.parts + blockIdx.y * ((int64_t)a.N * a.K + a.N);
+    float* out = a.parts + split * ((int64_t)a.N * a.K + a.N);
     if (!half) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -983,7 +1008,7 @@ __device__ __forceinline__ void weight_grad_tile(const WeightGradArgs& a, int n0
             for (int j = 0; j < 4; ++j) {
                 const int k = k0 + wk * 64 + 16 * j + 4 * quad;
                 const f32x4 v = acc[i][j] + red[(wave * 16 + 4 * i + j) * 64 + lane];
-                if (WHOLE) {
+                if (n < a.N && k + 4 <= a.K) {
                     *reinterpret_cast<f32x4_any*>(out + (int64_t)n * a.K + k) = v;
                 } else {
 #pragma unroll
@@ -1005,13 +1030,6 @@ __device__ __forceinline__ void weight_grad_tile(const WeightGradArgs& a, int n0
             out[(int64_t)a.N * a.K + n0 + tid] = v;
         }
     }
-}
-template <class T>
-__global__ __launch_bounds__(512) void weight_grad_kernel(WeightGradArgs a) {
-    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    const int n0 = ((int)blockIdx.x / a.k_tiles) * 128, k0 = ((int)blockIdx.x % a.k_tiles) * 128;
-    if (n0 + 128 <= a.N && k0 + 128 <= a.K) weight_grad_tile<T, true>(a, n0, k0, smem);
-    else weight_grad_tile<T, false>(a, n0, k0, smem);
 }
 template <class T>
 __global__ __launch_bounds__(256) void weight_join_kernel(const float* parts, int splits, int64_t n_weight, int64_t total, T* dw, T* db) {
@@ -1109,6 +1127,30 @@ static void adapter_grads(const AdapterGradArgs& a, hipStream_t s) {
         adapter_join_kernel<T><<<dim3((unsigned)ceil_div((int64_t)a.rank * (a.K + a.N), 256), (unsigned)multis), 256, 0, s>>>(a);
         VH_HIP(hipGetLastError());
     }
+}
+template <class T, int MASK, bool EVEN>
+static void launch_weight_grad(const WeightGradArgs& a, int splits, hipStream_t s) {
+    const int64_t blocks = (int64_t)a.tiles * splits;
+    VH_REQUIRE(blocks < (int64_t(1) << 31), "too many tiles for one launch");
+    constexpr int bytes = 2 * (Elem<T>::planes + 1) * 64 * 256;
+    if constexpr (bytes > 65536)
+        VH_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(weight_grad_kernel<T, MASK, EVEN>), hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    weight_grad_kernel<T, MASK, EVEN><<<(unsigned)blocks, 512, bytes, s>>>(a);
+    VH_HIP(hipGetLastError());
+}
+template <class T, int MASK>
+static void weight_grad_width(const WeightGradArgs& a, int splits, hipStream_t s) {
+    if (a.N % 8 == 0) launch_weight_grad<T, MASK, true>(a, splits, s);
+    else launch_weight_grad<T, MASK, false>(a, splits, s);
+}
+template <class T>
+static void weight_grad(const WeightGradArgs& a, int splits, void* dweight, void* dbias, hipStream_t s) {
+    if (a.mask.p == nullptr) weight_grad_width<T, kNoMask>(a, splits, s);
+    else if (a.mask.exps == nullptr) weight_grad_width<T, kMaskElements>(a, splits, s);
+    else weight_grad_width<T, kMaskCodes>(a, splits, s);
+    const int64_t n_weight = (int64_t)a.N * a.K, total = n_weight + a.N;
+    weight_join_kernel<T><<<(unsigned)ceil_div(total, 256), 256, 0, s>>>(a.parts, splits, n_weight, total, (T*)dweight, (T*)dbias);
+    VH_HIP(hipGetLastError());
 }
 // the backward pass's scratch, in words: v, up turned around, p, the parts of groups of several items
 struct BackwardScratch {
@@ -1449,22 +1491,10 @@ int vh_checkpoint8_weight_grad(const void* dy, int64_t lddy, const vh_held* x, c
         a.slope = negative_slope;
         a.parts = scratch;
         const int64_t splits = weight_splits(rows, n, k, &a.split_rows);
-        const int64_t tiles = ceil_div(n, 128) * a.k_tiles, total = n * k + n;
-        VH_REQUIRE(tiles < (int64_t(1) << 31) && splits < 65536, "too many tiles for one launch");
-        const dim3 grid((unsigned)tiles, (unsigned)splits);
-        hipStream_t s = (hipStream_t)stream;
-        if (dtype == VH_BF16) {
-            weight_grad_kernel<bf16_t><<<grid, 512, 2 * 2 * 64 * 256, s>>>(a);
-            VH_HIP(hipGetLastError());
-            weight_join_kernel<bf16_t><<<(unsigned)ceil_div(total, 256), 256, 0, s>>>(scratch, (int)splits, n * k, total, (bf16_t*)dweight, (bf16_t*)dbias);
-        } else {
-            constexpr int bytes = 2 * 4 * 64 * 256;
-            VH_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(weight_grad_kernel<float>), hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
-            weight_grad_kernel<float><<<grid, 512, bytes, s>>>(a);
-            VH_HIP(hipGetLastError());
-            weight_join_kernel<float><<<(unsigned)ceil_div(total, 256), 256, 0, s>>>(scratch, (int)splits, n * k, total, (float*)dweight, (float*)dbias);
-        }
-        VH_HIP(hipGetLastError());
+        const int64_t tiles = ceil_div(n, 128) * a.k_tiles;
+        a.tiles = (int)tiles;
+        if (dtype == VH_BF16) weight_grad<bf16_t>(a, (int)splits, dweight, dbias, (hipStream_t)stream);
+        else weight_grad<float>(a, (int)splits, dweight, dbias, (hipStream_t)stream);
     });
 }
 
