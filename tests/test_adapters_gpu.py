@@ -179,6 +179,24 @@ def test_backward(ad, shape, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,n,k", [(1, 8, 1), (63, 40, 33), (129, 33, 130), (700, 136, 300), (257, 257, 31), (320, 128, 128)])
+def test_weight_gradient_of_every_kind_of_mask(ad, dtype, rows, n, k):
+    """Masks as elements and as codes are the same mask, bit for bit; what stands beside the rows of dy and y enters nothing."""
+    c = make(90, dtype, rows, k, n, 1, 1)
+    x8 = ad.checkpoint8(c["x"])
+    y = make(91, dtype, rows, k, n, 1, 1)["dy"]
+    beside = [torch.full((rows, n + 8), float("nan"), dtype=dtype, device="cuda") for _ in range(2)]
+    dy, ys = (b[:, :n].copy_(t) for b, t in zip(beside, (c["dy"], y)))
+    got = ad.checkpoint_weight_grad(dy, x8, ys, SLOPE)
+    held = ad.checkpoint_weight_grad(c["dy"], x8, ad.checkpoint8(y), SLOPE)
+    assert all(torch.equal(a, b) for a, b in zip(got, held))
+    for slope, (dw, db) in ((SLOPE, got), (None, ad.checkpoint_weight_grad(dy, x8))):
+        want = backward_bounds(c, f64(x8.restore()), f64(y), np.zeros((rows, 1)), dtype, slope)
+        close(dw, *want["dw"], "dw")
+        close(db, *want["db"], "db")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows,cols", [(1, 1), (3, 31), (7, 32), (5, 33), (64, 154), (9, 512), (2, 1104)])
 def test_checkpoint(ad, rows, cols, dtype):
     rng = np.random.default_rng(rows * 1000 + cols)
