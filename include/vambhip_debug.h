@@ -69,6 +69,10 @@ int vh_debug_check_guards(char* report, int cap, int* damaged);
  * on the host clock).  Rows are zero where no workgroup ran.  cap_rows >= 4096. */
 int vh_debug_scan_timeline(vh_clu* h, unsigned long long* stamps, int cap_rows, int* n_rows, double* host_us);
 
+/* test hook (host only): the highest slot of the row plan of `rows` rows and `groups` groups that the adapter-gradient kernels read for an
+ * item (first slot, number of rows), and the plan's slots */
+int vh_debug_adapt_item_reads(int64_t rows, int64_t groups, int32_t first, int32_t count, int64_t* highest, int64_t* slots);
+
 #ifdef __cplusplus
 }
 #endif

@@ -185,3 +185,23 @@ def test_oracle_encoding():
     assert np.array_equal(codes & 127, want & 127)
     assert np.array_equal(codes >= 128, ~(scaled.numpy() > 0))
     assert np.abs(ao.decode(codes, exps, 70) - x).max() <= (2.0 ** -4 * np.abs(x)).max()
+
+
+@pytest.mark.parametrize("rows,groups", [(1, 1), (1, 2), (1, 200), (3, 4), (7, 9), (15, 16), (15, 200), (16, 40), (17, 3), (300, 5), (2000, 2)])
+def test_gradient_items_read_slots_that_exist(rows, groups):
+    """A plan laid out as adapt_common.hpp describes it: whatever groups the rows are of, groups without rows behind them too, no item's rows are
+    looked for at or behind the plan's last slot (behind it, in the last plane of p, the caller's scratch ends)."""
+    lib = _lib.load()
+    rng = np.random.default_rng(rows * 1000 + groups)
+    highest, slots = ctypes.c_int64(), ctypes.c_int64()
+    for of in (np.arange(rows) % groups, np.zeros(rows, int), rng.integers(0, groups, rows), np.full(rows, -1), np.full(rows, groups - 1)):
+        first = 0
+        for g in range(groups):
+            count = int((of == g).sum())
+            for at in range(0, max(count, 1), 128):
+                piece = min(128, count - at)
+                _lib.check(lib.vh_debug_adapt_item_reads(rows, groups, first + at, piece, highest, slots))
+                assert 0 <= highest.value < slots.value, (g, first + at, piece)
+                if piece:
+                    assert highest.value == first + at + piece - 1
+            first += -(-count // 16) * 16

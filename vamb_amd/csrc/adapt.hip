@@ -503,7 +503,7 @@ __device__ __forceinline__ void adapter_grad_tile(const AdapterGradArgs& a, cons
         for (int h = 0; h < H; ++h) {
             const int row = max(rid[h], 0);   // (a row that is not there is read as row 0 and counts with a factor of zero ...)
             if constexpr (UP) {
-                const int64_t slot = first + max(min(i + quad + 4 * h, count - 1), 0), at = min((int64_t)c0, a.ldp - 8);   // (in bounds; not used behind N)
+                const int64_t slot = item_slot(first, count, i + quad + 4 * h, a.ps.slots), at = min((int64_t)c0, a.ldp - 8);   // (in bounds; not used behind N)
 #pragma unroll
                 for (int p = 0; p < PW; ++p)
                     wp[h][p] = __builtin_bit_cast(s16x8, *(VH_GLOBAL(u32x4, a.p + ((int64_t)p * a.ps.slots + slot) * a.ldp + at)));
@@ -1417,6 +1417,21 @@ int vh_adapt_backward(const vh_adapt_layer* l, const void* dy, int64_t lddy, con
             adapter_first<float>(g, s);
             launch_linear_f32(a, true, s);
             adapter_grads<float>(g, s);
+        }
+    });
+}
+
+int vh_debug_adapt_item_reads(int64_t rows, int64_t groups, int32_t first, int32_t count, int64_t* highest, int64_t* slots) {
+    return guarded([&] {
+        check_rows(rows);
+        check_groups(groups);
+        check_ptr(highest, "highest");
+        check_ptr(slots, "slots");
+        *slots = plan_shape(rows, groups).slots;
+        *highest = -1;
+        for (int i = 0; i < (count > 32 ? count : 32); ++i) {   // (up to 32 rows a step, the first of them asked for whatever the count)
+            const int64_t at = item_slot(first, count, i, *slots);
+            if (at > *highest) *highest = at;
         }
     });
 }

@@ -217,6 +217,14 @@ inline PlanShape plan_shape(int64_t rows, int64_t groups) {
     s.words = s.o_multi + 4 * s.multis;
     return s;
 }
+// The slot that the gradient kernels read for row i of an item whose rows begin at slot `first`.  Rows behind the item's last are read as that
+// one and counted as nothing.  An item without rows has no slot of its own: behind the last run its `first` can be `slots` (one row, whose group
+// is not the last: 16 of 16), so the result is kept below it.
+__host__ __device__ __forceinline__ int64_t item_slot(int first, int count, int i, int64_t slots) {
+    const int last = count > 0 ? count - 1 : 0;
+    const int64_t slot = (int64_t)first + (i < last ? i : last);
+    return slot < slots ? slot : slots - 1;
+}
 enum { kPlanSubs = 0, kPlanItems = 1, kPlanMultis = 2, kPlanParts = 3 };
 
 // ---- arguments of the shared-projection kernel (adapt_linear.hpp) -----------------------------------------------------------------
