@@ -9,7 +9,8 @@
 // shared by no other wave), so u costs no second pass over x.  Both products are taken as D[column][row]: a
 // lane ends with four consecutive columns of one row, and u's accumulator layout (lane: row l & 15, ranks 4 (l >> 4) + i) IS the
 // operand layout of the 16-deep product with B_g, which therefore follows without leaving the registers.
-//   u is cut into planes there (two for bf16 tensors: 16 bits, three for float32), never rounded to 8 bits.
+//   u is cut into three planes there (24 bits, all of it) for tensors of either type: with two, a bf16 result differed from the rounded exact one
+//   in one element of 300 (16 bits of u against the 8 of a rounded sum); the third costs one 16-deep product in three per 16 columns and ranks.
 // x reaches the LDS by DMA where its rows are 16-byte aligned bf16, else through registers (any alignment, any row stride; float32 is cut
 // into planes there).  The backward pass's p has been cut, masked and brought into the plan's order before (adapt.hip): DMA always.
 // LDS rows are 128 B (64 B with three planes); 16-byte pieces are XOR-permuted by the row so that the 16 rows of an operand read fall
@@ -37,8 +38,7 @@ __device__ __forceinline__ void dma16(Buffer b, unsigned offset, unsigned char* 
 constexpr unsigned kBehind = 0xfffffff0u;   // behind every buffer (their sizes are below it)
 static __device__ const uint4 g_zero32[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
 
-template <int PU>
-__device__ __forceinline__ void cut4(const f32x4 v, s16x4 (&o)[PU]) {
+__device__ __forceinline__ void cut4(const f32x4 v, s16x4 (&o)[3]) {
     unsigned w[3][2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
@@ -50,7 +50,7 @@ __device__ __forceinline__ void cut4(const f32x4 v, s16x4 (&o)[PU]) {
         w[2][e] = (l0 >> 16) | (l1 & 0xffff0000u);
     }
 #pragma unroll
-    for (int p = 0; p < PU; ++p) o[p] = __builtin_bit_cast(s16x4, u32x2{w[p][0], w[p][1]});
+    for (int p = 0; p < 3; ++p) o[p] = __builtin_bit_cast(s16x4, u32x2{w[p][0], w[p][1]});
 }
 __device__ __forceinline__ f32x4 mfma16(s16x4 a, s16x4 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a, b, c, 0, 0, 0); }
 
@@ -75,7 +75,7 @@ __device__ __forceinline__ void load4(const float* p, int64_t stride, int valid,
     for (int i = 0; i < 4; ++i) o[i] = *(VH_GLOBAL(float, i < valid ? p + i * stride : (const float*)g_zero32));
 }
 __device__ __forceinline__ void planes4(const u32x2& r, s16x4 (&o)[1]) { o[0] = __builtin_bit_cast(s16x4, r); }
-__device__ __forceinline__ void planes4(const f32x4& r, s16x4 (&o)[3]) { cut4<3>(r, o); }
+__device__ __forceinline__ void planes4(const f32x4& r, s16x4 (&o)[3]) { cut4(r, o); }
 typedef short tr_s16x4 __attribute__((ext_vector_type(4)));
 template <class T> struct Raw4;
 template <> struct Raw4<bf16_t> { typedef u32x2 type; };
@@ -93,7 +93,6 @@ template <class T, class S, int RT, bool TRANS, bool DMA>
 __global__ __launch_bounds__(64 * S::WM * S::WN * S::KG) void linear_kernel(LinArgs a) {
     constexpr int WM = S::WM, WN = S::WN, MS = S::MS, NT = S::NT, NW = WM * WN, THREADS = 64 * NW, KG = S::KG;
     constexpr int P = Elem<T>::planes;
-    constexpr int PU = P == 1 ? 2 : 3;
     constexpr int BK = S::BK;
     constexpr int CH = BK / 8;                          // 16-byte pieces of a tile row
     constexpr int BM = 16 * MS * WM, BN = 16 * NT * WN;
@@ -471,8 +470,8 @@ __global__ __launch_bounds__(64 * S::WM * S::WN * S::KG) void linear_kernel(LinA
                 }
 #pragma unroll
                 for (int j = 0; j < RT; ++j) {
-                    s16x4 uf[PU];
-                    cut4<PU>(lo[j] * a.scale, uf);
+                    s16x4 uf[3];
+                    cut4(lo[j] * a.scale, uf);
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
                         s16x4 op[P];
@@ -482,7 +481,7 @@ __global__ __launch_bounds__(64 * S::WM * S::WN * S::KG) void linear_kernel(LinA
 #pragma unroll
                             for (int i = 0; i < P; ++i)
 #pragma unroll
-                                for (int k = 0; k < PU; ++k)
+                                for (int k = 0; k < 3; ++k)
                                     if (i + k == s) acc[m][n] = mfma16(op[i], uf[k], acc[m][n]);
                     }
                 }
