@@ -19,14 +19,15 @@ def ad():
 
 
 def test_low_products_keep_all_their_bits(ad):
-    """u = (1 + 2^-20, 1), B = (1, -1): y = scale 2^-20, and the same of v in the backward pass; nothing in it is rounded (bf16 tensors)."""
+    """u = (1 + 2^-8 + 2^-20, 1 + 2^-8), B = (1, -1): y = scale 2^-20, and the same of v in the backward pass; nothing in it is rounded (bf16
+    tensors).  (1 + 2^-20 alone would not do: its parts are 8 bits each.)"""
     rows, n, k = 20, 40, 72
     bf = lambda t: t.to("cuda", torch.bfloat16)  # noqa: E731
     x, dy = torch.zeros(rows, k), torch.zeros(rows, n)
-    x[:, 0], x[:, 1] = 1.0, 2.0 ** -20
-    dy[:, 0], dy[:, 1] = 1.0, 2.0 ** -20
+    for t in (x, dy):
+        t[:, 0], t[:, 1], t[:, 2] = 1.0, 2.0 ** -8, 2.0 ** -20
     down, up = torch.zeros(1, 2, k), torch.zeros(1, n, 2)
-    down[0, :, 0], down[0, 0, 1] = 1.0, 1.0       # u as above
+    down[0, :, :2], down[0, 0, 2] = 1.0, 1.0      # u as above
     up[0, :, 0], up[0, :, 1] = 1.0, -1.0
     shared = ad.SharedProjection(bf(torch.zeros(n, k)))
     groups = torch.zeros(rows, dtype=torch.int32, device="cuda")
@@ -35,7 +36,7 @@ def test_low_products_keep_all_their_bits(ad):
     for g in (groups, plan):
         assert (ad.adapted_linear(bf(x), shared, bf(down), bf(up), g, SCALE) == want).all()
     up[0] = 0.0
-    up[0, 0, :], up[0, 1, 0] = 1.0, 1.0           # v = scale (1 + 2^-20, 1)
+    up[0, :2, :], up[0, 2, 0] = 1.0, 1.0          # v = scale u
     down[0, 0], down[0, 1] = 1.0, -1.0
     dx, _, _ = ad.adapted_linear_backward(bf(dy), bf(x), None, torch.zeros(rows, 2, device="cuda"), shared, bf(down), bf(up), plan, SCALE)
     assert (dx == want).all()
