@@ -40,3 +40,45 @@ def test_low_products_keep_all_their_bits(ad):
     down[0, 0], down[0, 1] = 1.0, -1.0
     dx, _, _ = ad.adapted_linear_backward(bf(dy), bf(x), None, torch.zeros(rows, 2, device="cuda"), shared, bf(down), bf(up), plan, SCALE)
     assert (dx == want).all()
+
+
+def slope_case(ad, dtype, slope):
+    """Pairs of rows: p is (slope, 1, ...) in the first of a pair (the slope applies to its first column) and (t, 0, ...) in the second, t the
+    slope in the tensors' type; with these, sums that leave slope - t, which is below half a step of that type."""
+    pairs, n, k = 20, 40, 72
+    dy, y = torch.zeros(pairs, 2, n), torch.ones(pairs, 2, n)
+    t = float(torch.tensor(slope).to(dtype))
+    dy[:, 0, :2], dy[:, 1, 0] = 1.0, t
+    y[:, 0, 0] = -1.0
+    x = torch.zeros(pairs, 2, k)
+    x[:, 0], x[:, 1] = 1.0, -1.0
+    to = lambda z: z.reshape(2 * pairs, -1).to("cuda", dtype)  # noqa: E731
+    return pairs, n, k, to(dy), to(y), to(x), t, float(np.float32(slope)) - t
+
+
+@pytest.mark.parametrize("held", [False, True])
+@pytest.mark.parametrize("slope", [0.01, 0.3])
+def test_a_slope_leaves_dy_more_bits_than_it_had(ad, slope, held):
+    """p = dy slope of bf16 tensors is held to 2^-16 of its size in every product of the backward pass (rounded to bf16 it would be 2^-8,
+    and the sums below nothing)."""
+    dtype = torch.bfloat16
+    pairs, n, k, dy, y, x, t, rest = slope_case(ad, dtype, slope)
+    rows = 2 * pairs
+    plan = ad.group_rows(torch.zeros(rows, dtype=torch.int32, device="cuda"), 1)
+    low = torch.ones(rows, 1, device="cuda")
+    low[1::2] = -1.0
+    w, down, up = torch.zeros(n, k), torch.zeros(1, 1, k), torch.zeros(1, n, 1)
+    w[0], w[1] = 1.0, -t                              # p w: slope - t in a pair's first row, t in its second
+    up[0, 0], up[0, 1] = 1.0, -t                      # v: the same, times the scale
+    to = lambda z: z.to("cuda", dtype)  # noqa: E731
+    shared, down, up = ad.SharedProjection(to(w)), to(down), to(up)
+    ys, xs = (ad.checkpoint8(y), ad.checkpoint8(x)) if held else (y, x)
+    dx, ddown, dup = ad.adapted_linear_backward(dy, xs, ys, low, shared, down, up, plan, SCALE, slope)
+    tol = 2.0 ** -16 * slope + 2.0 ** -8 * abs(rest)  # p's bits, and the result's rounding
+    assert ((dx[0::2].double() - rest).abs() <= tol).all() and (dx[1::2] == t).all()
+    # dA = sum v x = scale pairs ((slope - t) - t)
+    want = SCALE * pairs * (rest - t)
+    assert ((ddown.double() - want).abs() <= SCALE * pairs * 2.0 ** -16 * slope + 2.0 ** -8 * abs(want)).all()
+    # dB of the first column = scale sum p u = scale pairs (slope - t)
+    assert ((dup[0, 0].double() - SCALE * pairs * rest).abs() <= SCALE * pairs * tol).all()
+    assert (dup[0, 1] == SCALE * pairs).all() and not dup[0, 2:].any()

@@ -466,7 +466,7 @@ struct AdapterGradArgs {
     void *ddown, *dup;
     const void* up;            // [groups][N][rank], and ...
     void* turned;              // ... [groups][rank][ldp], zeros behind N
-    bf16_t* p;                 // dy f' as operand planes [planes][slots][ldp] in the plan's order, zeros behind N and in filling slots
+    bf16_t* p;                 // dy f' as operand planes [PP][slots][ldp] in the plan's order, zeros behind N and in filling slots
     int64_t ldp;
     float* parts;
     int K, N, rank;
@@ -476,15 +476,15 @@ struct AdapterGradArgs {
 };
 
 // An item's rows, 4 H a step, and 128 columns: one wave (SPLIT = 1), or the workgroup's four, each with every fourth step (SPLIT = 4; their
-// sums are added in order).  WHOLE: all columns exist, so that the loads need no branch.
-template <class T, int RT, int H, int SPLIT, bool UP, bool WHOLE>
+// sums are added in order).  PP: p's planes.  WHOLE: all columns exist, so that the loads need no branch.
+template <class T, int RT, int H, int SPLIT, int PP, bool UP, bool WHOLE>
 __device__ __forceinline__ void adapter_grad_tile(const AdapterGradArgs& a, const int* it, int tile0, f32x4 (*red)[8][64]) {
     const int g = it[0], first = it[1], count = it[2], part = it[3];
     const int* slot_row = a.plan + a.ps.o_row;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, quad = lane >> 4;
     const int C = UP ? a.N : a.K, c0 = tile0 + 8 * l15, valid = WHOLE ? 8 : C - c0, r = a.rank;
     const float* small = UP ? a.low : a.v;
-    constexpr int PW = UP ? Elem<T>::planes : 1;
+    constexpr int PW = UP ? PP : 1;
     const int begin = SPLIT > 1 ? 4 * H * wave : 0;
     constexpr int STEP = 4 * H * SPLIT;
 
@@ -524,7 +524,7 @@ __device__ __forceinline__ void adapter_grad_tile(const AdapterGradArgs& a, cons
         float f[H][8], sc[H][RT];
 #pragma unroll
         for (int h = 0; h < H; ++h) {
-            if constexpr (UP) {   // (float32: the three cuts add up to what they were cut from)
+            if constexpr (UP) {   // (the cuts add up to what they were cut from)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     f[h][e] = bf_to_f((bf16_t)wp[h][PW - 1][e]);
@@ -625,9 +625,8 @@ __device__ __forceinline__ void turn_up(const AdapterGradArgs& a, int item, int 
         if (n0 + c < a.ldp) store8<T>(out + (int64_t)j * a.ldp + c, v, 8);   // (ldp is a multiple of 8)
     }
 }
-// p = dy f'(y), cut into operand planes, in the plan's order.  (bf16: where the slope applies p is rounded once more, to 8 bits: 2^-8 of
-// terms that the slope made small.)
-template <class T>
+// p = dy f'(y), cut into operand planes (cut8), in the plan's order
+template <class T, int PP>
 __device__ __forceinline__ void mask_and_order(const AdapterGradArgs& a, int64_t chunk0) {
     const int per = (int)(a.ldp / 8);
     const int slots = 16 * a.plan[kPlanSubs];
@@ -654,27 +653,25 @@ __device__ __forceinline__ void mask_and_order(const AdapterGradArgs& a, int64_t
         float f[8];
         values8<T>(dy, w[q], f);
         if (a.mask.p != nullptr) masked8<T>(a.mask, m[q], a.slope, f);
-        Raw8<T> o;
-        o.zero();
 #pragma unroll
-        for (int e = 0; e < 8; ++e) o.set(e, from_f<T>(rid[q] >= 0 ? f[e] : 0.f));
-        const Planes8<T> pl = to_planes(o);
+        for (int e = 0; e < 8; ++e) f[e] = rid[q] >= 0 ? f[e] : 0.f;
+        const Cut8<PP> pl = cut8<PP>(f);
 #pragma unroll
-        for (int p = 0; p < Elem<T>::planes; ++p)
+        for (int p = 0; p < PP; ++p)
             *reinterpret_cast<s16x8*>(a.p + ((int64_t)p * a.ps.slots + slot[q]) * a.ldp + col[q]) = pl.p[p];
     }
 }
 // before the projection's pass, two kinds of workgroups: up turned around (64 columns each), and p
-template <class T>
+template <class T, int PP>
 __global__ __launch_bounds__(256) void adapter_first_kernel(AdapterGradArgs a) {
     __shared__ T tile[64 * (kMaxRank + 1)];
     const int turns = (a.N + 63) / 64;
     const int64_t b = blockIdx.x, turning = a.ps.items * turns;
     if (b < turning) turn_up<T>(a, (int)(b / turns), 64 * (int)(b % turns), tile);
-    else mask_and_order<T>(a, (b - turning) * 1024);
+    else mask_and_order<T, PP>(a, (b - turning) * 1024);
 }
 // behind it (v): tiles of down, then tiles of up
-template <class T, int RT, int H, int SPLIT>
+template <class T, int RT, int H, int SPLIT, int PP>
 __global__ __launch_bounds__(256) void adapter_grad_kernel(AdapterGradArgs a) {
     __shared__ f32x4 red[SPLIT > 1 ? 3 : 1][SPLIT > 1 ? 8 : 1][64];
     auto* const r = reinterpret_cast<f32x4(*)[8][64]>(red);
@@ -683,11 +680,11 @@ __global__ __launch_bounds__(256) void adapter_grad_kernel(AdapterGradArgs a) {
     const int downs = (a.K + 127) / 128, ups = (a.N + 127) / 128;
     int tile = SPLIT > 1 ? (int)blockIdx.y : 4 * (int)blockIdx.y + ((int)threadIdx.x >> 6);
     if (tile < downs) {
-        if (128 * tile + 128 <= a.K) adapter_grad_tile<T, RT, H, SPLIT, false, true>(a, it, 128 * tile, r);
-        else adapter_grad_tile<T, RT, H, SPLIT, false, false>(a, it, 128 * tile, r);
+        if (128 * tile + 128 <= a.K) adapter_grad_tile<T, RT, H, SPLIT, PP, false, true>(a, it, 128 * tile, r);
+        else adapter_grad_tile<T, RT, H, SPLIT, PP, false, false>(a, it, 128 * tile, r);
     } else if ((tile -= downs) < ups) {
-        if (128 * tile + 128 <= a.N) adapter_grad_tile<T, RT, H, SPLIT, true, true>(a, it, 128 * tile, r);
-        else adapter_grad_tile<T, RT, H, SPLIT, true, false>(a, it, 128 * tile, r);
+        if (128 * tile + 128 <= a.N) adapter_grad_tile<T, RT, H, SPLIT, PP, true, true>(a, it, 128 * tile, r);
+        else adapter_grad_tile<T, RT, H, SPLIT, PP, true, false>(a, it, 128 * tile, r);
     }
 }
 template <class T>
@@ -1101,27 +1098,27 @@ static void few_rank(const FewArgs& a, hipStream_t s) {
     else if (a.rank <= 32) launch_few<T, 2>(a, s);
     else launch_few<T, 4>(a, s);
 }
-template <class T>
+template <class T, int PP>
 static void adapter_first(const AdapterGradArgs& a, hipStream_t s) {
     const int64_t blocks = a.ps.items * ceil_div(a.N, 64) + ceil_div(a.ps.slots * (a.ldp / 8), 1024);
     VH_REQUIRE(blocks < (int64_t(1) << 31), "too many rows for one launch");
-    adapter_first_kernel<T><<<(unsigned)blocks, 256, 0, s>>>(a);
+    adapter_first_kernel<T, PP><<<(unsigned)blocks, 256, 0, s>>>(a);
     VH_HIP(hipGetLastError());
 }
-template <class T, int RT>
+template <class T, int RT, int PP>
 static void adapter_grads_rank(const AdapterGradArgs& a, hipStream_t s) {
     // Few waves (up to 4096: a quarter of what the chip holds): the workgroup's four share a tile's rows, so that a group's rows are four
     // round trips fewer.  Many: a wave a tile, nothing to add up.  (200 groups, 8192 rows, K = N = 512: 20 us against 28)
     const int64_t tiles = ceil_div(a.K, 128) + ceil_div(a.N, 128);
-    if (a.ps.items * tiles < 4096) adapter_grad_kernel<T, RT, 2, 4><<<dim3((unsigned)a.ps.items, (unsigned)tiles), 256, 0, s>>>(a);
-    else adapter_grad_kernel<T, RT, 2, 1><<<dim3((unsigned)a.ps.items, (unsigned)ceil_div(tiles, 4)), 256, 0, s>>>(a);
+    if (a.ps.items * tiles < 4096) adapter_grad_kernel<T, RT, 2, 4, PP><<<dim3((unsigned)a.ps.items, (unsigned)tiles), 256, 0, s>>>(a);
+    else adapter_grad_kernel<T, RT, 2, 1, PP><<<dim3((unsigned)a.ps.items, (unsigned)ceil_div(tiles, 4)), 256, 0, s>>>(a);
     VH_HIP(hipGetLastError());
 }
-template <class T>
+template <class T, int PP>
 static void adapter_grads(const AdapterGradArgs& a, hipStream_t s) {
-    if (a.rank <= 16) adapter_grads_rank<T, 1>(a, s);
-    else if (a.rank <= 32) adapter_grads_rank<T, 2>(a, s);
-    else adapter_grads_rank<T, 4>(a, s);
+    if (a.rank <= 16) adapter_grads_rank<T, 1, PP>(a, s);
+    else if (a.rank <= 32) adapter_grads_rank<T, 2, PP>(a, s);
+    else adapter_grads_rank<T, 4, PP>(a, s);
     if (a.ps.rows > a.ps.item_rows) {
         const int64_t multis = a.ps.rows / a.ps.item_rows < a.ps.groups ? a.ps.rows / a.ps.item_rows : a.ps.groups;
         adapter_join_kernel<T><<<dim3((unsigned)ceil_div((int64_t)a.rank * (a.K + a.N), 256), (unsigned)multis), 256, 0, s>>>(a);
@@ -1158,7 +1155,7 @@ struct BackwardScratch {
 };
 static BackwardScratch backward_scratch(const PlanShape& ps, int64_t n, int64_t k, int64_t rank, int dtype) {
     BackwardScratch b{};
-    const int64_t es = dtype == VH_BF16 ? 2 : 4, planes = dtype == VH_BF16 ? 1 : 3;
+    const int64_t es = dtype == VH_BF16 ? 2 : 4, planes = dtype == VH_BF16 ? 2 : 3;   // (bf16 without an activation: one, of two)
     b.ldp = round_up(n, 8);
     b.turned = round_up(ps.rows * rank, 4);
     b.p = b.turned + round_up(ps.groups * rank * b.ldp * es / 4, 4);
@@ -1409,14 +1406,21 @@ int vh_adapt_backward(const vh_adapt_layer* l, const void* dy, int64_t lddy, con
         a.ldy = lddx;
         a.plan = plan;
         a.ps = ps;
-        if (l->dtype == VH_BF16) {
-            adapter_first<bf16_t>(g, s);
-            launch_linear_bf16(a, true, s);
-            adapter_grads<bf16_t>(g, s);
-        } else {
-            adapter_first<float>(g, s);
+        if (l->dtype == VH_F32) {
+            a.x_planes = 3;
+            adapter_first<float, 3>(g, s);
             launch_linear_f32(a, true, s);
-            adapter_grads<float>(g, s);
+            adapter_grads<float, 3>(g, s);
+        } else if (mask.p != nullptr) {
+            a.x_planes = 2;
+            adapter_first<bf16_t, 2>(g, s);
+            launch_linear_bf16(a, true, s);
+            adapter_grads<bf16_t, 2>(g, s);
+        } else {
+            a.x_planes = 1;
+            adapter_first<bf16_t, 1>(g, s);
+            launch_linear_bf16(a, true, s);
+            adapter_grads<bf16_t, 1>(g, s);
         }
     });
 }

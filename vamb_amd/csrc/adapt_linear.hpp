@@ -89,7 +89,8 @@ struct Shape {
     static constexpr int WM = WM_, WN = WN_, MS = MS_, NT = NT_, BK = BK_, KG = KG_;
 };
 
-template <class T, class S, int RT, bool TRANS, bool DMA>
+// XP: operand planes of x (backward: of p, which for bf16 tensors has two where a slope was applied)
+template <class T, class S, int RT, bool TRANS, bool DMA, int XP>
 __global__ __launch_bounds__(64 * S::WM * S::WN * S::KG) void linear_kernel(LinArgs a) {
     constexpr int WM = S::WM, WN = S::WN, MS = S::MS, NT = S::NT, NW = WM * WN, THREADS = 64 * NW, KG = S::KG;
     constexpr int P = Elem<T>::planes;
@@ -97,13 +98,13 @@ __global__ __launch_bounds__(64 * S::WM * S::WN * S::KG) void linear_kernel(LinA
     constexpr int CH = BK / 8;                          // 16-byte pieces of a tile row
     constexpr int BM = 16 * MS * WM, BN = 16 * NT * WN;
     constexpr int XB = BM * BK * 2, WB = BN * BK * 2;   // bytes of a plane
-    constexpr int BUF = P * (XB + WB);
+    constexpr int BUF = XP * XB + P * WB;
     constexpr int PX = BM * CH / THREADS;               // x pieces per thread (and plane)
     constexpr int NWI = P * BN * CH / 64;               // W pieces, one wave instruction each
     constexpr int QW = NWI ? (NWI + NW - 1) / NW : 1;
     constexpr int KC = BK / 32;                         // 32-deep products per tile
     constexpr int MU = MS / WN;                         // subtiles whose u this wave computes (its share of the WN waves on the same rows)
-    static_assert(PX >= 1 && BM * CH % THREADS == 0 && MS % WN == 0 && (!DMA || TRANS || P == 1) && (!TRANS || DMA), "tile shape");
+    static_assert(PX >= 1 && BM * CH % THREADS == 0 && MS % WN == 0 && (!DMA || TRANS || P == 1) && (!TRANS || DMA) && (TRANS || XP == P), "tile shape");
     static_assert(CH == 4 || CH == 8, "the piece permutations are for these");
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
 
@@ -132,9 +133,9 @@ __global__ __launch_bounds__(64 * S::WM * S::WN * S::KG) void linear_kernel(LinA
     const T* x_src[PX];
     int x_k[PX], rids[PX];
     unsigned x_off[PX];
-    Buffer x_buf[P];
+    Buffer x_buf[XP];
 #pragma unroll
-    for (int p = 0; p < P; ++p) {
+    for (int p = 0; p < XP; ++p) {
         if constexpr (TRANS) {
             // the tile's slots follow each other: its own buffer per plane (BM * 2^20 * 2 bytes at most), which ends with the slots
             const int64_t at = (int64_t)tile * BM, left = (a.ps.slots - at) * a.ldx * 2;
@@ -187,7 +188,7 @@ __global__ __launch_bounds__(64 * S::WM * S::WN * S::KG) void linear_kernel(LinA
     auto fetch_x = [&](auto whole, int k0, unsigned char* buf) {
         if constexpr (DMA) {
 #pragma unroll
-            for (int p = 0; p < P; ++p)
+            for (int p = 0; p < XP; ++p)
 #pragma unroll
                 for (int q = 0; q < PX; ++q) {
                     const int k = k0 + x_k[q];
@@ -269,38 +270,40 @@ __global__ __launch_bounds__(64 * S::WM * S::WN * S::KG) void linear_kernel(LinA
         for (int j = 0; j < RT; ++j) low[m][j] = f32x4{0, 0, 0, 0};
 
     auto compute = [&](const unsigned char* xb, const Raw8<T> (&in)[MU][KC][RT]) {
-        const unsigned char* const wb = xb + P * XB;
+        const unsigned char* const wb = xb + XP * XB;
         if constexpr (P == 1 && MS == 1 && NT > 0) {
-            // one product per operand that is read: all reads of the tile go ahead of the products
-            s16x8 xa[KC], wa[KC][NT];
+            // one or two products per operand that is read: all reads of the tile go ahead of the products
+            s16x8 xa[KC][XP], wa[KC][NT][1];
 #pragma unroll
             for (int c = 0; c < KC; ++c) {
                 const int xrow = wm * 16 + l15;
-                xa[c] = *reinterpret_cast<const s16x8*>(xb + (xrow * CH + ((4 * c + quad) ^ swz(xrow))) * 16);
+#pragma unroll
+                for (int p = 0; p < XP; ++p)
+                    xa[c][p] = *reinterpret_cast<const s16x8*>(xb + p * XB + (xrow * CH + ((4 * c + quad) ^ swz(xrow))) * 16);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     const int row = wn * NT * 16 + w_row(n);
-                    wa[c][n] = *reinterpret_cast<const s16x8*>(wb + (row * CH + ((4 * c + quad) ^ swz_w(row))) * 16);
+                    wa[c][n][0] = *reinterpret_cast<const s16x8*>(wb + (row * CH + ((4 * c + quad) ^ swz_w(row))) * 16);
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int c = 0; c < KC; ++c) {
 #pragma unroll
-                for (int n = 0; n < NT; ++n) acc[0][n] = mfma32(wa[c][n], xa[c], acc[0][n]);
+                for (int n = 0; n < NT; ++n) acc[0][n] = mma(wa[c][n], xa[c], acc[0][n]);
 #pragma unroll
-                for (int j = 0; j < RT; ++j) low[0][j] = mfma32(to_planes(in[0][c][j]).p[0], xa[c], low[0][j]);
+                for (int j = 0; j < RT; ++j) low[0][j] = mma(to_planes(in[0][c][j]).p, xa[c], low[0][j]);
             }
             return;
         }
 #pragma unroll
         for (int c = 0; c < KC; ++c) {
-            s16x8 xf[MS][P];
+            s16x8 xf[MS][XP];
 #pragma unroll
             for (int m = 0; m < MS; ++m) {
                 const int row = (wm * MS + m) * 16 + l15;
 #pragma unroll
-                for (int p = 0; p < P; ++p)
+                for (int p = 0; p < XP; ++p)
                     xf[m][p] = *reinterpret_cast<const s16x8*>(xb + p * XB + (row * CH + ((4 * c + quad) ^ swz(row))) * 16);
             }
 #pragma unroll
@@ -339,7 +342,7 @@ __global__ __launch_bounds__(64 * S::WM * S::WN * S::KG) void linear_kernel(LinA
             fetch_in(No(), k0, in);
             fetch_x(No(), k0, to);
         }
-        fetch_w(k0, to + P * XB);
+        fetch_w(k0, to + XP * XB);
     };
     if (kg < nk) {
         fetch(kg * BK, tiles, in0);
@@ -537,43 +540,44 @@ __global__ __launch_bounds__(64 * S::WM * S::WN * S::KG) void linear_kernel(LinA
     }
 }
 
-template <class T, class S, int RT, bool TRANS, bool DMA>
+template <class T, class S, int RT, bool TRANS, bool DMA, int XP>
 void launch_one(const LinArgs& a, hipStream_t s) {
     constexpr int P = Elem<T>::planes, BK = S::BK, BM = 16 * S::MS * S::WM, BN = 16 * S::NT * S::WN;
-    constexpr int bytes = S::KG * 2 * P * (BM + BN) * BK * 2;
+    constexpr int bytes = S::KG * 2 * (XP * BM + P * BN) * BK * 2;
+    static_assert(bytes <= 160 * 1024, "the LDS of a CU");
     if constexpr (bytes > 65536) {   // per device, cheap, and valid while a stream is captured
-        VH_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(linear_kernel<T, S, RT, TRANS, DMA>),
+        VH_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(linear_kernel<T, S, RT, TRANS, DMA, XP>),
                                    hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
     }
     const int64_t row_tiles = ceil_div(a.ps.subs, S::MS * S::WM), col_tiles = S::NT ? ceil_div(a.N, BN ? BN : 1) : 1;
     const int64_t blocks = round_up(row_tiles, 8) * col_tiles;
     VH_REQUIRE(blocks < (int64_t(1) << 31), "too many rows for one launch");
-    linear_kernel<T, S, RT, TRANS, DMA><<<dim3((unsigned)blocks), 64 * S::WM * S::WN * S::KG, bytes, s>>>(a);
+    linear_kernel<T, S, RT, TRANS, DMA, XP><<<dim3((unsigned)blocks), 64 * S::WM * S::WN * S::KG, bytes, s>>>(a);
     VH_HIP(hipGetLastError());
 }
 
-template <class T, int RT, bool TRANS, bool DMA>
+template <class T, int RT, bool TRANS, bool DMA, int XP>
 void launch_shape(const LinArgs& a, hipStream_t s) {
     constexpr bool F = Elem<T>::planes == 3;
     constexpr int BK = F ? 32 : 64;
     constexpr int KG = RT == 4 ? 2 : 4;   // (rank 33-64: the registers of 16 waves a CU are too few)
     if (a.y == nullptr) {
-        if constexpr (TRANS) launch_one<T, Shape<4, 1, 1, 0, BK, KG>, RT, TRANS, DMA>(a, s);
+        if constexpr (TRANS) launch_one<T, Shape<4, 1, 1, 0, BK, KG>, RT, TRANS, DMA, XP>(a, s);
         return;
     }
     // small grids, and the narrow latent layers
-    if (a.N <= 32 || ceil_div(a.ps.subs, 4) * ceil_div(a.N, 32) <= 1024) return launch_one<T, Shape<4, 1, 1, 2, BK, KG>, RT, TRANS, DMA>(a, s);
+    if (a.N <= 32 || ceil_div(a.ps.subs, 4) * ceil_div(a.N, 32) <= 1024) return launch_one<T, Shape<4, 1, 1, 2, BK, KG>, RT, TRANS, DMA, XP>(a, s);
     const int64_t big = ceil_div(a.ps.subs, F ? 8 : 16) * ceil_div(a.N, F ? 128 : 256);
-    if (big < 512 || a.N <= 128) return launch_one<T, Shape<4, 1, 1, 8, BK>, RT, TRANS, DMA>(a, s);
-    if constexpr (F) launch_one<T, Shape<4, 2, 2, 4, BK>, RT, TRANS, DMA>(a, s);
-    else if constexpr (RT == 1 && !TRANS) launch_one<T, Shape<4, 2, 4, 8, BK>, RT, TRANS, DMA>(a, s);
-    else launch_one<T, Shape<4, 2, 2, 8, BK>, RT, TRANS, DMA>(a, s);
+    if (big < 512 || a.N <= 128) return launch_one<T, Shape<4, 1, 1, 8, BK>, RT, TRANS, DMA, XP>(a, s);
+    if constexpr (F) launch_one<T, Shape<4, 2, 2, 4, BK>, RT, TRANS, DMA, XP>(a, s);
+    else if constexpr (RT == 1 && !TRANS) launch_one<T, Shape<4, 2, 4, 8, BK>, RT, TRANS, DMA, XP>(a, s);
+    else launch_one<T, Shape<4, 2, 2, 8, BK>, RT, TRANS, DMA, XP>(a, s);
 }
-template <class T, bool TRANS, bool DMA>
+template <class T, bool TRANS, bool DMA, int XP>
 void launch_rank(const LinArgs& a, hipStream_t s) {
-    if (a.rank <= 16) launch_shape<T, 1, TRANS, DMA>(a, s);
-    else if (a.rank <= 32) launch_shape<T, 2, TRANS, DMA>(a, s);
-    else launch_shape<T, 4, TRANS, DMA>(a, s);
+    if (a.rank <= 16) launch_shape<T, 1, TRANS, DMA, XP>(a, s);
+    else if (a.rank <= 32) launch_shape<T, 2, TRANS, DMA, XP>(a, s);
+    else launch_shape<T, 4, TRANS, DMA, XP>(a, s);
 }
 
 }  // namespace adapt
