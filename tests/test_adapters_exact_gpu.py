@@ -82,3 +82,14 @@ def test_a_slope_leaves_dy_more_bits_than_it_had(ad, slope, held):
     # dB of the first column = scale sum p u = scale pairs (slope - t)
     assert ((dup[0, 0].double() - SCALE * pairs * rest).abs() <= SCALE * pairs * tol).all()
     assert (dup[0, 1] == SCALE * pairs).all() and not dup[0, 2:].any()
+
+
+@pytest.mark.parametrize("held", [False, True])
+@pytest.mark.parametrize("slope", [0.01, 0.3])
+def test_weight_gradient_of_a_slope(ad, slope, held):
+    pairs, n, k, dy, y, x, t, rest = slope_case(ad, torch.bfloat16, slope)
+    dw, db = ad.checkpoint_weight_grad(dy, ad.checkpoint8(x), ad.checkpoint8(y) if held else y, slope)
+    tol = 2.0 ** -16 * slope + 2.0 ** -8 * abs(rest)
+    assert ((dw[0].double() - pairs * rest).abs() <= pairs * tol).all() and (dw[1] == pairs).all() and not dw[2:].any()
+    total = pairs * (float(np.float32(slope)) + t)      # the sum of p itself is of float32 values
+    assert abs(float(db[0]) - total) <= 2.0 ** -8 * total + 2 * pairs * 2.0 ** -24 * total and db[1] == pairs

@@ -425,19 +425,6 @@ __device__ __forceinline__ void store4(T* p, f32x4 v, int n) {
             if (i < n) p[i] = from_f<T>(v[i]);
     }
 }
-// eight values rounded to T
-template <class T>
-__device__ __forceinline__ Raw8<T> rounded8(const float (&f)[8]) {
-    Raw8<T> o;
-    if constexpr (sizeof(T) == 2) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o.v[e] = __builtin_bit_cast(unsigned, __builtin_convertvector(f32x2{f[2 * e], f[2 * e + 1]}, bfx2));
-    } else {
-        o.a = f32x4{f[0], f[1], f[2], f[3]};
-        o.b = f32x4{f[4], f[5], f[6], f[7]};
-    }
-    return o;
-}
 // f'(y) of eight columns applied to f
 template <class T>
 __device__ __forceinline__ void masked8(const Source& s, const Eight<T>& v, float slope, float (&f)[8]) {
@@ -833,7 +820,7 @@ __global__ __launch_bounds__(512) void few_kernel(FewArgs a) {
 // Gradient of the shared projection from checkpoints:  dW = p^T x  [N][K],  db = sum p  [N]
 // Tile 128 x 128, split over the rows; both operands are contracted along their slow dimension: row-major LDS tiles [64 rows][128
 // columns] read by the transposing LDS instruction.  x's values are exact in bf16 (one plane), so float32 dy costs three products, not
-// six.  8192 x 512 x 512 bf16: 19 us and 5 us for the join of 16 parts (eight steps of 0.6; the rest is the first
+// six, and bf16 dy one, or two where a slope was applied to it (cut8).  8192 x 512 x 512 bf16: 19 us and 5 us for the join of 16 parts (eight steps of 0.6; the rest is the first
 // loads, 64 KB of partial sums a workgroup and the launch); 4096 x 1104 x 512 float32: 31 us and 6 us.  256-byte tile rows: the
 // 32-byte pieces are XOR-permuted by the row so that the eight rows of half a read differ in their banks.
 // =====================================================================================================================
@@ -853,6 +840,7 @@ __device__ __forceinline__ s16x4 read_tr(const unsigned char* p) {
 __device__ __forceinline__ int tr_swz(int row) { return (row & 3) | ((row >> 1) & 4); }
 
 enum { kNoMask, kMaskElements, kMaskCodes };   // where f' comes from
+template <class T> constexpr int grad_planes(int mask) { return sizeof(T) == 4 ? 3 : mask == kNoMask ? 1 : 2; }
 
 // EVEN: N is a multiple of 8.  Which kind of tensor is read is part of the kernel's type: a load behind a branch, even a uniform one,
 // made every load in flight be waited for (8192 x 512 x 512, mask of codes: 1.5 us a step of 64 rows instead of 0.6)
@@ -861,7 +849,7 @@ __global__ __launch_bounds__(512) void weight_grad_kernel(WeightGradArgs a) {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     // (in an order that gives the tiles of a split to one XCD, whose L2 they would share: 32768 rows 45 us against 46, 8192 rows 26 against 24)
     const int split = (int)blockIdx.x / a.tiles, tile = (int)blockIdx.x % a.tiles, n0 = (tile / a.k_tiles) * 128, k0 = (tile % a.k_tiles) * 128;
-    constexpr int P = Elem<T>::planes, BR = 64, TB = BR * 256;   // smem: [2][P + 1][TB]: planes of p, then x
+    constexpr int P = grad_planes<T>(MASK), BR = 64, TB = BR * 256;   // smem: [2][P + 1][TB]: planes of p (cut8), then x
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l15 = lane & 15, quad = lane >> 4;
     const int64_t lo = split * a.split_rows, hi = min(lo + a.split_rows, a.rows);
     const int half = wave >> 2, wn = (wave >> 1) & 1, wk = wave & 1;   // waves 0-3 take rows 0-31 of a tile, waves 4-7 rows 32-63
@@ -895,25 +883,18 @@ __global__ __launch_bounds__(512) void weight_grad_kernel(WeightGradArgs a) {
                 t.pw[q].zero();
                 t.xw[q].code = u32x2{0, 0};
             }
-            Raw8<T> o = t.pw[q];
-            if (MASK != kNoMask || sums) {
-                float f[8];
+            float f[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) f[e] = t.pw[q].get(e);
-                if constexpr (MASK != kNoMask) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        if constexpr (MASK == kMaskCodes) f[e] *= slope_of(t.mw[q].code[e >> 2], e & 3, a.slope);
-                        else f[e] = t.me[q].get(e) > 0.f ? f[e] : f[e] * a.slope;
-                    }
-                    o = rounded8<T>(f);
-                }
-                if (sums) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) bsum[e] += f[e];
-                }
+            for (int e = 0; e < 8; ++e) {
+                f[e] = t.pw[q].get(e);
+                if constexpr (MASK == kMaskCodes) f[e] *= slope_of(t.mw[q].code[e >> 2], e & 3, a.slope);
+                if constexpr (MASK == kMaskElements) f[e] = t.me[q].get(e) > 0.f ? f[e] : f[e] * a.slope;
             }
-            const Planes8<T> pl = to_planes(o);
+            if (sums) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) bsum[e] += f[e];
+            }
+            const Cut8<P> pl = cut8<P>(f);
 #pragma unroll
             for (int p = 0; p < P; ++p) *reinterpret_cast<s16x8*>(buf + p * TB + at) = pl.p[p];
             const float scale = __uint_as_float(t.xw[q].exp << 23);
@@ -953,7 +934,7 @@ __global__ __launch_bounds__(512) void weight_grad_kernel(WeightGradArgs a) {
     unsigned char* const buf0 = smem;
     unsigned char* const buf1 = smem + (P + 1) * TB;
     // (rows behind the last one are read as the last and set to zero: every request is in bounds, and no branch is needed)
-    if constexpr (P == 1) {
+    if constexpr (sizeof(T) == 2) {
         fetch(lo, ahead[0]);
         fetch(lo + BR, ahead[1]);
         keep(buf0, lo, ahead[0]);
@@ -1129,7 +1110,7 @@ template <class T, int MASK, bool EVEN>
 static void launch_weight_grad(const WeightGradArgs& a, int splits, hipStream_t s) {
     const int64_t blocks = (int64_t)a.tiles * splits;
     VH_REQUIRE(blocks < (int64_t(1) << 31), "too many tiles for one launch");
-    constexpr int bytes = 2 * (Elem<T>::planes + 1) * 64 * 256;
+    constexpr int bytes = 2 * (grad_planes<T>(MASK) + 1) * 64 * 256;
     if constexpr (bytes > 65536)
         VH_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(weight_grad_kernel<T, MASK, EVEN>), hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
     weight_grad_kernel<T, MASK, EVEN><<<(unsigned)blocks, 512, bytes, s>>>(a);
