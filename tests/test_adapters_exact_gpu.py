@@ -93,3 +93,112 @@ def test_weight_gradient_of_a_slope(ad, slope, held):
     assert ((dw[0].double() - pairs * rest).abs() <= pairs * tol).all() and (dw[1] == pairs).all() and not dw[2:].any()
     total = pairs * (float(np.float32(slope)) + t)      # the sum of p itself is of float32 values
     assert abs(float(db[0]) - total) <= 2.0 ** -8 * total + 2 * pairs * 2.0 ** -24 * total and db[1] == pairs
+
+
+INF = float("inf")
+
+
+def positive(dtype, exact, rows=70, k=72, n=40, rank=3, groups=6):
+    """A layer all of whose numbers are positive (so that an infinity stays one in every sum that it enters) and, with `exact`, powers of two
+    (whose parts behind the first eight bits are zero).  Rows 10 and 11 are of group 2, rows 12 and 13 have no adapter."""
+    g = torch.Generator().manual_seed(5)
+
+    def t(*s):
+        z = torch.exp2(torch.randint(-3, 3, s, generator=g).float()) if exact else torch.rand(s, generator=g) + 0.25
+        return z.to("cuda", dtype)
+    of = torch.randint(0, groups, (rows,), generator=g, dtype=torch.int32)
+    of[10:12], of[12:14] = 2, -1
+    y = t(rows, n) * torch.where(torch.rand((rows, n), generator=g) < 0.5, -1.0, 1.0).to("cuda", dtype)
+    return dict(x=t(rows, k), w=t(n, k), b=t(n), down=t(groups, rank, k), up=t(groups, n, rank), dy=t(rows, n), y=y, low=t(rows, rank).float(), of=of.cuda())
+
+
+def forward_of(ad, c):
+    shared = ad.SharedProjection(c["w"], c["b"])
+    plan = ad.group_rows(c["of"], len(c["down"]))
+    y, low, _ = ad.adapted_linear_train(c["x"], shared, c["down"], c["up"], plan, SCALE, 0.01)
+    few = ad.adapted_linear(c["x"][8:24], shared, c["down"], c["up"], c["of"][8:24].contiguous(), SCALE, 0.01)     # (without a plan)
+    return {"y": y, "few": few, "low": low}
+
+
+def backward_of(ad, c, slope=0.01):
+    shared = ad.SharedProjection(c["w"], c["b"])
+    plan = ad.group_rows(c["of"], len(c["down"]))
+    out = ad.adapted_linear_backward(c["dy"], c["x"], c["y"], c["low"], shared, c["down"], c["up"], plan, SCALE, slope)
+    dw, db = ad.checkpoint_weight_grad(c["dy"], ad.checkpoint8(torch.ones_like(c["x"])), c["y"] if slope is not None else None, slope)
+    return dict(zip(("dx", "ddown", "dup"), out), dw=dw, db=db)
+
+
+def check(got, clean, want):
+    """Every result is the clean one, bit for bit, but for what `want` says: {name: index of the elements that are +infinity}."""
+    for name, z in clean.items():
+        z = z.clone()
+        for at in want.get(name, ()):
+            z[at] = INF
+        bad = ~((got[name] == z) | (torch.isnan(got[name]) & torch.isnan(z)))
+        assert not bad.any(), f"{name}: {int(bad.sum())} of {bad.numel()} off, such as {got[name][bad][:3].tolist()} for {z[bad][:3].tolist()}"
+
+
+def run_infinities(ad, dtype, exact, places, slope=0.01):
+    """Infinities at `places`, {tensor: index}: what they reach is infinite in the formulas, and nothing else is touched."""
+    c = positive(dtype, exact)
+    forward, backward = forward_of(ad, c), backward_of(ad, c, slope)
+    c = {k: v.clone() for k, v in c.items()}
+    of = c["of"].cpu()
+    fw, bw = {k: [] for k in forward}, {k: [] for k in backward}
+
+    def reach(rows, cols):      # of y
+        fw["y"].append((rows, cols))
+        few = [int(r) - 8 for r in torch.arange(len(of))[rows].tolist() if 8 <= r < 24]
+        fw["few"].append((few, cols))
+    every = slice(None)
+    for name, at in places.items():
+        c[name][at] = INF
+        if name == "x":
+            r, k = at
+            reach([r], every)
+            bw["dx"] += []
+            if of[r] >= 0:
+                fw["low"].append((r,))
+                bw["ddown"].append((int(of[r]), every, k))
+        elif name == "w":
+            reach(slice(0, len(of)), at[0])
+            bw["dx"].append((every, at[1]))
+        elif name == "b":
+            reach(slice(0, len(of)), at[0])
+        elif name == "down":
+            rows = torch.nonzero(of == at[0])[:, 0]
+            fw["low"].append((rows, at[1]))
+            reach(rows, every)
+            bw["dx"].append((rows, at[2]))
+        elif name == "up":
+            rows = torch.nonzero(of == at[0])[:, 0]
+            reach(rows, at[1])
+            bw["dx"].append((rows, every))
+            bw["ddown"].append((at[0], at[2]))
+        elif name == "dy":
+            bw["dx"].append((at[0], every))
+            bw["dw"].append((at[1], every))
+            bw["db"].append((at[1],))
+            if of[at[0]] >= 0:
+                bw["ddown"].append((int(of[at[0]]),))
+                bw["dup"].append((int(of[at[0]]), at[1]))
+        elif name == "low":
+            if of[at[0]] >= 0:
+                bw["dup"].append((int(of[at[0]]), every, at[1]))
+    check(forward_of(ad, c), forward, fw)
+    check(backward_of(ad, c, slope), backward, bw)
+
+
+@pytest.mark.parametrize("exact", [False, True])
+@pytest.mark.parametrize("slope", [0.01, None])
+@pytest.mark.parametrize("places", [{"x": (10, 3)}, {"x": (13, 3)}, {"dy": (10, 3)}, {"dy": (12, 5)}, {"b": (5,)}, {"low": (11, 2)}], ids=str)
+def test_an_infinity_of_a_bf16_row(ad, places, slope, exact):
+    """Ranks that end inside a tile, and rows without an adapter: the zeros that stand there do not meet the row's infinity."""
+    run_infinities(ad, torch.bfloat16, exact, places, slope)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_rows_without_an_adapter_have_no_low_product(ad, dtype):
+    c = positive(dtype, False)
+    c["x"][12, 3], c["x"][13, 5] = INF, float("nan")
+    assert not forward_of(ad, c)["low"][12:14].any()

@@ -416,6 +416,9 @@ __global__ __launch_bounds__(64 * S::WM * S::WN * S::KG) void linear_kernel(LinA
         for (int j = 0; j < RT; ++j) {
             if constexpr (WN > 1) lo[j] = *reinterpret_cast<const f32x4*>(lows + ((wm * MS + m) * 16 + l15) * LS + 16 * j + 4 * quad);
             else lo[j] = low[m][j];
+            // behind the rank, and in a row without an adapter, stand products with zeros: zero, but NaN where the row holds an infinity or a NaN
+#pragma unroll
+            for (int i = 0; i < 4; ++i) lo[j][i] = g >= 0 && 16 * j + 4 * quad + i < r ? lo[j][i] : 0.f;
         }
         if (a.low != nullptr && n0 == 0 && wn == 0 && rid >= 0) {
 #pragma unroll
