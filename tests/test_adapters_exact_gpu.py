@@ -202,3 +202,30 @@ def test_rows_without_an_adapter_have_no_low_product(ad, dtype):
     c = positive(dtype, False)
     c["x"][12, 3], c["x"][13, 5] = INF, float("nan")
     assert not forward_of(ad, c)["low"][12:14].any()
+
+
+PLACES = [{"x": (10, 3)}, {"x": (13, 3)}, {"dy": (10, 3)}, {"dy": (12, 5)}, {"w": (5, 3)}, {"b": (5,)}, {"down": (2, 1, 3)}, {"up": (2, 5, 1)}, {"low": (11, 2)},
+          {"x": (10, 3), "w": (5, 3)}, {"x": (10, 3), "down": (2, 1, 3)}, {"dy": (10, 3), "w": (3, 5)}, {"dy": (10, 3), "up": (2, 3, 1)}, {"down": (2, 1, 3), "up": (2, 5, 1)}]
+
+
+@pytest.mark.parametrize("exact", [False, True])
+@pytest.mark.parametrize("slope", [0.01, None])
+@pytest.mark.parametrize("places", PLACES, ids=str)
+def test_an_infinity_of_float32(ad, places, slope, exact):
+    """An infinity in any tensor, and two that meet: infinities where the formulas have them, no NaN; numbers whose later cuts are zero too."""
+    run_infinities(ad, torch.float32, exact, places, slope)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_signs_and_zeros_beside_an_infinity(ad, dtype):
+    """-inf, an infinity times zero (NaN in the formula) and two infinities of unlike sign (NaN)."""
+    c = positive(dtype, True)
+    rows = [10, 12]
+    c["x"][rows, 3], c["w"][7, 3] = -INF, 0.0
+    c["b"][:] = 0.0
+    got = forward_of(ad, c)
+    assert torch.isnan(got["y"][rows, 7]).all()
+    rest = [i for i in range(40) if i != 7]
+    assert (got["y"][rows][:, rest] == -INF).all() and (got["low"][10] == -INF).all()
+    c["x"][rows, 9] = INF
+    assert torch.isnan(forward_of(ad, c)["y"][rows]).all()

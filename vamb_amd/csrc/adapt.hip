@@ -894,7 +894,7 @@ __global__ __launch_bounds__(512) void weight_grad_kernel(WeightGradArgs a) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) bsum[e] += f[e];
             }
-            const Cut8<P> pl = cut8<P>(f);
+            const Cut8<P> pl = cut8<P, true>(f);   // (x holds no infinities)
 #pragma unroll
             for (int p = 0; p < P; ++p) *reinterpret_cast<s16x8*>(buf + p * TB + at) = pl.p[p];
             const float scale = __uint_as_float(t.xw[q].exp << 23);
