@@ -216,6 +216,14 @@ def test_an_infinity_of_float32(ad, places, slope, exact):
     run_infinities(ad, torch.float32, exact, places, slope)
 
 
+@pytest.mark.parametrize("exact", [False, True])
+@pytest.mark.parametrize("slope", [0.01, 0.5, None])
+@pytest.mark.parametrize("places", PLACES, ids=str)
+def test_an_infinity_of_bf16(ad, places, slope, exact):
+    """bf16 weights and adapters are one plane, u, v and a masked p several, whose later ones are often zero."""
+    run_infinities(ad, torch.bfloat16, exact, places, slope)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_signs_and_zeros_beside_an_infinity(ad, dtype):
     """-inf, an infinity times zero (NaN in the formula) and two infinities of unlike sign (NaN)."""

@@ -118,6 +118,14 @@ __device__ __forceinline__ void split3(float x, unsigned& h, unsigned& m, unsign
     l = __float_as_uint(q);
 }
 
+// A number's later cut beside an operand of ONE plane, which may hold infinities itself: never zero but for zero, so that the product with an
+// infinity is one of the number's sign in every cut.  `tiny` (of `x`'s sign, 2^-126) stands for a zero; it is 2^-25 of x at most: numbers
+// below 2^-100 keep their zeros (and make a NaN of an infinity, as if they were zero).  The cut has x's sign or is zero.
+__device__ __forceinline__ unsigned tiny_of(float x) {
+    return fabsf(x) >= 0x1p-100f ? (__float_as_uint(x) & 0x80000000u) | 0x00800000u : 0u;   // (a NaN: 0)
+}
+__device__ __forceinline__ unsigned not_zero(unsigned cut, unsigned tiny) { return cut > tiny ? cut : tiny; }   // (bits of one sign: the larger)
+
 template <class T> struct Planes8 { s16x8 p[Elem<T>::planes]; };
 
 __device__ __forceinline__ Planes8<bf16_t> to_planes(const Raw8<bf16_t>& r) {
@@ -165,8 +173,9 @@ __device__ __forceinline__ Cut8<PP> cut8(const float (&f)[8]) {
             const unsigned b = __float_as_uint(f[e]);
             o.p[0][e] = (short)(b >> 16);
             if constexpr (PP == 2) {
-                const float r = f[e] - __uint_as_float(b & 0xffff0000u);
-                o.p[1][e] = (short)f_to_bf(__builtin_isinf(f[e]) ? 0.f : r);
+                const float r = __builtin_isinf(f[e]) ? 0.f : f[e] - __uint_as_float(b & 0xffff0000u);
+                const unsigned low = (unsigned)f_to_bf(r) << 16;
+                o.p[1][e] = (short)((WHOLE ? low : not_zero(low, tiny_of(f[e]))) >> 16);
             }
         }
     }

@@ -38,13 +38,22 @@ __device__ __forceinline__ void dma16(Buffer b, unsigned offset, unsigned char* 
 constexpr unsigned kBehind = 0xfffffff0u;   // behind every buffer (their sizes are below it)
 static __device__ const uint4 g_zero32[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
 
+// ALONE: beside an operand of one plane, which may hold infinities
+template <bool ALONE>
 __device__ __forceinline__ void cut4(const f32x4 v, s16x4 (&o)[3]) {
     unsigned w[3][2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
         unsigned h0, m0, l0, h1, m1, l1;
-        split3(v[2 * e], h0, m0, l0);
-        split3(v[2 * e + 1], h1, m1, l1);
+        split3<ALONE>(v[2 * e], h0, m0, l0);
+        split3<ALONE>(v[2 * e + 1], h1, m1, l1);
+        if constexpr (ALONE) {
+            const unsigned t0 = tiny_of(v[2 * e]), t1 = tiny_of(v[2 * e + 1]);
+            m0 = not_zero(m0, t0);
+            l0 = not_zero(l0, t0);
+            m1 = not_zero(m1, t1);
+            l1 = not_zero(l1, t1);
+        }
         w[0][e] = (h0 >> 16) | (h1 & 0xffff0000u);
         w[1][e] = (m0 >> 16) | (m1 & 0xffff0000u);
         w[2][e] = (l0 >> 16) | (l1 & 0xffff0000u);
@@ -75,7 +84,7 @@ __device__ __forceinline__ void load4(const float* p, int64_t stride, int valid,
     for (int i = 0; i < 4; ++i) o[i] = *(VH_GLOBAL(float, i < valid ? p + i * stride : (const float*)g_zero32));
 }
 __device__ __forceinline__ void planes4(const u32x2& r, s16x4 (&o)[1]) { o[0] = __builtin_bit_cast(s16x4, r); }
-__device__ __forceinline__ void planes4(const f32x4& r, s16x4 (&o)[3]) { cut4(r, o); }
+__device__ __forceinline__ void planes4(const f32x4& r, s16x4 (&o)[3]) { cut4<false>(r, o); }
 typedef short tr_s16x4 __attribute__((ext_vector_type(4)));
 template <class T> struct Raw4;
 template <> struct Raw4<bf16_t> { typedef u32x2 type; };
@@ -477,7 +486,7 @@ __global__ __launch_bounds__(64 * S::WM * S::WN * S::KG) void linear_kernel(LinA
 #pragma unroll
                 for (int j = 0; j < RT; ++j) {
                     s16x4 uf[3];
-                    cut4(lo[j] * a.scale, uf);
+                    cut4<P == 1>(lo[j] * a.scale, uf);
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
                         s16x4 op[P];
