@@ -237,3 +237,16 @@ def test_signs_and_zeros_beside_an_infinity(ad, dtype):
     assert (got["y"][rows][:, rest] == -INF).all() and (got["low"][10] == -INF).all()
     c["x"][rows, 9] = INF
     assert torch.isnan(forward_of(ad, c)["y"][rows]).all()
+
+
+def test_encoding_with_adapters_that_require_a_gradient(ad):
+    """(a user's own optimiser may have set that): encoding gives none, and is not refused."""
+    from vamb_amd import encode
+    rng = np.random.default_rng(4)
+    loader = encode.make_dataloader(rng.random((40, 4)).astype(np.float32) + 0.1, rng.standard_normal((40, 103)).astype(np.float32),
+                                    rng.integers(2000, 9000, 40), batchsize=32, destroy=False)
+    a = encode.VAE(4, nhiddens=[32], nlatent=8, seed=1).adapters(3, rank=2)
+    want = a.encode(loader, np.arange(40) % 3)
+    for t in (*a.down, *a.up):
+        t.requires_grad_()
+    assert np.array_equal(a.encode(loader, np.arange(40) % 3), want)

@@ -205,3 +205,17 @@ def test_gradient_items_read_slots_that_exist(rows, groups):
                 if piece:
                     assert highest.value == first + at + piece - 1
             first += -(-count // 16) * 16
+
+
+@pytest.mark.parametrize("which", ["x", "down", "up"])
+def test_forward_refuses_what_asks_for_a_gradient(which):
+    """Its result would be cut off from autograd without a word."""
+    a = args()
+    a[which].requires_grad_()
+    with pytest.raises(ValueError, match="no gradients"):
+        ad.adapted_linear(**a)
+    with torch.no_grad(), pytest.raises(ValueError, match="on a GPU"):      # (past that check)
+        ad.adapted_linear(**a)
+    a[which] = a[which].detach()
+    with pytest.raises(ValueError, match="on a GPU"):
+        ad.adapted_linear(**a)

@@ -13,7 +13,8 @@ What the backward pass needs of the forward pass waits as a :class:`Checkpoint8`
 The functions take and return tensors of one GPU (float32 or bfloat16, all tensors of a call in one type; ``u`` is always float32), run on the current
 stream of that GPU, do not synchronise and may be captured into a graph.  Memory comes from torch's allocator, so a tensor (a plan, a
 packed weight, a checkpoint) that is used on another stream than the one that made it has to be ordered as any other
-tensor has.  They stand outside of autograd: gradients come from :func:`adapted_linear_backward` and :func:`checkpoint_weight_grad`.
+tensor has.  They stand outside of autograd: gradients come from :func:`adapted_linear_backward` and :func:`checkpoint_weight_grad`, for what
+:func:`adapted_linear_train` returns; :func:`adapted_linear`, which keeps nothing for them, refuses tensors that require a gradient.
 Sums are float32; gradients have the type of their parameters.  Equal inputs give equal bits.
 
 :class:`VAEAdapters` trains adapters for a VAE's encoder and encodes with them.
@@ -221,12 +222,16 @@ def adapted_linear(x, shared: SharedProjection, down, up, groups: Union[_torch.T
                    negative_slope: Optional[float] = None) -> _torch.Tensor:
     """``f(x W^T + b + scale u B_g^T)``, ``[rows, n]``: the layer with every row's own adapter.
 
-    ``groups``: an int32 tensor ``[rows]``, or the :class:`RowGroups` of these rows where several layers use it.  ``x`` may have any row stride."""
+    ``groups``: an int32 tensor ``[rows]``, or the :class:`RowGroups` of these rows where several layers use it.  ``x`` may have any row stride.
+    For inference: where autograd is on, tensors that require a gradient are refused (the result would have none)."""
     ld = _input(x, shared)
     rows = x.shape[0]
     planned = isinstance(groups, RowGroups)
     n_groups = groups.groups if planned else (down.shape[0] if isinstance(down, _torch.Tensor) and down.dim() == 3 else 0)
     layer = _layer(shared, down, up, n_groups, scale, negative_slope)
+    if _torch.is_grad_enabled() and (x.requires_grad or down.requires_grad or up.requires_grad):
+        raise ValueError("adapted_linear gives no gradients: call it under torch.no_grad() or on detached tensors, or use adapted_linear_train "
+                         "with adapted_linear_backward")
     if not planned:
         _check_groups(groups, n_groups)
     if (groups.rows if planned else groups.shape[0]) != rows:
@@ -542,6 +547,7 @@ class VAEAdapters:
         return _torch.where((g >= 0) & (g < self.n_groups), g, -1).to(_torch.int32)
 
     # ---- encode -----------------------------------------------------------------------------------------------------------------
+    @_torch.no_grad()
     def encode(self, data_loader, groups, batchsize: int = 262144):
         """Latents ``[n, nlatent]`` like ``VAE.encode`` (float32, the low 12 mantissa bits cleared, vambtools.py:324-330)."""
         if batchsize < 1:
