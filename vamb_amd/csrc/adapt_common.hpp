@@ -279,6 +279,17 @@ __host__ __device__ __forceinline__ int64_t item_slot(int first, int count, int 
 }
 enum { kPlanSubs = 0, kPlanItems = 1, kPlanMultis = 2, kPlanParts = 3 };
 
+// ---- which kernels a size takes (adapt_linear.hpp: launch_shape; adapt.hip: adapter_grads_rank) -------------------------------------
+enum { kTileNarrow, kTileMid, kTileWide };   // 64 rows x 32 columns, 64 x 128, and 128 (256) x 256 (float32: 128 x 128)
+inline int linear_tile(int64_t subs, int64_t n, int dtype_planes) {
+    const bool f32 = dtype_planes == 3;
+    if (n <= 32 || (subs + 3) / 4 * ((n + 31) / 32) <= 1024) return kTileNarrow;
+    const int64_t rows = f32 ? 8 : 16, cols = f32 ? 128 : 256;   // subtiles, columns
+    return n <= 128 || (subs + rows - 1) / rows * ((n + cols - 1) / cols) < 512 ? kTileMid : kTileWide;
+}
+// waves that share a tile of the adapters' gradients
+inline int grad_waves(const PlanShape& ps, int64_t n, int64_t k) { return ps.items * ((k + 127) / 128 + (n + 127) / 128) < 4096 ? 4 : 1; }
+
 // ---- arguments of the shared-projection kernel (adapt_linear.hpp) -----------------------------------------------------------------
 struct LinArgs {
     const void* x;            // forward: the layer's input [rows][ldx]; backward: p = dy f' as operand planes [planes][slots][ldx], in the plan's order

@@ -577,10 +577,9 @@ void launch_shape(const LinArgs& a, hipStream_t s) {
         if constexpr (TRANS) launch_one<T, Shape<4, 1, 1, 0, BK, KG>, RT, TRANS, DMA, XP>(a, s);
         return;
     }
-    // small grids, and the narrow latent layers
-    if (a.N <= 32 || ceil_div(a.ps.subs, 4) * ceil_div(a.N, 32) <= 1024) return launch_one<T, Shape<4, 1, 1, 2, BK, KG>, RT, TRANS, DMA, XP>(a, s);
-    const int64_t big = ceil_div(a.ps.subs, F ? 8 : 16) * ceil_div(a.N, F ? 128 : 256);
-    if (big < 512 || a.N <= 128) return launch_one<T, Shape<4, 1, 1, 8, BK>, RT, TRANS, DMA, XP>(a, s);
+    const int tile = linear_tile(a.ps.subs, a.N, Elem<T>::planes);
+    if (tile == kTileNarrow) return launch_one<T, Shape<4, 1, 1, 2, BK, KG>, RT, TRANS, DMA, XP>(a, s);
+    if (tile == kTileMid) return launch_one<T, Shape<4, 1, 1, 8, BK>, RT, TRANS, DMA, XP>(a, s);
     if constexpr (F) launch_one<T, Shape<4, 2, 2, 4, BK>, RT, TRANS, DMA, XP>(a, s);
     else if constexpr (RT == 1 && !TRANS) launch_one<T, Shape<4, 2, 4, 8, BK>, RT, TRANS, DMA, XP>(a, s);
     else launch_one<T, Shape<4, 2, 2, 8, BK>, RT, TRANS, DMA, XP>(a, s);
