@@ -27,13 +27,13 @@ def trained(samples, seed):
 
 def expected(a, weights, x, w, groups, noise, down, up, signs, held):
     """(loss, ddown, dup, dmu weight, dmu bias): weights [(W, b)] of encoder and decoder, signs [layer] what y > 0 was read as, held the
-    encoder layers' inputs as they were kept."""
+    encoder layers' inputs as they were kept (None: as they are)."""
     d = lambda t: t.detach().double().cpu()  # noqa: E731
     x, w, noise, groups = d(x), d(w), d(noise), groups.cpu().long()
     n_enc, rows, s = len(down), len(x), a.nsamples
     with_adapter = ((groups >= 0) & (groups < a.n_groups)).double()[:, None]
     at = groups.clamp(0, a.n_groups - 1)
-    h, us = x, []
+    h, us, ins = x, [], []
     for i, (W, b) in enumerate(weights):
         z = h @ d(W).t() + d(b)
         if i < n_enc:
@@ -41,12 +41,13 @@ def expected(a, weights, x, w, groups, noise, down, up, signs, held):
             u = torch.einsum("rjk,rk->rj", A, h) * with_adapter
             z = z + a.scale * torch.einsum("rnj,rj->rn", B, u)
             us.append(u)
+            ins.append(h)
         last = i in (n_enc - 1, len(weights) - 1)
         h = z if last else torch.where(signs[i], z, SLOPE * z)
         if i == n_enc - 1:
             mu = h
             h = h + noise
-    out = h
+    held, out = held or ins, h
     p = torch.softmax(out[:, :s], 1)
     wm = float(w.mean())
     ab, sse, kld = (1 - a.alpha) / s, a.alpha / 103, 1 / (a.nlatent * a.beta)
@@ -83,8 +84,8 @@ def expected(a, weights, x, w, groups, noise, down, up, signs, held):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("samples", [7, 1])
-def test_gradients_tensor_by_tensor(samples, dtype, monkeypatch):
+@pytest.mark.parametrize("samples,checkpoints", [(7, True), (1, True), (7, False)])
+def test_gradients_tensor_by_tensor(samples, checkpoints, dtype, monkeypatch):
     from vamb_amd import adapters as ad
     vae, loader, groups = trained(samples, 11)
     weights, held = [], []
@@ -103,7 +104,7 @@ def test_gradients_tensor_by_tensor(samples, dtype, monkeypatch):
         held.append(out[2])
         return out
     monkeypatch.setattr(ad.SharedProjection, "__init__", spy_init)
-    a = vae.adapters(5, rank=3, scale=0.5, dtype=dtype, seed=3)
+    a = vae.adapters(5, rank=3, scale=0.5, dtype=dtype, seed=3, **({} if checkpoints else {"checkpoints": False}))
     gen = torch.Generator(device="cuda").manual_seed(0)
     for u in a.up:
         u.copy_(0.3 * torch.randn(u.shape, generator=gen, device="cuda"))
@@ -117,13 +118,34 @@ def test_gradients_tensor_by_tensor(samples, dtype, monkeypatch):
     monkeypatch.setattr(ad, "checkpoint8", spy_keep)
     monkeypatch.setattr(ad, "adapted_linear_train", spy_train)
     loss, downs, ups, (dw, db) = a.gradients(x, w, of, noise, mu_too=True)
-    # held: the input, three layers of the encoder, the latent, three of the decoder
-    assert len(weights) == 6 and len(held) == 8
-    values = [h.restore().double().cpu() for h in held[:3]]
-    signs = [(h.codes[:, :h.columns] < 128).cpu() for h in held[1:4] + held[5:8]]
+    assert len(weights) == 6
+    if checkpoints:     # the input, three layers of the encoder, the latent, three of the decoder
+        assert len(held) == 8
+        values, held = [h.restore().double().cpu() for h in held[:3]], held[1:4] + held[5:8]
+    else:               # (the checkpoints that the layers' launches wrote, whose signs are those of the tensors that were kept)
+        assert len(held) == 6
+        values = None
+    signs = [(h.codes[:, :h.columns] < 128).cpu() for h in held]
     want_loss, ddown, dup, (mw, mb) = expected(a, weights, x, w, of, noise, a.down, a.up, signs, values)
     assert abs(float(loss) - want_loss) <= (1e-5 if dtype == torch.float32 else 2.0 ** -6) * abs(want_loss)
     found = {f"down {i}": (downs[i], ddown[i]) for i in range(3)} | {f"up {i}": (ups[i], dup[i]) for i in range(3)} | {"mu weight": (dw, mw), "mu bias": (db, mb)}
     off = {k: float((got.double().cpu() - want).norm() / want.norm()) for k, (got, want) in found.items()}
     assert all(want.norm() > 0 for _, want in found.values())
     assert max(off.values()) <= TOL[dtype], off
+
+
+def test_training_without_checkpoints():
+    from vamb_amd.adapters import VAEAdapters
+    import io
+    vae, loader, groups = trained(7, 12)
+    runs = []
+    for _ in range(2):
+        a = vae.adapters(5, rank=4, seed=2, checkpoints=False)
+        losses = a.train(loader, groups, nepochs=2, batchsize=256, mu_too=True)
+        runs.append((losses, a.encode(loader, groups), a))
+    assert np.isfinite(runs[0][0]).all() and runs[0][0] == runs[1][0] and np.array_equal(runs[0][1], runs[1][1])
+    f = io.BytesIO()
+    runs[0][2].save(f)
+    f.seek(0)
+    again = VAEAdapters.load(f, vae, checkpoints=False)
+    assert not again.checkpoints and np.array_equal(again.encode(loader, groups), runs[0][1])

@@ -465,12 +465,14 @@ class VAEAdapters:
     Every Linear of the encoder (the hidden layers and ``mu``) has an adapter of ``rank`` per group; the decoder is as it was trained.  The
     BatchNorm of a layer (eval mode, encode.py:264) is folded into the Linear behind it, so an adapter reads the layer's input in front of that BatchNorm.
     A new adapter changes nothing (``up`` is zero).  Arithmetic in ``dtype`` (default: the VAE's compute type), ``mu`` always
-    in float32; parameters and their optimiser (torch's Adam) in float32.  Activations wait for the backward pass as 8-bit checkpoints.
+    in float32; parameters and their optimiser (torch's Adam) in float32.  Activations wait for the backward pass as 8-bit checkpoints (a byte
+    each; the inputs in the gradients of ``down`` and of ``mu`` are then within 2^-4 of their values, whatever ``dtype`` is), or, with
+    ``checkpoints=False``, as they are.
 
     ``groups``: the sample of each contig of the data set, integers; a value outside ``[0, n_groups)`` stands for a contig without an adapter."""
 
     def __init__(self, vae, n_groups: int, rank: int = 8, scale: float = 1.0, seed: int = 0, dtype: Optional[_torch.dtype] = None,
-                 device: Union[str, _torch.device] = "cuda"):
+                 device: Union[str, _torch.device] = "cuda", checkpoints: bool = True):
         from . import encode as _encode
         if type(vae) is not _encode.VAE:
             raise ValueError("adapters are made for a plain VAE")
@@ -487,6 +489,7 @@ class VAEAdapters:
         self.nsamples, self.nlatent, self.alpha, self.beta = vae.nsamples, vae.nlatent, vae.alpha, vae.beta
         self.ntnf = vae.ntnf
         self.n_groups, self.rank, self.scale, self.dtype = n_groups, rank, float(scale), dtype
+        self.checkpoints = bool(checkpoints)
         device = _torch.device(device)
         self.device = _torch.device("cuda", _torch.cuda.current_device()) if device.type == "cuda" and device.index is None else device
         state = {k: v.double() for k, v in vae.state_dict().items()}
@@ -576,18 +579,24 @@ class VAEAdapters:
         plan, alone = group_rows(groups, self.n_groups), group_rows(_torch.full_like(groups, -1), 1)
         pairs = self._pairs()
         last = len(pairs) - 1
-        # forward: every layer leaves its input's checkpoint and its own (whose signs are the derivative)
-        h, held, low = x.to(self.dtype), [checkpoint8(x.to(self.dtype))], []
+        # forward: every layer leaves its input and its output (whose signs are the derivative), as checkpoints or as they are
+        h, held, low = x.to(self.dtype), [], []
+        c = checkpoint8(h) if self.checkpoints else None
         for i, (s, (d, u)) in enumerate(zip(self._encoder, pairs)):
-            h, l, c = adapted_linear_train(h.to(s.dtype), s, d, u, plan, self.scale, None if i == last else _SLOPE)
-            held.append(c)
+            below, h = c, h.to(s.dtype)
+            y, l, c = adapted_linear_train(h, s, d, u, plan, self.scale, None if i == last else _SLOPE)
+            held.append((below, c) if self.checkpoints else (h, y))
             low.append(l)
+            h = y
         mu = h
         h = (mu + noise).to(self.dtype)
-        kept = [checkpoint8(h)]
+        kept = []
+        c = checkpoint8(h) if self.checkpoints else None
         for i, (s, (d, u)) in enumerate(zip(self._decoder, self._none)):
-            h, zero, c = adapted_linear_train(h, s, d, u, alone, 0.0, None if i == len(self._decoder) - 1 else _SLOPE)
-            kept.append((c, zero))
+            below = c
+            y, zero, c = adapted_linear_train(h, s, d, u, alone, 0.0, None if i == len(self._decoder) - 1 else _SLOPE)
+            kept.append((below, c, zero) if self.checkpoints else (h, y, zero))
+            h = y
         out = h.float()
         # loss and its gradient
         ns, nt = self.nsamples, self.ntnf
@@ -611,8 +620,7 @@ class VAEAdapters:
         # backward
         dh = do.to(self.dtype)
         for i in range(len(self._decoder) - 1, -1, -1):
-            c, zero = kept[i + 1]
-            below = kept[i] if i == 0 else kept[i][0]
+            below, c, zero = kept[i]
             dh, _, _ = adapted_linear_backward(dh, below, c, zero, self._decoder[i], *self._none[i], alone, 0.0,
                                                None if i == len(self._decoder) - 1 else _SLOPE)
         dh = dh.float() + mu * (kld_w * per)
@@ -620,9 +628,10 @@ class VAEAdapters:
         for i in range(last, -1, -1):
             s, (d, u) = self._encoder[i], pairs[i]
             slope = None if i == last else _SLOPE
-            if i == last and mu_too:
-                shared = checkpoint_weight_grad(dh, held[i])
-            dh, dd, du = adapted_linear_backward(dh.to(s.dtype), held[i], held[i + 1], low[i], s, d, u, plan, self.scale, slope, need_dx=i > 0)
+            below, c = held[i]
+            if i == last and mu_too:   # (of tensors as they are: a product of nlatent columns, torch's)
+                shared = checkpoint_weight_grad(dh, below) if self.checkpoints else (dh.t() @ below, dh.sum(0))
+            dh, dd, du = adapted_linear_backward(dh.to(s.dtype), below, c, low[i], s, d, u, plan, self.scale, slope, need_dx=i > 0)
             downs[i], ups[i] = dd.float(), du.float()
         return loss, downs, ups, shared
 
@@ -668,10 +677,10 @@ class VAEAdapters:
                      "up": [t.cpu() for t in self.up], "mu": [self._mu_weight.cpu(), self._mu_bias.cpu()]}, file)
 
     @classmethod
-    def load(cls, file, vae, dtype: Optional[_torch.dtype] = None, device: Union[str, _torch.device] = "cuda"):
+    def load(cls, file, vae, dtype: Optional[_torch.dtype] = None, device: Union[str, _torch.device] = "cuda", checkpoints: bool = True):
         """Adapters that :meth:`save` wrote, on the VAE that they were made for."""
         d = _torch.load(file, map_location="cpu", weights_only=True)
-        self = cls(vae, d["n_groups"], d["rank"], d["scale"], dtype=dtype, device=device)
+        self = cls(vae, d["n_groups"], d["rank"], d["scale"], dtype=dtype, device=device, checkpoints=checkpoints)
         for mine, saved in ((self.down, d["down"]), (self.up, d["up"])):
             if [tuple(t.shape) for t in mine] != [tuple(t.shape) for t in saved]:
                 raise ValueError("the saved adapters do not match this VAE")
