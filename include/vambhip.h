@@ -495,7 +495,8 @@ int vh_vae_train_epoch_dp(vh_vae* h, const int64_t* perm, int64_t n_batches, int
  * into a graph.  Scratch memory is the caller's, 16-byte aligned and of the size that the *_size entry gives; calls that may run at the same
  * time need scratch of their own.  Tensors are float32 or bf16 (`dtype`), unit stride along a row, `ld*` elements between rows, any
  * alignment of the element type.  Widths up to 2^20, weights (padded to multiples of 256) below 4 GB in each
- * direction (bf16: 2 bytes, float32: 6 bytes an element), rows up to 2^30, ranks up to 64, groups up to 16384.
+ * direction (bf16: 2 bytes, float32: 6 bytes an element), rows up to 2^30, ranks up to 64, groups up to 16384.  A call whose work is more than
+ * one launch of 2^32 threads holds (2^28 float32 rows of 32 or of 512 columns, a weight gradient of 2^32 elements) is refused.
  * ============================================================================================= */
 enum { VH_F32 = 0, VH_BF16 = 1 };
 

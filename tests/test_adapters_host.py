@@ -219,3 +219,21 @@ def test_forward_refuses_what_asks_for_a_gradient(which):
     a[which] = a[which].detach()
     with pytest.raises(ValueError, match="on a GPU"):
         ad.adapted_linear(**a)
+
+
+def test_c_entries_refuse_what_no_launch_holds():
+    """Sizes within the documented limits whose launch would have 2^32 threads or more: an argument error, before any device work."""
+    lib = _lib.load()
+    some = 4096
+    for call, why in [
+        (lambda: lib.vh_adapt_forward(_lib.AdaptLayer(1, 0, 32, 8, 4, 1, some, some, some, 1.0, 0.0), some, 8, 2 ** 29, some, some, 32, None, None, None, None),
+         "rows"),
+        (lambda: lib.vh_adapt_forward(_lib.AdaptLayer(0, 0, 4096, 8, 40, 1, some, some, some, 1.0, 0.0), some, 8, 2 ** 28, some, some, 4096, None, None, None,
+                                      None), "rows"),
+        (lambda: lib.vh_adapt_backward(_lib.AdaptLayer(1, 0, 4096, 8, 4, 1, some, some, some, 1.0, 0.0), some, 4096, _lib.Held(some, 8, None, None), None,
+                                       some, 2 ** 26, some, some, 8, some, some, some, None), "rows"),
+        (lambda: lib.vh_checkpoint8_weight_grad(some, 2 ** 16, _lib.Held(None, 0, some, some), None, 0.0, 5, 2 ** 16, 2 ** 16, 1, some, None, some, None),
+         "gradient"),
+    ]:
+        with pytest.raises(ValueError, match=why + ".*one launch"):
+            _lib.check(call())

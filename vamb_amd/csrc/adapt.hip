@@ -1082,7 +1082,7 @@ static void few_rank(const FewArgs& a, hipStream_t s) {
 template <class T, int PP>
 static void adapter_first(const AdapterGradArgs& a, hipStream_t s) {
     const int64_t blocks = a.ps.items * ceil_div(a.N, 64) + ceil_div(a.ps.slots * (a.ldp / 8), 1024);
-    VH_REQUIRE(blocks < (int64_t(1) << 31), "too many rows for one launch");
+    VH_REQUIRE(fits_a_launch(blocks, 256), "%lld rows of %d columns are too many for one launch", (long long)a.ps.rows, a.N);
     adapter_first_kernel<T, PP><<<(unsigned)blocks, 256, 0, s>>>(a);
     VH_HIP(hipGetLastError());
 }
@@ -1109,7 +1109,7 @@ static void adapter_grads(const AdapterGradArgs& a, hipStream_t s) {
 template <class T, int MASK, bool EVEN>
 static void launch_weight_grad(const WeightGradArgs& a, int splits, hipStream_t s) {
     const int64_t blocks = (int64_t)a.tiles * splits;
-    VH_REQUIRE(blocks < (int64_t(1) << 31), "too many tiles for one launch");
+    VH_REQUIRE(fits_a_launch(blocks, 512), "a gradient of %d x %d is too large for one launch", a.N, a.K);
     constexpr int bytes = 2 * (grad_planes<T>(MASK) + 1) * 64 * 256;
     if constexpr (bytes > 65536)
         VH_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(weight_grad_kernel<T, MASK, EVEN>), hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
@@ -1123,10 +1123,11 @@ static void weight_grad_width(const WeightGradArgs& a, int splits, hipStream_t s
 }
 template <class T>
 static void weight_grad(const WeightGradArgs& a, int splits, void* dweight, void* dbias, hipStream_t s) {
+    const int64_t n_weight = (int64_t)a.N * a.K, total = n_weight + a.N;
+    VH_REQUIRE(fits_a_launch(ceil_div(total, 256), 256), "a gradient of %d x %d is too large for one launch", a.N, a.K);
     if (a.mask.p == nullptr) weight_grad_width<T, kNoMask>(a, splits, s);
     else if (a.mask.exps == nullptr) weight_grad_width<T, kMaskElements>(a, splits, s);
     else weight_grad_width<T, kMaskCodes>(a, splits, s);
-    const int64_t n_weight = (int64_t)a.N * a.K, total = n_weight + a.N;
     weight_join_kernel<T><<<(unsigned)ceil_div(total, 256), 256, 0, s>>>(a.parts, splits, n_weight, total, (T*)dweight, (T*)dbias);
     VH_HIP(hipGetLastError());
 }
@@ -1221,6 +1222,7 @@ int vh_adapt_weight_pack(const void* weight, int64_t ld, const void* bias, int64
         VH_REQUIRE((uintptr_t)packed % 16 == 0, "packed weight must be 16-byte aligned");
         const WeightShape ws = weight_shape(n, k, dtype);
         float* out_bias = reinterpret_cast<float*>((char*)packed + ws.bias_off);
+        VH_REQUIRE(fits_a_launch(ceil_div(ws.fwd + ws.bwd, 256), 256), "a weight of %lld x %lld is too large for one launch", (long long)n, (long long)k);
         const unsigned blocks = (unsigned)ceil_div(ws.fwd + ws.bwd, 256);
         if (dtype == VH_BF16)
             pack_weight_kernel<bf16_t><<<blocks, 256, 0, (hipStream_t)stream>>>((const bf16_t*)weight, ld, (const bf16_t*)bias, (int)n, (int)k,

@@ -317,6 +317,8 @@ struct LinArgs {
     int dma;                  // forward: x rows are 16-byte aligned, K is a multiple of 8 and x ends below 2^32 - 16 bytes: ...
     unsigned x_bytes;         // ... its size, as a buffer
 };
+// a launch has fewer than 2^32 threads
+inline bool fits_a_launch(int64_t blocks, int64_t threads) { return blocks * threads < (int64_t(1) << 32); }
 void launch_linear_bf16(const LinArgs& a, bool backward, hipStream_t s);
 void launch_linear_f32(const LinArgs& a, bool backward, hipStream_t s);
 

@@ -555,16 +555,16 @@ __global__ __launch_bounds__(64 * S::WM * S::WN * S::KG) void linear_kernel(LinA
 template <class T, class S, int RT, bool TRANS, bool DMA, int XP>
 void launch_one(const LinArgs& a, hipStream_t s) {
     constexpr int P = Elem<T>::planes, BK = S::BK, BM = 16 * S::MS * S::WM, BN = 16 * S::NT * S::WN;
-    constexpr int bytes = S::KG * 2 * (XP * BM + P * BN) * BK * 2;
+    constexpr int bytes = S::KG * 2 * (XP * BM + P * BN) * BK * 2, threads = 64 * S::WM * S::WN * S::KG;
     static_assert(bytes <= 160 * 1024, "the LDS of a CU");
+    const int64_t row_tiles = ceil_div(a.ps.subs, S::MS * S::WM), col_tiles = S::NT ? ceil_div(a.N, BN ? BN : 1) : 1;
+    const int64_t blocks = round_up(row_tiles, 8) * col_tiles;
+    VH_REQUIRE(fits_a_launch(blocks, threads), "%lld rows of %d columns are too many for one launch", (long long)a.ps.rows, a.N);
     if constexpr (bytes > 65536) {   // per device, cheap, and valid while a stream is captured
         VH_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(linear_kernel<T, S, RT, TRANS, DMA, XP>),
                                    hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
     }
-    const int64_t row_tiles = ceil_div(a.ps.subs, S::MS * S::WM), col_tiles = S::NT ? ceil_div(a.N, BN ? BN : 1) : 1;
-    const int64_t blocks = round_up(row_tiles, 8) * col_tiles;
-    VH_REQUIRE(blocks < (int64_t(1) << 31), "too many rows for one launch");
-    linear_kernel<T, S, RT, TRANS, DMA, XP><<<dim3((unsigned)blocks), 64 * S::WM * S::WN * S::KG, bytes, s>>>(a);
+    linear_kernel<T, S, RT, TRANS, DMA, XP><<<dim3((unsigned)blocks), threads, bytes, s>>>(a);
     VH_HIP(hipGetLastError());
 }
 
