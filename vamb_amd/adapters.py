@@ -279,7 +279,8 @@ def adapted_linear_train(x, shared: SharedProjection, down, up, groups: RowGroup
 
 def adapted_linear_backward(dy, x, y, low, shared: SharedProjection, down, up, groups: RowGroups, scale: float = 1.0,
                             negative_slope: Optional[float] = None, need_dx: bool = True):
-    """``(dx, ddown, dup)`` of :func:`adapted_linear_train`; ``dx`` is None with ``need_dx=False`` (a first layer).
+    """``(dx, ddown, dup)`` of :func:`adapted_linear_train`; ``dx`` is None with ``need_dx=False`` (a first layer), the
+    others are the same bits.
 
     ``x`` and ``y`` are the layer's input and output, as tensors or checkpoints (``y`` may be None without an activation: it gives
     the derivative); ``low`` is its ``u``.  The gradients of a group without rows are zero."""

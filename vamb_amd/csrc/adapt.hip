@@ -1419,9 +1419,8 @@ int vh_debug_adapt_choice(int64_t rows, int64_t groups, int64_t n, int64_t k, in
         check_ptr(backward_tile, "backward_tile");
         check_ptr(waves, "waves");
         const PlanShape ps = plan_shape(rows, groups);
-        const int planes = dtype == VH_BF16 ? 1 : 3;
-        *forward_tile = linear_tile(ps.subs, n, planes);
-        *backward_tile = linear_tile(ps.subs, k, planes);
+        *forward_tile = linear_tile(ps.subs, n, dtype == VH_F32);
+        *backward_tile = linear_tile(ps.subs, k, dtype == VH_F32);
         *waves = grad_waves(ps, n, k);
     });
 }

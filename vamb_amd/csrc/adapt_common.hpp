@@ -280,12 +280,17 @@ __host__ __device__ __forceinline__ int64_t item_slot(int first, int count, int 
 enum { kPlanSubs = 0, kPlanItems = 1, kPlanMultis = 2, kPlanParts = 3 };
 
 // ---- which kernels a size takes (adapt_linear.hpp: launch_shape; adapt.hip: adapter_grads_rank) -------------------------------------
-enum { kTileNarrow, kTileMid, kTileWide };   // 64 rows x 32 columns, 64 x 128, and 128 (256) x 256 (float32: 128 x 128)
-inline int linear_tile(int64_t subs, int64_t n, int dtype_planes) {
-    const bool f32 = dtype_planes == 3;
-    if (n <= 32 || (subs + 3) / 4 * ((n + 31) / 32) <= 1024) return kTileNarrow;
-    const int64_t rows = f32 ? 8 : 16, cols = f32 ? 128 : 256;   // subtiles, columns
-    return n <= 128 || (subs + rows - 1) / rows * ((n + cols - 1) / cols) < 512 ? kTileMid : kTileWide;
+// Tiles of the projection, kernel times in us.
+// Narrow against mid, 512 -> 512, rank 16, 4 groups: bf16 1024 rows (272 narrow workgroups) 11.8 / 11.8, 2048 rows (528) 17.2 / 11.9, 3800 rows
+// (960) 24 / 12; float32 22 / 27, 33 / 27, 46 / 28.  One narrow workgroup fills a CU's LDS, so that more than 256 and a few take turns.  Up to 32
+// columns three quarters of a mid tile are idle: 512 -> 32, 2048 rows bf16 6.6 / 10.7, float32 12 / 26; 131072 rows 53 / 47 and 115 / 160.
+// Mid against wide, bf16: 16000 rows 27.8 / 29.8 (rank 40: 44 / 32), 32768 rows (260 of the 256 x 256) 47.6 / 48.6 (93 / 79), 60000 rows 81 / 62 (152 / 117);
+// backward 57 / 57, 102 / 85.  float32 has no wide tile: 128 x 128 took 1.05 of the mid one's time in the mean, and 172 / 155 at 32768 rows.
+// Over 150 drawn layers, both directions, this choice takes 1.01 of the fastest tile's time in the mean and 1.36 at worst.
+enum { kTileNarrow, kTileMid, kTileWide };   // 64 rows x 32 columns, 64 x 128, and (bf16) 128 or 256 x 256
+inline int linear_tile(int64_t subs, int64_t n, bool f32) {
+    if (n <= 32 || (subs + 3) / 4 * ((n + 31) / 32) <= 320) return kTileNarrow;
+    return f32 || n <= 128 || (subs + 15) / 16 * ((n + 255) / 256) < 256 ? kTileMid : kTileWide;
 }
 // waves that share a tile of the adapters' gradients
 inline int grad_waves(const PlanShape& ps, int64_t n, int64_t k) { return ps.items * ((k + 127) / 128 + (n + 127) / 128) < 4096 ? 4 : 1; }

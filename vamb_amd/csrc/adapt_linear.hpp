@@ -573,16 +573,21 @@ void launch_shape(const LinArgs& a, hipStream_t s) {
     constexpr bool F = Elem<T>::planes == 3;
     constexpr int BK = F ? 32 : 64;
     constexpr int KG = RT == 4 ? 2 : 4;   // (rank 33-64: the registers of 16 waves a CU are too few)
-    if (a.y == nullptr) {
-        if constexpr (TRANS) launch_one<T, Shape<4, 1, 1, 0, BK, KG>, RT, TRANS, DMA, XP>(a, s);
+    const int tile = linear_tile(a.ps.subs, a.N, F);
+    if (a.y == nullptr) {   // (v in the order in which the tile with dx sums it: the adapters' gradients are the same bits with and without dx)
+        if constexpr (TRANS) {
+            if (tile == kTileNarrow) launch_one<T, Shape<4, 1, 1, 0, BK, KG>, RT, TRANS, DMA, XP>(a, s);
+            else launch_one<T, Shape<4, 1, 1, 0, BK, 1>, RT, TRANS, DMA, XP>(a, s);
+        }
         return;
     }
-    const int tile = linear_tile(a.ps.subs, a.N, Elem<T>::planes);
     if (tile == kTileNarrow) return launch_one<T, Shape<4, 1, 1, 2, BK, KG>, RT, TRANS, DMA, XP>(a, s);
     if (tile == kTileMid) return launch_one<T, Shape<4, 1, 1, 8, BK>, RT, TRANS, DMA, XP>(a, s);
-    if constexpr (F) launch_one<T, Shape<4, 2, 2, 4, BK>, RT, TRANS, DMA, XP>(a, s);
-    else if constexpr (RT == 1 && !TRANS) launch_one<T, Shape<4, 2, 4, 8, BK>, RT, TRANS, DMA, XP>(a, s);
-    else launch_one<T, Shape<4, 2, 2, 8, BK>, RT, TRANS, DMA, XP>(a, s);
+    if constexpr (!F) {   // 256 rows where the sums fit the registers (65536 rows 512 -> 512, rank 16: 83 us, 91 with 128 rows; rank 32: 183, it spills, 115)
+        // and the planes of p the LDS
+        if constexpr (RT == 1 && !TRANS) launch_one<T, Shape<4, 2, 4, 8, BK>, RT, TRANS, DMA, XP>(a, s);
+        else launch_one<T, Shape<4, 2, 2, 8, BK>, RT, TRANS, DMA, XP>(a, s);
+    }
 }
 template <class T, bool TRANS, bool DMA, int XP>
 void launch_rank(const LinArgs& a, hipStream_t s) {
