@@ -75,7 +75,8 @@ int vh_debug_adapt_item_reads(int64_t rows, int64_t groups, int32_t first, int32
 
 /* test hook (host only): which kernels the adapters' entries choose for a size.  Tiles of the projection, forward and backward: 0 = 64 x 32,
  * 1 = 64 x 128, 2 = the wide ones (bf16); waves: how many share a tile of the adapters' gradients (4 or 1) */
-int vh_debug_adapt_choice(int64_t rows, int64_t groups, int64_t n, int64_t k, int dtype, int* forward_tile, int* backward_tile, int* waves);
+int vh_debug_adapt_choice(int64_t rows, int64_t groups, int64_t n, int64_t k, int64_t rank, int dtype, int* forward_tile,
+                          int* backward_tile, int* waves);
 
 #ifdef __cplusplus
 }

@@ -26,10 +26,10 @@ def ad():
     return adapters
 
 
-def choice(rows, groups, n, k, dtype):
+def choice(rows, groups, n, k, rank, dtype):
     from vamb_amd import _lib
     out = [ctypes.c_int() for _ in range(3)]
-    _lib.check(_lib.load().vh_debug_adapt_choice(rows, groups, n, k, 0 if dtype == torch.float32 else 1, *out))
+    _lib.check(_lib.load().vh_debug_adapt_choice(rows, groups, n, k, rank, 0 if dtype == torch.float32 else 1, *out))
     return tuple(o.value for o in out)
 
 
@@ -44,16 +44,19 @@ def close(got, want, tol, what):
 
 # rows, k, n, rank, groups, dtype, forward tile, backward tile, waves of the gradients
 CASES = [
-    (3000, 154, 512, 40, 30, torch.bfloat16, MID, NARROW, 4),
-    (9001, 304, 200, 40, 60, torch.bfloat16, MID, MID, 4),
-    (70001, 300, 520, 24, 300, torch.bfloat16, WIDE, WIDE, 4),
-    (70001, 520, 300, 40, 300, torch.bfloat16, WIDE, WIDE, 4),
+    (3000, 154, 512, 20, 30, torch.bfloat16, MID, NARROW, 4),
+    (9001, 304, 200, 24, 60, torch.bfloat16, MID, MID, 4),
+    (9001, 200, 304, 40, 60, torch.bfloat16, MID, MID, 1),
+    (40001, 264, 264, 9, 20, torch.bfloat16, WIDE, WIDE, 1),
+    (70001, 300, 520, 24, 300, torch.bfloat16, WIDE, WIDE, 1),
+    (70001, 520, 300, 40, 300, torch.bfloat16, WIDE, WIDE, 1),
     (70001, 304, 512, 16, 700, torch.bfloat16, WIDE, WIDE, 1),
     (65537, 300, 520, 32, 900, torch.bfloat16, WIDE, WIDE, 1),
     (66000, 136, 264, 64, 1500, torch.bfloat16, WIDE, WIDE, 1),
-    (3000, 154, 512, 40, 30, torch.float32, MID, NARROW, 4),
-    (20001, 300, 520, 24, 200, torch.float32, MID, MID, 4),
-    (20001, 520, 300, 64, 200, torch.float32, MID, MID, 4),
+    (3000, 154, 512, 20, 30, torch.float32, MID, NARROW, 4),
+    (9001, 300, 200, 32, 60, torch.float32, MID, MID, 4),
+    (20001, 300, 520, 24, 200, torch.float32, MID, MID, 1),
+    (20001, 520, 300, 64, 200, torch.float32, MID, MID, 1),
     (30001, 300, 520, 33, 900, torch.float32, MID, MID, 1),
 ]
 
@@ -62,7 +65,7 @@ CASES = [
 @pytest.mark.parametrize("case", CASES, ids=lambda c: "-".join(str(x).replace("torch.", "") for x in c))
 def test_every_tile(ad, case, held):
     rows, k, n, rank, groups, dtype, *kernels = case
-    assert choice(rows, groups, n, k, dtype) == tuple(kernels)
+    assert choice(rows, groups, n, k, rank, dtype) == tuple(kernels)
     gen = torch.Generator(device="cuda").manual_seed(rows + rank)
     t = lambda *s: torch.randn(s, generator=gen, device="cuda").to(dtype)  # noqa: E731
     x, w, b, dy = t(rows, k), t(n, k) * k ** -0.5, t(n), t(rows, n)

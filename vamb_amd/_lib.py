@@ -179,7 +179,7 @@ SIGNATURES = {
     "vh_adapt_backward_size": (_int, [_i64, _i64, _i64, _i64, _i64, _int, ctypes.POINTER(_i64)]),
     "vh_adapt_backward": (_int, [ctypes.POINTER(AdaptLayer), _vp, _i64, ctypes.POINTER(Held), ctypes.POINTER(Held), _vp, _i64, _vp, _vp, _i64, _vp, _vp,
                                  _vp, _vp]),
-    "vh_debug_adapt_choice": (_int, [_i64, _i64, _i64, _i64, _int, ctypes.POINTER(_int), ctypes.POINTER(_int), ctypes.POINTER(_int)]),
+    "vh_debug_adapt_choice": (_int, [_i64, _i64, _i64, _i64, _i64, _int, ctypes.POINTER(_int), ctypes.POINTER(_int), ctypes.POINTER(_int)]),
     "vh_debug_adapt_item_reads": (_int, [_i64, _i64, ctypes.c_int32, ctypes.c_int32, ctypes.POINTER(_i64), ctypes.POINTER(_i64)]),
     "vh_checkpoint8": (_int, [_vp, _i64, _i64, _i64, _int, _vp, _vp, _vp]),
     "vh_checkpoint8_restore": (_int, [_vp, _vp, _i64, _i64, _int, _vp, _vp]),

@@ -1088,11 +1088,15 @@ static void adapter_first(const AdapterGradArgs& a, hipStream_t s) {
 }
 template <class T, int RT, int PP>
 static void adapter_grads_rank(const AdapterGradArgs& a, hipStream_t s) {
-    // Few waves (up to 4096: a quarter of what the chip holds): the workgroup's four share a tile's rows, so that a group's rows are four
-    // round trips fewer.  Many: a wave a tile, nothing to add up.  (200 groups, 8192 rows, K = N = 512: 20 us against 28)
     const int64_t tiles = ceil_div(a.K, 128) + ceil_div(a.N, 128);
-    if (grad_waves(a.ps, a.N, a.K) == 4) adapter_grad_kernel<T, RT, 2, 4, PP><<<dim3((unsigned)a.ps.items, (unsigned)tiles), 256, 0, s>>>(a);
-    else adapter_grad_kernel<T, RT, 2, 1, PP><<<dim3((unsigned)a.ps.items, (unsigned)ceil_div(tiles, 4)), 256, 0, s>>>(a);
+    if constexpr (RT < 4) {
+        if (grad_waves(a.ps, a.N, a.K, a.rank) == 4) {
+            adapter_grad_kernel<T, RT, 2, 4, PP><<<dim3((unsigned)a.ps.items, (unsigned)tiles), 256, 0, s>>>(a);
+            VH_HIP(hipGetLastError());
+            return;
+        }
+    }
+    adapter_grad_kernel<T, RT, 2, 1, PP><<<dim3((unsigned)a.ps.items, (unsigned)ceil_div(tiles, 4)), 256, 0, s>>>(a);
     VH_HIP(hipGetLastError());
 }
 template <class T, int PP>
@@ -1408,12 +1412,13 @@ int vh_adapt_backward(const vh_adapt_layer* l, const void* dy, int64_t lddy, con
     });
 }
 
-int vh_debug_adapt_choice(int64_t rows, int64_t groups, int64_t n, int64_t k, int dtype, int* forward_tile, int* backward_tile, int* waves) {
+int vh_debug_adapt_choice(int64_t rows, int64_t groups, int64_t n, int64_t k, int64_t rank, int dtype, int* forward_tile, int* backward_tile, int* waves) {
     return guarded([&] {
         check_rows(rows);
         check_groups(groups);
         check_width(n, "n");
         check_width(k, "k");
+        check_rank(rank);
         check_dtype(dtype);
         check_ptr(forward_tile, "forward_tile");
         check_ptr(backward_tile, "backward_tile");
@@ -1421,7 +1426,7 @@ int vh_debug_adapt_choice(int64_t rows, int64_t groups, int64_t n, int64_t k, in
         const PlanShape ps = plan_shape(rows, groups);
         *forward_tile = linear_tile(ps.subs, n, dtype == VH_F32);
         *backward_tile = linear_tile(ps.subs, k, dtype == VH_F32);
-        *waves = grad_waves(ps, n, k);
+        *waves = grad_waves(ps, n, k, rank);
     });
 }
 

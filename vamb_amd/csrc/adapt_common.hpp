@@ -258,7 +258,9 @@ inline PlanShape plan_shape(int64_t rows, int64_t groups) {
     s.subs = rows / 16 + runs;
     s.slots = 16 * s.subs;
     int64_t ir = (rows / 512 + 15) / 16 * 16;
-    const int64_t least = groups < 128 ? 128 : 512;   // (few groups: more pieces, many: fewer parts to join)
+    // (few groups: more pieces, many: fewer parts to join.  Gradients and join, 512 + 512 columns, bf16, pieces of 128 / 512 rows: 65536 rows of
+    // 100 groups 60 / 107 us, 32768 of 50 36 / 45, 2048 of 10 9 / 11; 32768 of 200 45 / 40, 65536 of 300 67 / 60)
+    const int64_t least = groups < 128 ? 128 : 512;
     s.item_rows = ir < least ? least : ir;
     s.items = groups + rows / s.item_rows;
     s.multis = rows / s.item_rows + 1;
@@ -292,8 +294,13 @@ inline int linear_tile(int64_t subs, int64_t n, bool f32) {
     if (n <= 32 || (subs + 3) / 4 * ((n + 31) / 32) <= 320) return kTileNarrow;
     return f32 || n <= 128 || (subs + 15) / 16 * ((n + 255) / 256) < 256 ? kTileMid : kTileWide;
 }
-// waves that share a tile of the adapters' gradients
-inline int grad_waves(const PlanShape& ps, int64_t n, int64_t k) { return ps.items * ((k + 127) / 128 + (n + 127) / 128) < 4096 ? 4 : 1; }
+// Waves that share a tile (an item, 128 columns) of the adapters' gradients.  Few tiles: four, so that an item's rows are a quarter of the round trips.
+// Many, or ranks above 32 (whose sums fill the registers): one, with nothing to add up.  8192 rows, 512 + 512 columns, rank 16, bf16, four
+// against one: 50 groups (912 tiles) 15.3 / 20.7 us, 200 groups (1728) 16.8 / 13.5, 1000 groups (8128) 40 / 16; float32 of 4096 rows, rank 8, 50 groups (656)
+// 8.2 / 14.0; rank 64, 2331 rows of 107 groups, 256 + 512 columns (750) 24.5 / 11.8.
+inline int grad_waves(const PlanShape& ps, int64_t n, int64_t k, int64_t rank) {
+    return rank <= 32 && ps.items * ((k + 127) / 128 + (n + 127) / 128) < 1024 ? 4 : 1;
+}
 
 // ---- arguments of the shared-projection kernel (adapt_linear.hpp) -----------------------------------------------------------------
 struct LinArgs {
