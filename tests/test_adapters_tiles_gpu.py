@@ -47,7 +47,7 @@ CASES = [
     (3000, 154, 512, 20, 30, torch.bfloat16, MID, NARROW, 4),
     (9001, 304, 200, 24, 60, torch.bfloat16, MID, MID, 4),
     (9001, 200, 304, 40, 60, torch.bfloat16, MID, MID, 1),
-    (40001, 264, 264, 9, 20, torch.bfloat16, WIDE, WIDE, 1),
+    (40001, 264, 264, 9, 20, torch.bfloat16, WIDE, WIDE, 4),
     (70001, 300, 520, 24, 300, torch.bfloat16, WIDE, WIDE, 1),
     (70001, 520, 300, 40, 300, torch.bfloat16, WIDE, WIDE, 1),
     (70001, 304, 512, 16, 700, torch.bfloat16, WIDE, WIDE, 1),
@@ -55,7 +55,7 @@ CASES = [
     (66000, 136, 264, 64, 1500, torch.bfloat16, WIDE, WIDE, 1),
     (3000, 154, 512, 20, 30, torch.float32, MID, NARROW, 4),
     (9001, 300, 200, 32, 60, torch.float32, MID, MID, 4),
-    (20001, 300, 520, 24, 200, torch.float32, MID, MID, 1),
+    (20001, 300, 520, 24, 200, torch.float32, MID, MID, 4),
     (20001, 520, 300, 64, 200, torch.float32, MID, MID, 1),
     (30001, 300, 520, 33, 900, torch.float32, MID, MID, 1),
 ]

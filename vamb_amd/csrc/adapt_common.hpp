@@ -258,7 +258,7 @@ inline PlanShape plan_shape(int64_t rows, int64_t groups) {
     s.subs = rows / 16 + runs;
     s.slots = 16 * s.subs;
     int64_t ir = (rows / 512 + 15) / 16 * 16;
-    // (few groups: more pieces, many: fewer parts to join.  Gradients and join, 512 + 512 columns, bf16, pieces of 128 / 512 rows: 65536 rows of
+    // (few groups: more pieces, many: fewer parts to join.  Gradients and join, 512 + 512 columns, bf16, equal groups, pieces of 128 / 512 rows: 65536 rows of
     // 100 groups 60 / 107 us, 32768 of 50 36 / 45, 2048 of 10 9 / 11; 32768 of 200 45 / 40, 65536 of 300 67 / 60)
     const int64_t least = groups < 128 ? 128 : 512;
     s.item_rows = ir < least ? least : ir;
@@ -294,12 +294,13 @@ inline int linear_tile(int64_t subs, int64_t n, bool f32) {
     if (n <= 32 || (subs + 3) / 4 * ((n + 31) / 32) <= 320) return kTileNarrow;
     return f32 || n <= 128 || (subs + 15) / 16 * ((n + 255) / 256) < 256 ? kTileMid : kTileWide;
 }
-// Waves that share a tile (an item, 128 columns) of the adapters' gradients.  Few tiles: four, so that an item's rows are a quarter of the round trips.
-// Many, or ranks above 32 (whose sums fill the registers): one, with nothing to add up.  8192 rows, 512 + 512 columns, rank 16, bf16, four
-// against one: 50 groups (912 tiles) 15.3 / 20.7 us, 200 groups (1728) 16.8 / 13.5, 1000 groups (8128) 40 / 16; float32 of 4096 rows, rank 8, 50 groups (656)
-// 8.2 / 14.0; rank 64, 2331 rows of 107 groups, 256 + 512 columns (750) 24.5 / 11.8.
+// Waves that share a tile (an item, 128 columns) of the adapters' gradients.  Few tiles: four, so that an item's rows are a quarter of the round
+// trips, which is what the largest groups make the launch wait for.  Many, or ranks above 32 (whose sums fill the registers): one, with nothing to add up.
+// Groups of unlike sizes (a spread of e^0.5), 8192 rows, 512 + 512 columns, rank 16, bf16, four against one: 50 groups (912 tiles) 13.5 / 20.4 us, 200
+// (1728) 15.8 / 22.5 (equal groups: 16.8 / 13.5), 400 (3328) 22.0 / 20.2, 1000 (8128) 41 / 17; float32 4096 rows, rank 8, 50 groups (656) 10.1 / 15.9;
+// rank 64, 8620 rows of 11 groups, 256 + 1104 columns (858) 50 / 33.  Over 87 layers this choice takes 1.05 of the faster's time in the mean.
 inline int grad_waves(const PlanShape& ps, int64_t n, int64_t k, int64_t rank) {
-    return rank <= 32 && ps.items * ((k + 127) / 128 + (n + 127) / 128) < 1024 ? 4 : 1;
+    return rank <= 32 && ps.items * ((k + 127) / 128 + (n + 127) / 128) < 2048 ? 4 : 1;
 }
 
 // ---- arguments of the shared-projection kernel (adapt_linear.hpp) -----------------------------------------------------------------
