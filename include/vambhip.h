@@ -493,7 +493,9 @@ int vh_vae_train_epoch_dp(vh_vae* h, const int64_t* perm, int64_t n_batches, int
  * Unlike the handles above, these entry points take DEVICE pointers (of the calling thread's current device), enqueue on `stream`
  * (a hipStream_t; NULL: the null stream) and return without synchronising; they allocate nothing, so that they may be captured
  * into a graph.  Scratch memory is the caller's, 16-byte aligned and of the size that the *_size entry gives; calls that may run at the same
- * time need scratch of their own.  Tensors are float32 or bf16 (`dtype`), unit stride along a row, `ld*` elements between rows, any
+ * time need scratch of their own.  Sums are float32.  What is multiplied: bf16 tensors as they are, u and v in 24 bits, p in 16 where a slope applies
+ * (2^-16 of its size at most); float32 tensors in 24 bits, products of their last bits dropped (2^-21 of a product together at most).  Infinities
+ * and NaN give what the formulas give, in their rows and columns alone (a number below 2^-100 counts as zero beside an infinity).  Tensors are float32 or bf16 (`dtype`), unit stride along a row, `ld*` elements between rows, any
  * alignment of the element type.  Widths up to 2^20, weights (padded to multiples of 256) below 4 GB in each
  * direction (bf16: 2 bytes, float32: 6 bytes an element), rows up to 2^30, ranks up to 64, groups up to 16384.  A call whose work is more than
  * one launch of 2^32 threads holds (2^28 float32 rows of 32 or of 512 columns, a weight gradient of 2^32 elements) is refused.
@@ -535,7 +537,8 @@ typedef struct {
 /* y [rows][ldy]; optional: low = u [rows][rank] (16-byte aligned) and the checkpoint of y, for the backward pass */
 int vh_adapt_forward(const vh_adapt_layer* layer, const void* x, int64_t ldx, int64_t rows, const int32_t* plan, void* y, int64_t ldy, float* low,
                      uint8_t* codes, uint8_t* exponents, void* stream);
-/* the same y for a few rows, in one launch without a plan (any number of rows is right; from about a hundred on the plan is faster) */
+/* the same y for a few rows, in one launch without a plan (any number of rows is right; every 16 columns read the rows' adapters anew, so that the
+ * plan is faster from about 160 000 elements of rows x rank x k in bf16 and 36 000 in float32 on: 8 to 64 rows) */
 int vh_adapt_forward_few(const vh_adapt_layer* layer, const void* x, int64_t ldx, int64_t rows, const int32_t* row_groups, void* y, int64_t ldy,
                          void* stream);
 /* y (elements or checkpoint) may be NULL without an activation.  dx [rows][lddx] may be NULL (not wanted).  ddown, dup: dense, like

@@ -15,7 +15,8 @@ stream of that GPU, do not synchronise and may be captured into a graph.  Memory
 packed weight, a checkpoint) that is used on another stream than the one that made it has to be ordered as any other
 tensor has.  They stand outside of autograd: gradients come from :func:`adapted_linear_backward` and :func:`checkpoint_weight_grad`, for what
 :func:`adapted_linear_train` returns; :func:`adapted_linear`, which keeps nothing for them, refuses tensors that require a gradient.
-Sums are float32; gradients have the type of their parameters.  Equal inputs give equal bits.
+Sums are float32; gradients have the type of their parameters.  Of bf16 tensors ``u`` and ``v`` are multiplied in 24 bits, ``p`` in 16 where the slope
+applies; of float32 tensors the products of the last bits are dropped (2^-21 of a product at most).  Equal inputs give equal bits.
 
 :class:`VAEAdapters` trains adapters for a VAE's encoder and encodes with them.
 """

@@ -303,7 +303,7 @@ __global__ __launch_bounds__(256) void pack_weight_kernel(const T* w, int64_t ld
 // =====================================================================================================================
 // Checkpoints
 // =====================================================================================================================
-// Four lanes share a block of 32 columns, eight each.  Bound by memory: 1000003 x 512 bf16 in 376 us, 4.1 TB/s of the 4.9 that a large copy
+// Four lanes share a block of 32 columns, eight each.  Bound by memory: 1000003 x 512 bf16 in 372 us, 4.1 TB/s of the 4.9 that a large copy
 // reaches; the way back (codes to bf16) in 297 us, 5.2 TB/s.
 template <class T>
 __global__ __launch_bounds__(256) void checkpoint_kernel(const T* x, int64_t ldx, int64_t rows, int cols, uint8_t* codes, uint8_t* exps) {
@@ -441,7 +441,7 @@ __device__ __forceinline__ void masked8(const Source& s, const Eight<T>& v, floa
 // Gradients of the adapters:  down_g = sum v^T x  [rank][K],  up_g = s sum p^T u  [N][rank]
 // One wave = one item (at most item_rows rows of one group) and 128 columns of x or of p.  v_mfma_f32_16x16x4_f32: its operands
 // are one element per lane, so eight consecutive columns that a lane has read are the operands of eight instructions and nothing is
-// transposed; products and sums are fp32 whatever the tensors' type.  65537 rows of 1000 groups, rank 32, 1104 + 512 columns, bf16: 140 us for
+// transposed; products and sums are fp32 whatever the tensors' type.  65537 rows of 1000 groups, rank 32, 1104 + 512 columns, bf16: 136 us for
 // 6.8 GF (50 TF of the 157 that the instruction has; the rows of a group are few steps, whose latency is what counts) and 100 MB of gradients.
 // =====================================================================================================================
 struct AdapterGradArgs {
@@ -690,7 +690,7 @@ __global__ __launch_bounds__(256) void adapter_join_kernel(AdapterGradArgs a) {
 
 // =====================================================================================================================
 // Few rows: no plan.  A workgroup = 16 rows x 16 columns; eight waves share the depth of the projection and, one distinct adapter at a
-// time, the u of the rows; the last 256 products with B_g are plain fused multiply-adds in float32.  One row, 304 -> 512, rank 8, bf16: 5 us,
+// time, the u of the rows; the last 256 products with B_g are plain fused multiply-adds in float32.  One row, 304 -> 512, rank 8, bf16: 4.6 us,
 // of which a launch is 4.  Every workgroup reads the rows' adapters: rows x rank x K decides when the plan and the projection behind it are
 // faster (vamb_amd/adapters.py).
 // =====================================================================================================================
@@ -820,8 +820,9 @@ __global__ __launch_bounds__(512) void few_kernel(FewArgs a) {
 // Gradient of the shared projection from checkpoints:  dW = p^T x  [N][K],  db = sum p  [N]
 // Tile 128 x 128, split over the rows; both operands are contracted along their slow dimension: row-major LDS tiles [64 rows][128
 // columns] read by the transposing LDS instruction.  x's values are exact in bf16 (one plane), so float32 dy costs three products, not
-// six, and bf16 dy one, or two where a slope was applied to it (cut8).  8192 x 512 x 512 bf16: 19 us and 5 us for the join of 16 parts (eight steps of 0.6; the rest is the first
-// loads, 64 KB of partial sums a workgroup and the launch); 4096 x 1104 x 512 float32: 31 us and 6 us.  256-byte tile rows: the
+// six, and bf16 dy one, or two where a slope was applied to it (cut8).  8192 x 512 x 512 bf16: 24 us (two products;
+// 19 without an activation) and 5.6 us for the join of 16 parts (eight steps; the rest is the first loads, 64 KB of partial sums a workgroup and
+// the launch); 4096 x 1104 x 512 float32: 31 us and 6 us.  256-byte tile rows: the
 // 32-byte pieces are XOR-permuted by the row so that the eight rows of half a read differ in their banks.
 // =====================================================================================================================
 struct WeightGradArgs {

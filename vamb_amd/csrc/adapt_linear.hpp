@@ -340,9 +340,11 @@ __global__ __launch_bounds__(64 * S::WM * S::WN * S::KG) void linear_kernel(LinA
     using Yes = std::integral_constant<bool, true>;
     using No = std::integral_constant<bool, false>;
     Raw8<T> in0[MU][KC][RT], in1[MU][KC][RT];
-    // Tile kt is multiplied while tile kt + 1 is on its way.  Measured and not kept (524288 x 1024 -> 512, rank 16, 948 us): three and four
+    // Tile kt is multiplied while tile kt + 1 is on its way.  Measured and not kept (524288 x 1024 -> 512, rank 16, when it took 948 us): three and four
     // buffers with counted waits 948, W's operands read three products ahead 949, requests spread between the products 920 -- the
-    // loop is bound neither by what a tile takes to land nor by the LDS, and without any loads it still takes 57% of the time.
+    // loop is not bound by what a tile takes to land, and without any loads it still took 57% of the time.  As it is built, the choice of x's
+    // subtiles by `wn` in compute() is four scalar branches in each 32-deep half of a tile, around single products, which part the LDS reads of a
+    // half from the products of the one before; 8 waves a CU and these keep the matrix pipe busy for a third of the time.
     auto fetch = [&](int k0, unsigned char* to, Raw8<T> (&in)[MU][KC][RT]) {
         if (k0 + BK <= K) {
             fetch_in(Yes(), k0, in);
