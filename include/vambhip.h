@@ -537,8 +537,8 @@ typedef struct {
 /* y [rows][ldy]; optional: low = u [rows][rank] (16-byte aligned) and the checkpoint of y, for the backward pass */
 int vh_adapt_forward(const vh_adapt_layer* layer, const void* x, int64_t ldx, int64_t rows, const int32_t* plan, void* y, int64_t ldy, float* low,
                      uint8_t* codes, uint8_t* exponents, void* stream);
-/* the same y for a few rows, in one launch without a plan (any number of rows is right; every 16 columns read the rows' adapters anew, so that the
- * plan is faster from about 160 000 elements of rows x rank x k in bf16 and 36 000 in float32 on: 8 to 64 rows) */
+/* the same y for a few rows, in one launch without a plan (any number of rows is right; every 16 rows and 16 columns read their adapters anew, so
+ * that the plan is faster from 10 to 16 rows of unlike adapters on, or from some hundred of one adapter: vamb_amd/adapters.py has the measured rule) */
 int vh_adapt_forward_few(const vh_adapt_layer* layer, const void* x, int64_t ldx, int64_t rows, const int32_t* row_groups, void* y, int64_t ldy,
                          void* stream);
 /* y (elements or checkpoint) may be NULL without an activation.  dx [rows][lddx] may be NULL (not wanted).  ddown, dup: dense, like

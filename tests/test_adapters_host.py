@@ -237,3 +237,12 @@ def test_c_entries_refuse_what_no_launch_holds():
     ]:
         with pytest.raises(ValueError, match=why + ".*one launch"):
             _lib.check(call())
+
+
+@pytest.mark.parametrize("dtype,rows,k,n,rank,groups,few", [
+    (torch.bfloat16, 64, 304, 512, 8, 4, True), (torch.bfloat16, 5000, 32, 512, 1, 200, False), (torch.bfloat16, 16, 1104, 512, 16, 200, False),
+    (torch.bfloat16, 14, 304, 512, 8, 200, True), (torch.float32, 17, 512, 512, 1, 200, False), (torch.float32, 3, 304, 512, 8, 200, True),
+    (torch.bfloat16, 312, 512, 512, 1, 200, False), (torch.bfloat16, 2500, 64, 1104, 1, 1, False)])
+def test_calls_that_go_without_a_plan(dtype, rows, k, n, rank, groups, few):
+    """The measured side of each (adapters.py): what a workgroup reads counts, not the rows' elements alone."""
+    assert (ad._few_cost(rows, n, k, rank, groups) <= ad._FEW[dtype]) == few

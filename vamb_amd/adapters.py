@@ -34,11 +34,18 @@ from . import _lib
 MAX_RANK = 64
 MAX_GROUPS = 16384
 BLOCK = 32   # columns of a checkpoint that share an exponent
-# Up to so many elements of adapters that the rows of a call ask for (rows x rank x k), adapted_linear goes without a plan: one launch, in
-# which every 16 columns read them anew.  Measured, that launch against plan and projection: bf16 304 -> 512, rank 8, 64 rows (156 k) 9.3 us
-# against 10.7; 1104 -> 512, rank 16, 8 rows (141 k) 11.8 / 13.5, 16 rows (283 k) 23 / 14; float32 (six products for one) 304 -> 512,
-# rank 8, 8 rows (19 k) 10.4 / 13.3, 16 rows (39 k) 17 / 13.5.  One or two rows always (512 -> 512, rank 64, one row: bf16 8 / 13, float32 12 / 26).
-_FEW = {_torch.bfloat16: 160_000, _torch.float32: 36_000}
+# Up to this cost adapted_linear goes without a plan: one launch, in which each workgroup (16 rows, 16 columns) reads the adapters of its rows.
+# Cost = (adapters that 16 rows can have x pieces of 16 ranks x k + 1000) x rounds of 256 workgroups.  Times of a call, that launch against
+# plan and projection: bf16 304 -> 512, rank 8, 64 rows of 200 groups 10 us / 16 (cost 5900); 1104 -> 512, rank 16, 8 rows of 200 groups 13 / 16 (9800), 16 rows
+# 23 / 16 (18700); 32 -> 512, rank 1, 5000 rows of 200 groups 54 / 16 (59000); float32 (six products for one) 512 -> 512, rank 1, 8 rows of 200 groups 15 / 17
+# (5100), 17 rows 27 / 17 (9200).  Over 420 drawn calls this takes 1.004 of the faster way's time in the mean, 1.54 at worst.  One or two rows always
+# (512 -> 512, rank 64, one row: bf16 9.3 / 15, float32 12 / 29).
+_FEW = {_torch.bfloat16: 12_000, _torch.float32: 8_000}
+
+
+def _few_cost(rows: int, n: int, k: int, rank: int, groups: int) -> float:
+    return (min(16, rows, groups) * -(-rank // 16) * k + 1000) * max(1.0, -(-rows // 16) * -(-n // 16) / 256)
+
 
 _DTYPES = {_torch.float32: 0, _torch.bfloat16: 1}
 # the current stream's handle without a Stream object around it (a call here is a few microseconds in all)
@@ -243,7 +250,7 @@ def adapted_linear(x, shared: SharedProjection, down, up, groups: Union[_torch.T
         y = x.new_empty((rows, shared.n))
         if rows == 0:
             return y
-        if not planned and (rows <= 2 or rows * down.shape[1] * shared.k <= _FEW[x.dtype]):
+        if not planned and (rows <= 2 or _few_cost(rows, shared.n, shared.k, down.shape[1], n_groups) <= _FEW[x.dtype]):
             _lib.check(lib.vh_adapt_forward_few(layer, x.data_ptr(), ld, rows, groups.data_ptr(), y.data_ptr(), shared.n, stream))
             return y
         if not planned:
