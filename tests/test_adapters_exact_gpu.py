@@ -156,7 +156,6 @@ def run_infinities(ad, dtype, exact, places, slope=0.01):
         if name == "x":
             r, k = at
             reach([r], every)
-            bw["dx"] += []
             if of[r] >= 0:
                 fw["low"].append((r,))
                 bw["ddown"].append((int(of[r]), every, k))
